@@ -1,0 +1,511 @@
+// Backward of the attention operators (include/ekaid_hip.h: ekaid_attn_t).  Scores are formed again from q, k and the stored log2
+// denominators; two kernels, so that no output is an atomic target: dq (and the bias table) with one workgroup per block of query rows,
+// dk / dv with one per block of keys, walking the rows of every head that shares them.
+#include "attn.h"
+#include <algorithm>
+
+namespace ekaid {
+
+// f16 only: powers of two that keep the score gradients P (dP - delta) inside the f16 range whatever the scale of the incoming gradient
+// (a loss divided by thousands of tokens): |dP_ij| <= |dout_i| |v_j|, so |dout_i| is brought to ~2^4.  Exact, taken out in f32.
+template <typename T> __device__ __forceinline__ float ds_scale(float norm2) {
+    if constexpr (__is_same(T, _Float16)) {
+        if (!(norm2 > 0.f) || norm2 == POS_INF) return 1.f;
+        const int e = (int)((__builtin_bit_cast(uint32_t, norm2) >> 23) & 255) - 127;      // norm^2 in [2^e, 2^(e+1))
+        const int k = 4 - (e >> 1);
+        return ldexpf(1.f, k < -60 ? -60 : k > 60 ? 60 : k);
+    } else return 1.f;
+}
+
+template <typename T, int DH, int G, int NW, int KT, bool REL>
+__global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
+    constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
+    constexpr int LD = Ld<T, DH>::row, nq = Blk<G>::nq, ng = Blk<G>::ng;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* Ks = reinterpret_cast<T*>(smem);
+    T* Vs = Ks + KT * LD;
+    unsigned char* kms = reinterpret_cast<unsigned char*>(Vs + KT * LD);
+    float* red = reinterpret_cast<float*>(kms + KT);          // [NW] row-norm maxima
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
+    float* bias = red + NW;                                   // [width]
+    float* dsum = bias + width;                               // [NW][width]: this wave's sums of score gradients by distance
+    float* skew = dsum + NW * width + wave * G * (G + 1);     // [NW][G][G + 1]
+    const RowWork w(a);
+    const ekaid_attn_t& d = a.d;
+    const int h = w.head0, row0 = (w.tile * NW + wave) * G, i0 = row0 + lane % G;
+    const bool ok = i0 < d.Lq;
+    const int i = ok ? i0 : 0, p0 = query_pos(d, w.b), pos = p0 + i0, len = key_len(d, w.b);
+    int kend = len;
+    if (d.causal) kend = max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G)));
+    const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
+    const unsigned char* mask = d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr;
+    if constexpr (REL) {
+        fill_bias(d, bias, h, 1, tid, NT);
+        for (int x = tid; x < NW * width; x += NT) dsum[x] = 0.f;
+    }
+
+    u32x4 qf[NC], gf[NC];
+    const long long orow = ((long long)w.b * d.Lq + i) * d.H * d.dh + (long long)h * d.dh;
+    const T* qrow = reinterpret_cast<const T*>(d.q) + w.b * d.q_batch + i * d.q_row + (long long)h * d.dh;
+    const T* grow = reinterpret_cast<const T*>(d.dout) + orow;
+    const T* yrow = reinterpret_cast<const T*>(d.out) + orow;
+    float delta = 0.f, n2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        qf[c] = row_frag_global<T, G>(qrow, c, d.dh, ok, lane);
+        gf[c] = row_frag_global<T, G>(grow, c, d.dh, ok, lane);
+        const u32x4 y = row_frag_global<T, G>(yrow, c, d.dh, ok, lane);
+#pragma unroll
+        for (int e = 0; e < Elem<T>::epl; ++e) {
+            const float x = elem<T>(gf[c], e);
+            delta += x * elem<T>(y, e);
+            n2 += x * x;
+        }
+    }
+    delta = across_groups_sum<G>(delta);
+    n2 = across_groups_sum<G>(n2);
+    const long long srow = ((long long)w.b * d.H + h) * d.Lq + i;
+    const float lse = ok ? d.lse[srow] : POS_INF;
+    if (ok && g == 0 && w.split == 0) a.delta[srow] = delta;
+    const float rs = ds_scale<T>(n2);
+    if constexpr (__is_same(T, _Float16)) {
+        float mx = wave_max(n2);
+        if (lane == 0) red[wave] = mx;
+    }
+
+    const T* kb = reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh;
+    const T* vb = reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh;
+    Stage<T, DH, KT, NT> sk, sv;
+    typename Blk<G>::acc o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
+    float far_back = 0.f, far_ahead = 0.f;
+    if (t0 < t1) {
+        sk.load(kb, d.k_row, t0 * KT, len, d.dh, mask, tid);
+        sv.load(vb, d.v_row, t0 * KT, len, d.dh, mask, tid);
+    }
+    for (int t = t0; t < t1; ++t) {
+        sk.store(Ks, LD, tid);
+        sv.store(Vs, LD, tid);
+        if (mask) for (int j = tid; j < KT; j += NT) kms[j] = t * KT + j < len ? mask[t * KT + j] : 0;
+        __syncthreads();
+        if (t + 1 < t1) {
+            sk.load(kb, d.k_row, (t + 1) * KT, len, d.dh, mask, tid);
+            sv.load(vb, d.v_row, (t + 1) * KT, len, d.dh, mask, tid);
+        }
+        typename Blk<G>::acc s[NB], dp[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            s[b] = zero_acc<G>();
+            dp[b] = zero_acc<G>();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s[b] = mma<T, G>(row_frag<T, G>(Ks, LD, b * G, c, lane), qf[c], s[b]);
+                dp[b] = mma<T, G>(row_frag<T, G>(Vs, LD, b * G, c, lane), gf[c], dp[b]);
+            }
+        }
+        const bool partial = mask || (t + 1) * KT > len || (d.causal && (t + 1) * KT > p0 + w.tile * NW * G + 1);
+        finish_scores<G, NB>(a, s, t * KT, len, pos, REL ? bias : nullptr, mask ? kms : nullptr, partial, lane);
+        if (d.drop_p > 0.f) {
+            const uint64_t seed = drop_seed_value(a.seed);
+#pragma unroll
+            for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    dp[q / nq][4 * (q % nq) + e] *= drop_keep(a, seed, w.b, h, i, t * KT + 4 * ng * q + 4 * g + e);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4 * nq; ++r) {
+                const float p = __builtin_amdgcn_exp2f(s[b][r] - lse);
+                s[b][r] = p == 0.f ? 0.f : p * (dp[b][r] - delta);
+            }
+        if constexpr (REL) {
+            // sums over equal distance j - pos: a block that lies wholly beyond the reach goes to one bucket; otherwise the block is written
+            // to LDS and lane x adds up diagonal x (rows ascending: a fixed order), whose distance no other lane of the wave holds
+            const int prow = p0 + row0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int jb = t * KT + b * G;
+                if (jb + G - 1 - prow <= -d.reach || jb - (prow + G - 1) >= d.reach) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 4 * nq; ++r) x += s[b][r];
+                    if (jb - prow < 0) far_back += x; else far_ahead += x;
+                } else {
+                    wave_fence();
+#pragma unroll
+                    for (int q = 0; q < nq; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) skew[(lane % G) * (G + 1) + 4 * ng * q + 4 * g + e] = s[b][4 * q + e];
+                    wave_fence();
+                    if (lane < 2 * G - 1) {
+                        const int off = lane - (G - 1);
+                        float x = 0.f;
+#pragma unroll 8
+                        for (int r = 0; r < G; ++r) {
+                            const int c = r + off;
+                            x += (c >= 0 && c < G) ? skew[r * (G + 1) + c] : 0.f;
+                        }
+                        const int rel = jb - prow + off;
+                        if (rel <= -d.reach) far_back += x;
+                        else if (rel >= d.reach) far_ahead += x;
+                        else dsum[wave * width + rel + d.reach] += x;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4 * nq; ++r) s[b][r] *= rs;
+#pragma unroll
+        for (int c = 0; c < PC; ++c) {
+            const u32x4 sf = score_frag<T, G, NB>(s, c);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) o[mt] = mma<T, G>(col_frag<T, G>(Ks, LD, mt * G, c, lane), sf, o[mt]);
+        }
+        __syncthreads();
+    }
+    if constexpr (REL) {
+        __syncthreads();                                      // (a workgroup without a key tile has not met its own zeroing yet)
+        far_back = wave_sum(far_back);
+        far_ahead = wave_sum(far_ahead);
+        if (lane == 0) {
+            dsum[wave * width] = far_back;
+            dsum[wave * width + 2 * d.reach] = far_ahead;
+        }
+        __syncthreads();
+        // distances of one bucket are summed in ascending order by one thread
+        const int nb = (d.n_border + 1) * (d.bidirectional ? 2 : 1);
+        float* part = a.ptab + ((long long)(w.b * d.H + h) * a.dq_parts + w.tile * a.splits + w.split) * nb;
+        for (int c = tid; c < nb; c += NT) {
+            float x = 0.f;
+            const int side = c / (d.n_border + 1), lo = c % (d.n_border + 1) ? d.border[c % (d.n_border + 1) - 1] : 0,
+                      hi = c % (d.n_border + 1) == d.n_border ? d.reach : d.border[c % (d.n_border + 1)] - 1;
+            for (int wv = 0; wv < NW; ++wv) {
+                const float* ds = dsum + wv * width + d.reach;
+                if (d.bidirectional && side) for (int r = max(lo, 1); r <= hi; ++r) x += ds[r];
+                else for (int r = lo; r <= hi; ++r) x += ds[-r];
+                if (!d.bidirectional && c == 0) for (int r = 1; r <= d.reach; ++r) x += ds[r];
+            }
+            part[c] = x;
+        }
+    }
+    if constexpr (__is_same(T, _Float16)) {
+        __syncthreads();
+        if (tid == 0) {
+            float mx = red[0];
+            for (int x = 1; x < NW; ++x) mx = fmaxf(mx, red[x]);
+            a.nrm[(long long)(w.b * d.H + h) * a.dq_parts + w.tile * a.splits + w.split] = mx;
+        }
+    }
+    if (!ok) return;
+    const float f = d.scale / rs;
+    if (a.splits > 1) {
+        float* p = a.po + w.split * ((long long)d.B * d.Lq * d.H * d.dh) + orow;
+#pragma unroll
+        for (int q = 0; q < MT * nq; ++q) {
+            const int col = 4 * ng * q + 4 * g;
+            const auto& x = o[q / nq];
+            if (col < d.dh) store4<float>(p + col, x[4 * (q % nq)] * f, x[4 * (q % nq) + 1] * f, x[4 * (q % nq) + 2] * f, x[4 * (q % nq) + 3] * f);
+        }
+    } else {
+        T* p = reinterpret_cast<T*>(d.dq) + orow;
+#pragma unroll
+        for (int q = 0; q < MT * nq; ++q) {
+            const int col = 4 * ng * q + 4 * g;
+            const auto& x = o[q / nq];
+            if (col < d.dh) store4<T>(p + col, x[4 * (q % nq)] * f, x[4 * (q % nq) + 1] * f, x[4 * (q % nq) + 2] * f, x[4 * (q % nq) + 3] * f);
+        }
+    }
+}
+
+template <typename T, int DH, int G, int NW, int QT>
+__global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(const AttnArgs a) {
+    constexpr int NT = 64 * NW, NB = QT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = QT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
+    constexpr int LD = Ld<T, DH>::row, nq = Blk<G>::nq, ng = Blk<G>::ng;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* Qs = reinterpret_cast<T*>(smem);
+    T* Ds = Qs + QT * LD;
+    float* ls = reinterpret_cast<float*>(Ds + QT * LD);       // [QT] log2 denominators (+inf: no such row)
+    float* dl = ls + QT;                                      // [QT] delta
+    float* bias = dl + QT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G;
+    const ekaid_attn_t& d = a.d;
+    const int wi = die_order(blockIdx.x, gridDim.x), tile = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
+    const int b = bk / d.KV, kvh = bk % d.KV, group = d.H / d.KV;
+    const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tile * NW * G, j = j0 + wave * G + lane % G;
+    const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
+    const bool ok = j < len && (!mask || mask[j]);
+    const int qtiles = (d.Lq + QT - 1) / QT, first = d.causal ? min(qtiles, max(0, j0 - p0) / QT) : 0, live = qtiles - first;
+    const int items = j0 < len ? group * live : 0, per = (items + a.splits - 1) / a.splits, t0 = split * per, t1 = min(items, t0 + per);
+
+    u32x4 kf[NC], vf[NC];
+    const int jr = ok ? j : 0;
+    const T* krow = reinterpret_cast<const T*>(d.k) + b * d.k_batch + jr * d.k_row + (long long)kvh * d.dh;
+    const T* vrow = reinterpret_cast<const T*>(d.v) + b * d.v_batch + jr * d.v_row + (long long)kvh * d.dh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        kf[c] = row_frag_global<T, G>(krow, c, d.dh, ok, lane);
+        vf[c] = row_frag_global<T, G>(vrow, c, d.dh, ok, lane);
+    }
+    float rs = 1.f;
+    if constexpr (__is_same(T, _Float16)) {                   // the largest |dout| row of the heads that share these keys
+        float mx = 0.f;
+        const float* n = a.nrm + (long long)(b * d.H + kvh * group) * a.dq_parts;
+        for (int x = lane; x < group * a.dq_parts; x += 64) mx = fmaxf(mx, n[x]);
+        rs = ds_scale<T>(wave_max(mx));
+    }
+    typename Blk<G>::acc ok_[MT], ov[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        ok_[mt] = zero_acc<G>();
+        ov[mt] = zero_acc<G>();
+    }
+    Stage<T, DH, QT, NT> sq, sd;
+    auto fetch = [&](int t) {
+        const int h = kvh * group + t / live, q0 = (first + t % live) * QT;
+        sq.load(reinterpret_cast<const T*>(d.q) + b * d.q_batch + (long long)h * d.dh, d.q_row, q0, d.Lq, d.dh, nullptr, tid);
+        sd.load(reinterpret_cast<const T*>(d.dout) + (long long)b * d.Lq * d.H * d.dh + (long long)h * d.dh, (long long)d.H * d.dh, q0, d.Lq, d.dh,
+                nullptr, tid);
+    };
+    if (t0 < t1) fetch(t0);
+    int bias_head = -1;
+    for (int t = t0; t < t1; ++t) {
+        const int h = kvh * group + t / live, q0 = (first + t % live) * QT;
+        const long long srow = ((long long)b * d.H + h) * d.Lq;
+        sq.store(Qs, LD, tid);
+        sd.store(Ds, LD, tid);
+        for (int x = tid; x < QT; x += NT) {
+            ls[x] = q0 + x < d.Lq ? d.lse[srow + q0 + x] : POS_INF;
+            dl[x] = q0 + x < d.Lq ? a.delta[srow + q0 + x] : 0.f;
+        }
+        if (d.table && bias_head != h) {
+            fill_bias(d, bias, h, 1, tid, NT);
+            bias_head = h;
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        typename Blk<G>::acc s[NB], dp[NB];
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+            s[x] = zero_acc<G>();
+            dp[x] = zero_acc<G>();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s[x] = mma<T, G>(row_frag<T, G>(Qs, LD, x * G, c, lane), kf[c], s[x]);
+                dp[x] = mma<T, G>(row_frag<T, G>(Ds, LD, x * G, c, lane), vf[c], dp[x]);
+            }
+        }
+        const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
+#pragma unroll
+        for (int q = 0; q < NB * nq; ++q) {
+            const int iq = 4 * ng * q + 4 * g;
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + iq), d4 = *reinterpret_cast<const f32x4*>(dl + iq);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * (q % nq) + e, i = q0 + iq + e, rel = j - (p0 + i);
+                float x = s[q / nq][r] * a.sc2;
+                if (d.table) x += bias[min(max(rel, -d.reach), d.reach) + d.reach];
+                float p = __builtin_amdgcn_exp2f(x - l4[e]);
+                if (!ok || l4[e] == POS_INF || (d.causal && rel > 0)) p = 0.f;
+                float keep = 1.f;
+                if (d.drop_p > 0.f) keep = drop_keep(a, seed, b, h, i, j);
+                dp[q / nq][r] = p == 0.f ? 0.f : p * (dp[q / nq][r] * keep - d4[e]) * rs;
+                s[q / nq][r] = p * keep;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < PC; ++c) {
+            const u32x4 pf = score_frag<T, G, NB>(s, c), df = score_frag<T, G, NB>(dp, c);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                ov[mt] = mma<T, G>(col_frag<T, G>(Ds, LD, mt * G, c, lane), pf, ov[mt]);
+                ok_[mt] = mma<T, G>(col_frag<T, G>(Qs, LD, mt * G, c, lane), df, ok_[mt]);
+            }
+        }
+        __syncthreads();
+    }
+    if (j >= d.Lk) return;
+    const float f = d.scale / rs;
+    const long long row = ((long long)b * d.Lk + j) * d.KV * d.dh + (long long)kvh * d.dh;
+    const long long n = (long long)d.B * d.Lk * d.KV * d.dh;
+#pragma unroll
+    for (int q = 0; q < MT * nq; ++q) {
+        const int col = 4 * ng * q + 4 * g, r = 4 * (q % nq);
+        if (col >= d.dh) continue;
+        const auto& x = ok_[q / nq];
+        const auto& y = ov[q / nq];
+        if (a.splits > 1) {
+            store4<float>(a.pk + split * n + row + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
+            store4<float>(a.pv + split * n + row + col, y[r], y[r + 1], y[r + 2], y[r + 3]);
+        } else {
+            store4<T>(reinterpret_cast<T*>(d.dk) + row + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
+            store4<T>(reinterpret_cast<T*>(d.dv) + row + col, y[r], y[r + 1], y[r + 2], y[r + 3]);
+        }
+    }
+}
+
+// out[n] = sum of `splits` partial outputs, in order (n a multiple of 4)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, T* out, long long n, int splits) {
+    for (long long x = 4 * ((long long)blockIdx.x * 256 + threadIdx.x); x < n; x += 4ll * 256 * gridDim.x) {
+        f32x4 s = *reinterpret_cast<const f32x4*>(part + x);
+        for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + x);
+        store4<T>(out + x, s[0], s[1], s[2], s[3]);
+    }
+}
+// dtable[c][h] = sum over samples and row blocks, one wave per entry, fixed order
+__global__ __launch_bounds__(64) void attn_table_kernel(const AttnArgs a, int nb) {
+    const int c = blockIdx.x % nb, h = blockIdx.x / nb, lane = threadIdx.x;
+    float s = 0.f;
+    const long long n = (long long)a.d.B * a.dq_parts;
+    for (long long x = lane; x < n; x += 64) s += a.ptab[(((x / a.dq_parts) * a.d.H + h) * a.dq_parts + x % a.dq_parts) * nb + c];
+    s = wave_sum(s);
+    if (lane) return;
+    const long long o = (long long)c * a.d.H + h;
+    if (a.d.table_dtype == EKAID_F32) reinterpret_cast<float*>(a.d.dtable)[o] = s;
+    else if (a.d.table_dtype == EKAID_BF16) reinterpret_cast<__bf16*>(a.d.dtable)[o] = (__bf16)s;
+    else reinterpret_cast<_Float16*>(a.d.dtable)[o] = (_Float16)s;
+}
+
+struct BwdPlan {
+    int gq, nwq, tq, sq;        // dq: block edge, waves, row tiles, splits
+    int gk, nwk, tk, sk;        // dk / dv
+    size_t delta, nrm, tab, po, pk, total;      // float offsets
+};
+static int bwd_tile(const ekaid_attn_t* a) { return a->dh > 128 || (a->dtype == EKAID_F32 && a->dh > 64) ? 32 : 64; }
+static size_t align4(size_t n) { return (n + 3) & ~(size_t)3; }
+
+static BwdPlan bwd_plan(const ekaid_attn_t* a) {
+    BwdPlan p;
+    const int kt = bwd_tile(a);
+    p.gq = a->Lq <= 64 || (a->dtype == EKAID_F32 && a->dh > 128) ? 16 : 32;
+    const bool wide = a->dtype == EKAID_F32 && a->dh > 128;       // one wave would have to hold a whole staged tile: it spills
+    p.nwq = wide ? 4 : a->Lq <= 16 ? 1 : a->Lq <= 32 && p.gq == 16 ? 2 : 4;
+    p.tq = cdiv(a->Lq, p.gq * p.nwq);
+    p.gk = a->Lk <= 64 || a->dh > 128 ? 16 : 32;
+    p.nwk = wide ? 4 : a->Lk <= 16 ? 1 : a->Lk <= 32 ? 2 : 4;
+    p.tk = cdiv(a->Lk, p.gk * p.nwk);
+    auto split = [](long long wgs, int waves, int work) {
+        const long long want = 4 * 512 / waves;
+        long long s = wgs > 0 && wgs < want / 2 ? (want + wgs - 1) / wgs : 1;
+        if (s > (work + 1) / 2) s = (work + 1) / 2;
+        return (int)(s < 1 ? 1 : s);
+    };
+    p.sq = split((long long)a->B * a->H * p.tq, p.nwq, cdiv(a->Lk, kt));
+    p.sk = split((long long)a->B * a->KV * p.tk, p.nwk, cdiv(a->Lq, kt) * (a->H / a->KV));
+    const size_t rows = (size_t)a->B * a->H * a->Lq, bh = (size_t)a->B * a->H;
+    const int nb = a->table ? (a->n_border + 1) * (a->bidirectional ? 2 : 1) : 0;
+    size_t o = 0;
+    p.delta = o; o += align4(rows);
+    p.nrm = o; o += align4(bh * p.tq * p.sq);
+    p.tab = o; o += align4(bh * p.tq * p.sq * nb);
+    p.po = o; o += p.sq > 1 ? p.sq * rows * a->dh : 0;
+    p.pk = o; o += p.sk > 1 ? 2 * p.sk * (size_t)a->B * a->Lk * a->KV * a->dh : 0;
+    p.total = o * sizeof(float);
+    return p;
+}
+size_t attn_bwd_workspace(const ekaid_attn_t* a) { return bwd_plan(a).total; }
+
+static int lds_limit(const void* fn) {
+    if (func_attr_once(fn) && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) {
+        set_error("attn_bwd: cannot raise the LDS limit");
+        return EKAID_ERR_LAUNCH;
+    }
+    return EKAID_OK;
+}
+template <typename T, int DH, int G, int NW, int KT, bool REL> static int launch_dq(const AttnArgs& a, hipStream_t st) {
+    size_t lds = (size_t)2 * KT * Ld<T, DH>::row * sizeof(T) + KT + 4 * NW;
+    if (REL) lds += 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + NW * G * (G + 1));
+    if (int rc = lds_limit((const void*)attn_dq_kernel<T, DH, G, NW, KT, REL>)) return rc;
+    hipLaunchKernelGGL((attn_dq_kernel<T, DH, G, NW, KT, REL>), dim3(a.d.B * a.d.H * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
+    return check_launch("attn_dq");
+}
+template <typename T, int DH, bool REL> static int pick_dq(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
+    constexpr int KT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
+    if constexpr (!(sizeof(T) == 4 && DH > 128))
+        if (p.gq == 32) return launch_dq<T, DH, 32, 4, KT, REL>(a, st);
+    if constexpr (!(sizeof(T) == 4 && DH > 128)) {
+        if (p.nwq == 1) return launch_dq<T, DH, 16, 1, KT, REL>(a, st);
+        if (p.nwq == 2) return launch_dq<T, DH, 16, 2, KT, REL>(a, st);
+    }
+    return launch_dq<T, DH, 16, 4, KT, REL>(a, st);
+}
+template <typename T, int DH, int G, int NW, int QT> static int launch_dkv(const AttnArgs& a, hipStream_t st) {
+    const size_t lds = (size_t)2 * QT * Ld<T, DH>::row * sizeof(T) + 8 * QT + (a.d.table ? 4 * (2 * a.d.reach + 1) : 0);
+    if (int rc = lds_limit((const void*)attn_dkv_kernel<T, DH, G, NW, QT>)) return rc;
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DH, G, NW, QT>), dim3(a.d.B * a.d.KV * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
+    return check_launch("attn_dkv");
+}
+template <typename T, int DH> static int pick_dkv(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
+    constexpr int QT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
+    if constexpr (DH <= 128)
+        if (p.gk == 32) return launch_dkv<T, DH, 32, 4, QT>(a, st);
+    if constexpr (!(sizeof(T) == 4 && DH > 128)) {
+        if (p.nwk == 1) return launch_dkv<T, DH, 16, 1, QT>(a, st);
+        if (p.nwk == 2) return launch_dkv<T, DH, 16, 2, QT>(a, st);
+    }
+    return launch_dkv<T, DH, 16, 4, QT>(a, st);
+}
+template <typename T> static int sum_parts(const float* part, void* out, long long n, int splits, hipStream_t st) {
+    hipLaunchKernelGGL(attn_sum_kernel<T>, dim3((int)std::min<long long>((n / 4 + 255) / 256, 4096)), dim3(256), 0, st, part, (T*)out, n, splits);
+    return check_launch("attn_sum");
+}
+template <typename T> static int run_bwd(AttnArgs a, const BwdPlan& p, hipStream_t st) {
+    const ekaid_attn_t& d = a.d;
+    int rc = EKAID_OK;
+    a.gp = 1;
+    a.tiles = p.tq;
+    a.splits = p.sq;
+    a.dq_parts = p.tq * p.sq;
+    if (d.table)
+        rc = d.dh <= 64 ? pick_dq<T, 64, true>(a, p, st) : d.dh <= 128 ? pick_dq<T, 128, true>(a, p, st) : pick_dq<T, 256, true>(a, p, st);
+    else
+        rc = d.dh <= 64 ? pick_dq<T, 64, false>(a, p, st) : d.dh <= 128 ? pick_dq<T, 128, false>(a, p, st) : pick_dq<T, 256, false>(a, p, st);
+    if (rc) return rc;
+    if (p.sq > 1 && (rc = sum_parts<T>(a.po, d.dq, (long long)d.B * d.Lq * d.H * d.dh, p.sq, st))) return rc;
+    if (d.table) {
+        const int nb = (d.n_border + 1) * (d.bidirectional ? 2 : 1);
+        hipLaunchKernelGGL(attn_table_kernel, dim3(nb * d.H), dim3(64), 0, st, a, nb);
+        if ((rc = check_launch("attn_table"))) return rc;
+    }
+    if (d.Lk == 0) return EKAID_OK;
+    a.tiles = p.tk;
+    a.splits = p.sk;
+    rc = d.dh <= 64 ? pick_dkv<T, 64>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128>(a, p, st) : pick_dkv<T, 256>(a, p, st);
+    if (rc || p.sk == 1) return rc;
+    const long long n = (long long)d.B * d.Lk * d.KV * d.dh;
+    if ((rc = sum_parts<T>(a.pk, d.dk, n, p.sk, st))) return rc;
+    return sum_parts<T>(a.pv, d.dv, n, p.sk, st);
+}
+}  // namespace ekaid
+
+extern "C" int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace ekaid;
+    if (int rc = attn_check(a, "attn_bwd")) return rc;
+    if (a->B == 0 || a->Lq == 0) { set_error("attn_bwd: no query rows (the caller zeroes dk, dv, dtable)"); return EKAID_ERR_ARG; }
+    if (!a->q || !a->out || !a->dout || !a->lse || !a->dq || (a->table && !a->dtable) || (a->Lk && (!a->k || !a->v || !a->dk || !a->dv))) {
+        set_error("attn_bwd: null operand");
+        return EKAID_ERR_ARG;
+    }
+    if (((uintptr_t)a->dout | (uintptr_t)a->out) & 15) { set_error("attn_bwd: operands must be 16-byte aligned"); return EKAID_ERR_ARG; }
+    const BwdPlan p = bwd_plan(a);
+    if (!workspace || workspace_bytes < p.total) { set_error("attn_bwd: workspace of %zu bytes needed", p.total); return EKAID_ERR_ARG; }
+    AttnArgs k = {};
+    k.d = *a;
+    k.seed = DS(a->drop_seed);
+    k.inv_keep = 1.f / (1.f - a->drop_p);
+    k.sc2 = a->scale * LOG2E;
+    float* w = (float*)workspace;
+    k.delta = w + p.delta;
+    k.nrm = w + p.nrm;
+    k.ptab = w + p.tab;
+    k.po = w + p.po;
+    k.pk = w + p.pk;
+    k.pv = k.pk + (size_t)p.sk * a->B * a->Lk * a->KV * a->dh;
+    hipStream_t st = (hipStream_t)stream;
+    return a->dtype == EKAID_F32 ? run_bwd<float>(k, p, st) : a->dtype == EKAID_BF16 ? run_bwd<__bf16>(k, p, st) : run_bwd<_Float16>(k, p, st);
+}

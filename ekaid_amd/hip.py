@@ -95,6 +95,17 @@ class SpeakerGreedy(Structure):
                 ('seq', c_void_p), ('seq_logp', c_void_p), ('seq_len', c_int), ('n_unfinished', c_void_p)]
 
 
+class Attn(Structure):
+    """ekaid_attn_t: one attention call, forward and backward."""
+    _fields_ = ([(n, c_void_p) for n in ('q', 'k', 'v')] + [(n, c_int) for n in ('dtype', 'B', 'H', 'KV', 'dh', 'Lq', 'Lk')] +
+                [(n, c_longlong) for n in ('q_batch', 'q_row', 'k_batch', 'k_row', 'v_batch', 'v_row')] +
+                [('scale', c_float), ('k_len', c_void_p), ('q_pos', c_void_p), ('k_len64', c_int), ('q_pos64', c_int),
+                 ('key_mask', c_void_p), ('mask_batch', c_longlong), ('table', c_void_p)] +
+                [(n, c_int) for n in ('table_dtype', 'bidirectional', 'n_border', 'reach')] +
+                [('border', c_int * 128), ('causal', c_int), ('drop_p', c_float), ('drop_seed', c_uint64)] +
+                [(n, c_void_p) for n in ('out', 'lse', 'dout', 'dq', 'dk', 'dv', 'dtable')])
+
+
 P, I, L, F, U64 = c_void_p, c_int, c_longlong, c_float, c_uint64
 
 # name -> argtypes (restype is int unless listed in _RESTYPES); mirrors include/ekaid_hip.h 1:1
@@ -215,9 +226,12 @@ SIGNATURES = {
     'ekaid_seq_fault_flag': [P, P],
     'ekaid_launch_count': [I],
     'ekaid_amax_rc': [P, L, I, I, P, P, I, P],
+    'ekaid_attn_workspace_bytes': [POINTER(Attn), I],
+    'ekaid_attn_fwd': [POINTER(Attn), P, c_size_t, P],
+    'ekaid_attn_bwd': [POINTER(Attn), P, c_size_t, P],
     'ekaid_amax_rc_multi': [P, P, P, P, P, P, I, I, P],
 }
-_RESTYPES = {'ekaid_last_error': c_char_p, 'ekaid_launch_count': c_longlong, 'ekaid_gemm_workspace_bytes': c_size_t, 'ekaid_gemm_pair_workspace_bytes': c_size_t, 'ekaid_gru_seq_workspace_bytes': c_size_t, 'ekaid_gru_seq_persistent_workspace_bytes': c_size_t,
+_RESTYPES = {'ekaid_last_error': c_char_p, 'ekaid_attn_workspace_bytes': c_size_t, 'ekaid_launch_count': c_longlong, 'ekaid_gemm_workspace_bytes': c_size_t, 'ekaid_gemm_pair_workspace_bytes': c_size_t, 'ekaid_gru_seq_workspace_bytes': c_size_t, 'ekaid_gru_seq_persistent_workspace_bytes': c_size_t,
              'ekaid_speaker_seq_workspace_bytes': c_size_t, 'ekaid_speaker_seq_persistent_workspace_bytes': c_size_t,
              'ekaid_speaker_seq_persistent_status_ptr': c_void_p, 'ekaid_speaker_seq_bwd_persistent_workspace_bytes': c_size_t, 'ekaid_speaker_greedy_workspace_bytes': c_size_t, 'ekaid_speaker_greedy_persistent_workspace_bytes': c_size_t}
 

@@ -5,12 +5,15 @@ PyTorch supplies device memory (``torch.empty``), the stream and the autograd ta
 arithmetic on the path is done by ATen.  Every operator raises if its inputs are not on the
 HIP device -- there is no CPU fallback (the CPU restatement is ``oracle/``, test-only).
 """
+import contextlib
 import ctypes
+import functools
 import math
 import os
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import hip
 from .hip import (ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, GemmDesc, check, ptr, require_cuda,
@@ -2156,3 +2159,191 @@ class HeadAttentionFn(Function):
 
 def head_attention(q, k, v, heads, p=0.0, training=False):
     return HeadAttentionFn.apply(q, k, v, heads, p, training)
+
+
+# --------------------------------------------------------------------------- #
+# attention to the states of another length; attention with a learned relative position bias
+# --------------------------------------------------------------------------- #
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # EKAID_F32 / BF16 / F16
+_ATTN_MAX_REACH = 1024                                                            # EKAID_ATTN_MAX_REACH
+
+
+def _refuse(cond, msg):
+    if cond:
+        raise hip.EkaidError(msg)
+
+
+def _on_device(t):
+    """Make ``t``'s device current for the launches inside (kernels run on the device of their tensors, on its current stream)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _scratch(nbytes, device):
+    """Workspace of one call from torch's allocator: stream-ordered, private to a captured graph (unlike ``hip.workspace``)."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def _vec_rows(t):
+    """``t`` (B, L, D) as the attention kernels read it: unit inner stride, whole 16-byte vectors between rows and samples (else a copy)."""
+    epl = 16 // t.element_size()
+    if t.numel() == 0:
+        return t.contiguous()
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st % epl == 0 for n, st in zip(t.shape[:2], t.stride()[:2]))
+    if ok:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_strides(t):
+    """(between samples, between rows) in elements; an axis of one entry has no stride that counts."""
+    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+@functools.lru_cache(maxsize=None)
+def relative_borders(buckets, max_distance):
+    """Smallest distance of bucket 1, 2, ... of one direction: the first ``buckets // 2`` distances have a bucket each, the others share
+    the rest by the logarithm of the distance up to ``max_distance``.  Decided in whole numbers: bucket e + s begins at the first d with
+    (d / e)^n >= (max_distance / e)^s, n = buckets - e."""
+    e = buckets // 2
+    n = buckets - e
+    out = list(range(1, e + 1))
+    for s in range(1, n):
+        lo, hi = out[-1], max_distance
+        while lo < hi:
+            d = (lo + hi) // 2
+            if d ** n * e ** s >= max_distance ** s * e ** n:
+                hi = d
+            else:
+                lo = d + 1
+        out.append(lo)
+    return tuple(out)
+
+
+class AttentionFn(Function):
+    """One pass over the keys per query row, nothing of size Lq x Lk kept; the backward forms the scores again
+    (include/ekaid_hip.h: ekaid_attn_t)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, cfg):
+        (heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, seed) = cfg
+        q, k, v = _vec_rows(q), _vec_rows(k), _vec_rows(v)
+        table = None if table is None else _c(table)
+        B, Lq, D = q.shape
+        out = torch.empty(B, Lq, D, device=q.device, dtype=q.dtype)
+        need = any(ctx.needs_input_grad[:4])
+        lse = torch.empty(B, heads, Lq, device=q.device, dtype=torch.float32) if need else None
+        with _on_device(q):
+            d = AttentionFn._desc(q, k, v, table, cfg, out, lse)
+            L = hip.lib()
+            nb = L.ekaid_attn_workspace_bytes(ctypes.byref(d), 0)
+            ws = _scratch(nb, q.device) if nb else None
+            check(L.ekaid_attn_fwd(ctypes.byref(d), ptr(ws), nb, stream()), 'attn_fwd')
+        if need:
+            ctx.cfg = cfg
+            ctx.save_for_backward(q, k, v, table, out, lse, k_len, key_mask, q_pos)
+        return out
+
+    @staticmethod
+    def _desc(q, k, v, table, cfg, out, lse):
+        (heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, seed) = cfg
+        d = hip.Attn()
+        d.q, d.k, d.v, d.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[q.dtype]
+        d.B, d.Lq, d.Lk, d.H, d.KV, d.dh = q.shape[0], q.shape[1], k.shape[1], heads, kv_heads, q.shape[2] // heads
+        (d.q_batch, d.q_row), (d.k_batch, d.k_row), (d.v_batch, d.v_row) = _row_strides(q), _row_strides(k), _row_strides(v)
+        d.scale = scale
+        d.k_len, d.k_len64 = ptr(k_len), int(k_len is not None and k_len.dtype == torch.int64)
+        d.q_pos, d.q_pos64 = ptr(q_pos), int(q_pos is not None and q_pos.dtype == torch.int64)
+        d.key_mask, d.mask_batch = ptr(key_mask), (key_mask.stride(0) if key_mask is not None and q.shape[0] > 1 else 0)
+        if table is not None:
+            borders = relative_borders(table.shape[0] // 2 if bidirectional else table.shape[0], max_distance)
+            d.table, d.table_dtype, d.bidirectional = table.data_ptr(), _DTYPE_CODE[table.dtype], int(bidirectional)
+            d.n_border, d.reach = len(borders), borders[-1]
+            d.border[:len(borders)] = borders
+        d.causal = int(causal)
+        d.drop_p, d.drop_seed = p, seed
+        d.out, d.lse = out.data_ptr(), ptr(lse)
+        return d
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, out, lse, k_len, key_mask, q_pos = ctx.saved_tensors
+        dout = _c(dout)
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq = torch.empty_like(out)
+        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+        dtable = torch.empty_like(table) if table is not None else None
+        if q.shape[0] == 0 or q.shape[1] == 0:
+            return dq, dk.zero_(), dv.zero_(), (dtable.zero_() if table is not None else None), None
+        with _on_device(q):
+            d = AttentionFn._desc(q, k, v, table, ctx.cfg, out, lse)
+            d.dout, d.dq, d.dk, d.dv, d.dtable = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(dtable)
+            L = hip.lib()
+            nb = L.ekaid_attn_workspace_bytes(ctypes.byref(d), 1)
+            ws = _scratch(nb, q.device)
+            check(L.ekaid_attn_bwd(ctypes.byref(d), ptr(ws), nb, stream()), 'attn_bwd')
+        return dq, dk, dv, dtable, None
+
+
+def _attention(what, q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, training):
+    require_cuda(q, k, v, table, k_len, key_mask, q_pos)
+    kv_heads = heads if kv_heads is None else kv_heads
+    for t in (q, k, v):
+        _refuse(t.dim() != 3, '%s: q, k, v are (batch, length, heads * width), got %s' % (what, tuple(t.shape)))
+        _refuse(t.dtype not in _DTYPE_CODE or t.dtype != q.dtype, '%s: q, k, v share one of float32, bfloat16, float16 (got %s, %s, %s)' % (what, q.dtype, k.dtype, v.dtype))
+    for t in (k, v, table, k_len, key_mask, q_pos):
+        _refuse(t is not None and t.device != q.device, '%s: every tensor must be on %s' % (what, q.device))
+    B, Lq, D = q.shape
+    _refuse(heads < 1 or kv_heads < 1 or heads % kv_heads or D % heads, '%s: %d heads, %d key heads, width %d do not divide' % (what, heads, kv_heads, D))
+    dh = D // heads
+    _refuse(dh % 8 or not 8 <= dh <= 256, '%s: head width %d (a multiple of 8 up to 256)' % (what, dh))
+    _refuse(k.shape != v.shape or k.shape[0] != B or k.shape[2] != kv_heads * dh,
+            '%s: k %s and v %s do not fit q %s with %d of %d heads' % (what, tuple(k.shape), tuple(v.shape), tuple(q.shape), kv_heads, heads))
+    for name, t in (('k_len', k_len), ('q_pos', q_pos)):
+        _refuse(t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,)), '%s: %s is an int32 or int64 tensor of shape (%d,)' % (what, name, B))
+    if key_mask is not None:
+        _refuse(key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, k.shape[1]), '%s: key_mask is a bool tensor of shape %s' % (what, (B, k.shape[1])))
+        if key_mask.stride(1) != 1 and k.shape[1] > 1:
+            key_mask = key_mask.contiguous()
+    _refuse(not 0.0 <= p < 1.0, '%s: dropout probability %r' % (what, p))
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    _refuse(not math.isfinite(scale), '%s: scale %r' % (what, scale))
+    if table is not None:
+        _refuse(table.dim() != 2 or table.shape[1] != heads or table.dtype not in (torch.float32, q.dtype),
+                '%s: table is (buckets, %d), float32 or %s (got %s %s)' % (what, heads, q.dtype, tuple(table.shape), table.dtype))
+        _refuse(bidirectional and table.shape[0] % 2, '%s: %d buckets for two directions' % (what, table.shape[0]))
+        side = table.shape[0] // 2 if bidirectional else table.shape[0]
+        _refuse(not 2 <= side <= 128, '%s: 2 to 128 buckets a direction (got %d)' % (what, side))
+        _refuse(int(max_distance) != max_distance or max_distance <= side // 2, '%s: max_distance %r must exceed the %d exact buckets' % (what, max_distance, side // 2))
+        _refuse(relative_borders(side, int(max_distance))[-1] > _ATTN_MAX_REACH, '%s: the last bucket must begin within %d positions' % (what, _ATTN_MAX_REACH))
+    p = float(p) if training else 0.0
+    cfg = (heads, kv_heads, None if k_len is None else _c(k_len), key_mask, None if q_pos is None else _c(q_pos), bool(causal), bool(bidirectional),
+           int(max_distance), scale, p, next_seed() if p > 0.0 else 0)
+    out = AttentionFn.apply(q, k, v, table, cfg)
+    if q.dtype == torch.float32:
+        assert_finite(out, what)
+    return out
+
+
+def cross_attention(q, k, v, heads, kv_heads=None, k_len=None, key_mask=None, scale=None, p=0.0, training=False):
+    """Attention of (B, Lq, heads * dh) queries to (B, Lk, kv_heads * dh) states of another length (an answer decoder over region states;
+    one new token: Lq = 1).  ``kv_heads`` divides ``heads``: query head h reads key head h // (heads // kv_heads).  ``k_len`` (B,) int32 /
+    int64: valid states of a sample; ``key_mask`` (B, Lk) bool: True = may be attended.  A row left without any state gives zeros and
+    zero gradients; what masked states hold does not matter.  ``scale`` defaults to dh ** -0.5.  Dropout of the probabilities as in
+    ``head_attention``.  float32, bfloat16 or float16; dh a multiple of 8 up to 256; unit inner stride (else copied)."""
+    return _attention('cross_attention', q, k, v, None, heads, kv_heads, k_len, key_mask, None, False, False, 0, scale, p, training)
+
+
+def relative_attention(q, k, v, table, heads, kv_heads=None, k_len=None, key_mask=None, q_pos=None, causal=False, bidirectional=None,
+                       max_distance=128, scale=None, p=0.0, training=False):
+    """``cross_attention`` with a learned bias by distance: score (i, j) gains ``table[bucket(j - pos_i), head]``, pos_i = q_pos[b] + i
+    (``q_pos`` (B,) int32 / int64, default 0: a new token of a cache passes its position).  ``causal``: j <= pos_i only.  ``table``
+    (buckets, heads), float32 or q's type; ``bidirectional`` (default: not causal) gives half the buckets to j > pos_i, otherwise those
+    share bucket 0.  Per direction the nearest half of the buckets hold one distance each, the others share the distances up to
+    ``max_distance`` by logarithm (``relative_borders``), the last takes everything beyond.  The bias is never a (heads, Lq, Lk) tensor;
+    its gradient is summed in float32 in a fixed order."""
+    _refuse(table is None, 'relative_attention: table is required')
+    bidirectional = (not causal) if bidirectional is None else bidirectional
+    return _attention('relative_attention', q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, training)

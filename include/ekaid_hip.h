@@ -672,6 +672,59 @@ int ekaid_seq_fault_flag(float* flag, void* stream);
 #define EKAID_COUNT_N 12
 long long ekaid_launch_count(int which);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention of query rows to the states of another length, with shared keys, ragged lengths and a learned relative position bias.
+ *   s[i][j] = scale <q_i, k_j> (+ table[bucket(j - (q_pos + i))][head]),   o_i = sum_j softmax_j(s[i][:]) v_j
+ * over the keys j < k_len[b] with key_mask[b][j] != 0 (causal: also j <= q_pos + i).  A row without any such key gives o = 0 and
+ * gradients 0.  Masked key and value rows are never read into a product (NaN there stays there).  Scores are never stored.
+ * q [B][Lq][H dh], k and v [B][Lk][KV dh]: strides between samples and rows in elements, heads dh apart, all 16-byte aligned;
+ * out, dout, dq [B][Lq][H dh] and dk, dv [B][Lk][KV dh] contiguous.  H % KV == 0, dh % 8 == 0, dh <= 256.  dtype: EKAID_F32 / BF16 / F16
+ * of every tensor but lse, table; products accumulate and softmax statistics are held in f32; probabilities and score gradients are
+ * rounded to the tensors' type where they enter a matrix product.  Dropout multiplies the probabilities, mask index
+ * ((b H + h) Lq + i) Lk + j.
+ * Relative bias (table != NULL): table [buckets][H]; bucket of a distance = number of `border` entries <= distance (n_border of them,
+ * not descending); distances: |j - pos| with the upper half of the buckets for j > pos (bidirectional), else max(pos - j, 0).  reach >= 1 and
+ * >= the last border, <= EKAID_ATTN_MAX_REACH.
+ * lse [B][H][Lq]: log2 of the softmax denominator (+inf for an empty row); written by fwd when not NULL, read by bwd.
+ * bwd writes dq, dk, dv and (table != NULL) dtable [buckets][H] of type table_dtype.  No float atomics: bit-reproducible.
+ * No counterpart in the reference: its SelfAttention (modules.py:17-77) is the equal-length, unmasked, unbiased case.
+ * ------------------------------------------------------------------------------------------ */
+#define EKAID_F32 0
+#define EKAID_BF16 1
+#define EKAID_F16 2
+#define EKAID_ATTN_MAX_BUCKETS 128
+#define EKAID_ATTN_MAX_REACH 1024
+typedef struct ekaid_attn {
+    const void* q;
+    const void* k;
+    const void* v;
+    int dtype;
+    int B, H, KV, dh, Lq, Lk;
+    long long q_batch, q_row, k_batch, k_row, v_batch, v_row;
+    float scale;
+    const void* k_len;      /* optional DEVICE [B], int32 or (k_len64) int64; clamped to [0, Lk] */
+    const void* q_pos;      /* optional DEVICE [B]: position of query row 0; NULL = 0 */
+    int k_len64, q_pos64;
+    const unsigned char* key_mask; /* optional DEVICE [B][Lk] bytes, samples mask_batch apart: 0 = not attended */
+    long long mask_batch;
+    const void* table;      /* optional */
+    int table_dtype, bidirectional, n_border, reach;
+    int border[EKAID_ATTN_MAX_BUCKETS];
+    int causal;
+    float drop_p;
+    uint64_t drop_seed;
+    void* out;
+    float* lse;
+    const void* dout;
+    void* dq;
+    void* dk;
+    void* dv;
+    void* dtable;
+} ekaid_attn_t;
+size_t ekaid_attn_workspace_bytes(const ekaid_attn_t* a, int backward);
+int ekaid_attn_fwd(const ekaid_attn_t* a, void* workspace, size_t workspace_bytes, void* stream);
+int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
