@@ -106,6 +106,13 @@ class Attn(Structure):
                 [(n, c_void_p) for n in ('out', 'lse', 'dout', 'dq', 'dk', 'dv', 'dtable')])
 
 
+class LinearLoss(Structure):
+    """ekaid_linear_loss_t."""
+    _fields_ = ([('x', c_void_p), ('weight', c_void_p), ('bias', c_void_p)] + [(n, c_int) for n in ('dtype', 'B', 'T', 'D', 'V')] +
+                [('ldx', c_longlong), ('target', c_void_p), ('ld_target', c_longlong), ('mask', c_void_p), ('ld_mask', c_longlong)] +
+                [(n, c_void_p) for n in ('denom', 'loss', 'state', 'dloss', 'dx', 'dweight', 'dbias')])
+
+
 P, I, L, F, U64 = c_void_p, c_int, c_longlong, c_float, c_uint64
 
 # name -> argtypes (restype is int unless listed in _RESTYPES); mirrors include/ekaid_hip.h 1:1
@@ -229,9 +236,14 @@ SIGNATURES = {
     'ekaid_attn_workspace_bytes': [POINTER(Attn), I],
     'ekaid_attn_fwd': [POINTER(Attn), P, c_size_t, P],
     'ekaid_attn_bwd': [POINTER(Attn), P, c_size_t, P],
+    'ekaid_linear_loss_state_bytes': [POINTER(LinearLoss)],
+    'ekaid_linear_loss_workspace_bytes': [POINTER(LinearLoss), I],
+    'ekaid_linear_loss_fwd': [POINTER(LinearLoss), P, c_size_t, P],
+    'ekaid_linear_loss_bwd': [POINTER(LinearLoss), P, c_size_t, P],
     'ekaid_amax_rc_multi': [P, P, P, P, P, P, I, I, P],
 }
-_RESTYPES = {'ekaid_last_error': c_char_p, 'ekaid_attn_workspace_bytes': c_size_t, 'ekaid_launch_count': c_longlong, 'ekaid_gemm_workspace_bytes': c_size_t, 'ekaid_gemm_pair_workspace_bytes': c_size_t, 'ekaid_gru_seq_workspace_bytes': c_size_t, 'ekaid_gru_seq_persistent_workspace_bytes': c_size_t,
+_RESTYPES = {'ekaid_last_error': c_char_p, 'ekaid_attn_workspace_bytes': c_size_t, 'ekaid_linear_loss_state_bytes': c_size_t,
+             'ekaid_linear_loss_workspace_bytes': c_size_t, 'ekaid_launch_count': c_longlong, 'ekaid_gemm_workspace_bytes': c_size_t, 'ekaid_gemm_pair_workspace_bytes': c_size_t, 'ekaid_gru_seq_workspace_bytes': c_size_t, 'ekaid_gru_seq_persistent_workspace_bytes': c_size_t,
              'ekaid_speaker_seq_workspace_bytes': c_size_t, 'ekaid_speaker_seq_persistent_workspace_bytes': c_size_t,
              'ekaid_speaker_seq_persistent_status_ptr': c_void_p, 'ekaid_speaker_seq_bwd_persistent_workspace_bytes': c_size_t, 'ekaid_speaker_greedy_workspace_bytes': c_size_t, 'ekaid_speaker_greedy_persistent_workspace_bytes': c_size_t}
 

@@ -1873,6 +1873,106 @@ def lm_loss(logp, target, mask, denom=None):
     return LMLossFn.apply(logp, target, mask, denom)
 
 
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # EKAID_F32 / BF16 / F16
+
+
+def _refuse(cond, msg):
+    if cond:
+        raise hip.EkaidError(msg)
+
+
+def _on_device(t):
+    """Make ``t``'s device current for the launches inside (kernels run on the device of their tensors, on its current stream)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _scratch(nbytes, device):
+    """Workspace of one call from torch's allocator: stream-ordered, private to a captured graph (unlike ``hip.workspace``)."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+class LinearLossFn(Function):
+    """Loss of a linear layer over the vocabulary without its logits (include/ekaid_hip.h: ekaid_linear_loss_t)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, mask, denom):
+        shape = x.shape
+        x2, ld = _rows2d(x)
+        if x2.dtype != torch.float32 and x2.numel() and (ld % 8 or x2.data_ptr() % 16):
+            x2, ld = x2.clone(memory_format=torch.contiguous_format), shape[2]
+        weight, bias = _c(weight), (None if bias is None else _c(bias))
+        if weight.data_ptr() % 16 and weight.dtype != torch.float32:
+            weight = weight.clone()
+        loss = torch.empty((), device=x.device, dtype=torch.float32)
+        L = hip.lib()
+        with _on_device(x):
+            d = LinearLossFn._desc(x2, ld, shape, weight, bias, target, mask, denom)
+            state = _scratch(L.ekaid_linear_loss_state_bytes(ctypes.byref(d)), x.device)
+            nb = L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 0)
+            ws = _scratch(nb, x.device)
+            d.loss, d.state = loss.data_ptr(), state.data_ptr()
+            check(L.ekaid_linear_loss_fwd(ctypes.byref(d), ptr(ws), nb, stream()), 'linear_loss_fwd')
+        ctx.shape, ctx.ld = shape, ld
+        ctx.save_for_backward(x2, weight, bias, target, mask, denom, state)
+        return loss
+
+    @staticmethod
+    def _desc(x2, ld, shape, weight, bias, target, mask, denom):
+        d = hip.LinearLoss()
+        d.x, d.weight, d.bias, d.dtype = x2.data_ptr(), weight.data_ptr(), ptr(bias), _DTYPE_CODE[x2.dtype]
+        d.B, d.T, d.D, d.V, d.ldx = shape[0], shape[1], shape[2], weight.shape[0], max(ld, shape[2])
+        d.target, d.ld_target, d.mask, d.ld_mask = target.data_ptr(), target.stride(0), mask.data_ptr(), mask.stride(0)
+        d.denom = ptr(denom)
+        return d
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x2, weight, bias, target, mask, denom, state = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        f32 = weight.dtype == torch.float32
+        dx = torch.empty(ctx.shape, device=x2.device, dtype=x2.dtype) if need[0] else None
+        dw = (grad_out(weight) if f32 else torch.empty_like(weight)) if need[1] else None
+        db = (grad_out(bias) if f32 else torch.empty_like(bias)) if bias is not None and need[2] else None
+        if x2.numel() == 0:
+            return tuple(None if g is None else g.zero_() for g in (dx, dw, db)) + (None, None, None)
+        dloss = _c(dloss)
+        L = hip.lib()
+        with _on_device(x2):
+            d = LinearLossFn._desc(x2, ctx.ld, ctx.shape, weight, bias, target, mask, denom)
+            d.state, d.dloss, d.dx, d.dweight, d.dbias = state.data_ptr(), dloss.data_ptr(), ptr(dx), ptr(dw), ptr(db)
+            nb = L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 1)
+            ws = _scratch(nb, x2.device)
+            check(L.ekaid_linear_loss_bwd(ctypes.byref(d), ptr(ws), nb, stream()), 'linear_loss_bwd')
+        return dx, dw, db, None, None, None
+
+
+def linear_lm_loss(x, weight, bias, target, mask, denom=None):
+    """``lm_loss(log_softmax(linear(x, weight, bias)), target, mask, denom)`` without the logits: x (B, T, D) states, weight (V, D), bias
+    (V,) or None, of one type (float32, bfloat16, float16; 16-bit: D a multiple of 8); target (B, >= T) int64 and mask (B, >= T) float32
+    as ``lm_loss`` takes them, mask values weigh their rows.  The vocabulary is taken in pieces and the logits are formed again in the
+    backward.  Rows with mask 0 add nothing and get zero gradients whatever x and target hold there; a target outside the vocabulary in
+    a row that counts makes the loss NaN; an all-zero mask gives 0 / 0 (as ``lm_loss``) with zero gradients."""
+    require_cuda(x, weight, bias, target, mask, denom)
+    _refuse(x.dim() != 3 or weight.dim() != 2 or weight.shape[1] != x.shape[2] or weight.shape[0] < 1 or x.shape[2] < 1,
+            'linear_lm_loss: x %s and weight %s are (B, T, D) and (V, D)' % (tuple(x.shape), tuple(weight.shape)))
+    _refuse(x.dtype not in _DTYPE_CODE or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype),
+            'linear_lm_loss: x, weight, bias share one of float32, bfloat16, float16 (got %s, %s)' % (x.dtype, weight.dtype))
+    _refuse(x.dtype != torch.float32 and x.shape[2] % 8, 'linear_lm_loss: width %d is not a multiple of 8' % x.shape[2])
+    _refuse(bias is not None and tuple(bias.shape) != (weight.shape[0],), 'linear_lm_loss: bias is (%d,)' % weight.shape[0])
+    for t in (weight, bias, target, mask, denom):
+        _refuse(t is not None and t.device != x.device, 'linear_lm_loss: every tensor must be on %s' % x.device)
+    B, T = x.shape[:2]
+    for name, t, dt in (('target', target, torch.int64), ('mask', mask, torch.float32)):
+        _refuse(t.dim() != 2 or t.dtype != dt or t.shape[0] != B or t.shape[1] < T, 'linear_lm_loss: %s is %s of shape (%d, >= %d)' % (name, dt, B, T))
+    _refuse(denom is not None and (denom.numel() != 1 or denom.dtype != torch.float32), 'linear_lm_loss: denom is a float32 scalar')
+    _refuse(B * T > 1 << 28 or weight.shape[0] > 1 << 28, 'linear_lm_loss: at most 2^28 rows and words')
+    target, mask = (t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous() for t in (target, mask))
+    loss = LinearLossFn.apply(x, weight, bias, target, mask, denom)
+    assert_finite(loss, 'linear_lm_loss')
+    return loss
+
+
 class TotalLossFn(Function):
     """speaker_loss + coef * (sum(att_bef) + sum(att_aft)).  ref: train_mimic.py:246-247."""
 
@@ -2164,23 +2264,7 @@ def head_attention(q, k, v, heads, p=0.0, training=False):
 # --------------------------------------------------------------------------- #
 # attention to the states of another length; attention with a learned relative position bias
 # --------------------------------------------------------------------------- #
-_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # EKAID_F32 / BF16 / F16
 _ATTN_MAX_REACH = 1024                                                            # EKAID_ATTN_MAX_REACH
-
-
-def _refuse(cond, msg):
-    if cond:
-        raise hip.EkaidError(msg)
-
-
-def _on_device(t):
-    """Make ``t``'s device current for the launches inside (kernels run on the device of their tensors, on its current stream)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _scratch(nbytes, device):
-    """Workspace of one call from torch's allocator: stream-ordered, private to a captured graph (unlike ``hip.workspace``)."""
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
 
 
 def _vec_rows(t):

@@ -131,6 +131,16 @@ class LanguageModelCriterion(nn.Module):
         return ops.lm_loss(input, target, mask, denom)
 
 
+class LinearLanguageModelCriterion(nn.Module):
+    """``LanguageModelCriterion`` of ``log_softmax(layer(hidden))`` for a large vocabulary: the logits are never kept
+    (``ops.linear_lm_loss``).  ``layer``: a Linear (``DynamicSpeaker.logit``); ``hidden``: its (B, T, D) input."""
+
+    def forward(self, hidden, layer, target, mask, denom=None):
+        if mask.dtype != torch.float32:
+            mask = mask.float()
+        return ops.linear_lm_loss(hidden, layer.weight, layer.bias, target, mask, denom)
+
+
 def total_loss(speaker_loss, att_bef, att_aft):
     """speaker_loss + 2.5e-3 * (sum(att_bef) + sum(att_aft)) / (2B)   (train_mimic.py:246-247)."""
     return ops.total_loss(speaker_loss, att_bef, att_aft)

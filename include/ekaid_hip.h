@@ -725,6 +725,44 @@ size_t ekaid_attn_workspace_bytes(const ekaid_attn_t* a, int backward);
 int ekaid_attn_fwd(const ekaid_attn_t* a, void* workspace, size_t workspace_bytes, void* stream);
 int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Loss of a linear layer over a vocabulary, without its logits (and its gradient).
+ *   z[r][v] = <x_r, weight_v> + bias_v,  lse_r = log sum_v exp z[r][v],
+ *   loss = sum_r mask_r (lse_r - z[r][target_r]) / (denom, else sum_r mask_r)          r = (b, t), b < B, t < T
+ * = ekaid_nll_fwd of log_softmax of the linear layer.  x [B T][D] with ldx, weight [V][D] contiguous, bias [V] or NULL: one dtype
+ * (EKAID_F32 / BF16 / F16), 16-byte aligned (16-bit types: D and ldx multiples of 8).  target int64 and mask f32: rows ld_target, ld_mask
+ * apart.  The vocabulary is taken in pieces; fwd keeps per-row statistics only, bwd forms the logits again.  Rows with mask 0 contribute
+ * nothing whatever x and target hold there (16-bit types leave them out of the products as well); a target outside [0, V) in a row that
+ * counts makes the loss NaN.  All-zero mask: loss 0/0, gradients 0.
+ * state (ekaid_linear_loss_state_bytes) is written by fwd and read by bwd.  dloss: device scalar.  dx [B T][D], dweight [V][D],
+ * dbias [V] contiguous, any may be NULL.  f32 products run as ekaid_gemm_f32 in the selected arithmetic; 16-bit products accumulate in
+ * f32, logit gradients are rounded to the type (scaled by an exact power of two) where they enter a product.  No float atomics.
+ * ref: DynamicSpeaker.logit + log_softmax (dynamic_speaker_change_pos.py:163,238) + LanguageModelCriterion (utils/utils.py:204-216).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct ekaid_linear_loss {
+    const void* x;
+    const void* weight;
+    const void* bias;
+    int dtype;
+    int B, T, D, V;
+    long long ldx;
+    const int64_t* target;
+    long long ld_target;
+    const float* mask;
+    long long ld_mask;
+    const float* denom;     /* optional device scalar */
+    float* loss;
+    void* state;
+    const float* dloss;
+    void* dx;
+    void* dweight;
+    void* dbias;
+} ekaid_linear_loss_t;
+size_t ekaid_linear_loss_state_bytes(const ekaid_linear_loss_t* a);
+size_t ekaid_linear_loss_workspace_bytes(const ekaid_linear_loss_t* a, int backward);
+int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream);
+int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
