@@ -72,7 +72,7 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const RowWork& w, 
     if (g == 0 && a.d.lse) a.d.lse[row] = l == 0.f ? POS_INF : m + __builtin_amdgcn_logf(l);
 }
 
-// ---- rows on the lanes, key tiles through LDS, shared by the NW waves of a workgroup (NW * G query rows)
+// ---- few query rows (a new token; the heads that share keys packed into the rows): key tiles through registers into LDS
 template <typename T, int DH, int G, int NW, int KT>
 __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs a) {
     }
     const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
     const unsigned char* mask = d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr;
-    if (d.table) fill_bias(d, bias, w.head0, a.gp, tid, NT);
+    if (d.table) fill_bias(d, bias, w.head0, a.gp, 0, tid, NT);
 
     u32x4 qf[NC];
     const T* qrow = reinterpret_cast<const T*>(d.q) + w.b * d.q_batch + i * d.q_row + (long long)h * d.dh;
@@ -152,6 +152,97 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs a) {
     write_rows<T, DH, G>(a, w, o, m, l, i, h, ok, lane);
 }
 
+// ---- many query rows: NW * G rows a workgroup, key tiles copied to LDS one tile ahead of the products
+template <typename T, int DH, int G, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) void attn_tile_fwd_kernel(const AttnArgs a) {
+    constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G, nv = 4 * Blk<G>::nq;
+    __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* bias = reinterpret_cast<float*>(smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const RowWork w(a);
+    const ekaid_attn_t& d = a.d;
+    const int row0 = (w.tile * NW + wave) * G, h = w.head0;
+    const bool ok = row0 + lane % G < d.Lq, live = row0 < d.Lq;
+    const int i = min(row0 + lane % G, d.Lq - 1), p0 = query_pos(d, w.b), pos = p0 + i, pmin = p0 + min(row0, d.Lq - 1), pmax = p0 + min(row0 + G, d.Lq) - 1;
+    const int len = key_len(d, w.b), kend = d.causal ? max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G))) : len;
+    const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
+    const int width = d.table ? 2 * (d.reach + BIAS_PAD) + 1 : 0;
+    if (d.table) {
+        fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
+        __syncthreads();
+    }
+    MaskRing<KT> ring;
+    ring.init(d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr, reinterpret_cast<unsigned char*>(bias + width), len, t0, tid);
+
+    u32x4 qf[NC];
+    const T* qrow = reinterpret_cast<const T*>(d.q) + w.b * d.q_batch + i * d.q_row + (long long)h * d.dh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qf[c] = row_frag_global<T, G>(qrow, c, d.dh, ok, lane);
+    TileFrag<T, DH, G> tf(lane);
+    TileCopy<T, DH, KT, NW> ck, cv;
+    ck.init(reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh, d.k_row, lane);
+    cv.init(reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh, d.v_row, lane);
+    typename Blk<G>::acc o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
+    float m = NEG_INF, l = 0.f;
+    if (t0 < t1) {
+        ck.issue(k0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+        cv.issue(v0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+    }
+    auto tile = [&](int t, const T* ks, const T* vs, T* kn, T* vn) __attribute__((always_inline)) {
+        settle();
+        ring.step(t);
+        if (t + 1 < t1) {
+            ck.issue(kn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+            cv.issue(vn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+        }
+        if (!live || (d.causal && t * KT > pmax)) return;
+        if constexpr (DH * sizeof(T) > 128) tf.refresh();
+        typename Blk<G>::acc s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) s[b] = zero_acc<G>();
+        fragment_loop<T, NC * NB>([&](int n) __attribute__((always_inline)) { return tf.rows(ks, (n % NB) * G, n / NB); },
+                                  [&](int n, u32x4 x) __attribute__((always_inline)) { s[n % NB] = mma<T, G>(x, qf[n / NB], s[n % NB]); });
+        const Affine f = scores_by_row<G, NB>(a, s, t * KT, len, pos, pmin, pmax, d.table ? bias : nullptr, ring.tile(t), lane);
+        float mx = s[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < nv; ++r) mx = fmaxf(mx, s[b][r]);
+        const float mn = fmaxf(m, across_groups_max<G>(mx) * f.mult + f.add);      // (mult >= 0)
+        const float base = mn == NEG_INF ? 0.f : mn, shift = f.add - base;
+        if (__any(mn != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            l *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < nv; ++e) o[mt][e] *= alpha;
+        }
+        m = mn;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < nv; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] * f.mult + shift);
+                l += s[b][r];
+            }
+        if (d.drop_p > 0.f) drop_scores<G, NB>(a, s, w.b, h, i, t * KT, lane);
+        u32x4 pf[PC];
+#pragma unroll
+        for (int c = 0; c < PC; ++c) pf[c] = score_frag<T, G, NB>(s, c);
+        fragment_loop<T, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(vs, (n % MT) * G, 0, n / MT); },
+                                  [&](int n, u32x4 x) __attribute__((always_inline)) { o[n % MT] = mma<T, G>(x, pf[n / MT], o[n % MT]); });
+    };
+    for (int t = t0; t < t1; t += 2) {
+        tile(t, k0, v0, k1, v1);
+        if (t + 1 < t1) tile(t + 1, k1, v1, k0, v0);
+    }
+    write_rows<T, DH, G>(a, w, o, m, l, i, h, ok, lane);
+}
+
 // joins the partial outputs of a split launch: one wave per row
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
@@ -183,6 +274,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 }
 
 // ---- host side
+int attn_lds_limit(const void* fn, int bytes) {
+    if (func_attr_once(fn) && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        set_error("attention: cannot raise the LDS limit");
+        return EKAID_ERR_LAUNCH;
+    }
+    return EKAID_OK;
+}
+
 int attn_check(const ekaid_attn_t* a, const char* who) {
     if (!a) { set_error("%s: null descriptor", who); return EKAID_ERR_ARG; }
     if (a->dtype < EKAID_F32 || a->dtype > EKAID_F16) { set_error("%s: dtype %d", who, a->dtype); return EKAID_ERR_ARG; }
@@ -213,18 +313,35 @@ int attn_check(const ekaid_attn_t* a, const char* who) {
     return EKAID_OK;
 }
 
-struct FwdPlan { int g, nw, gp, tiles, splits, kt; size_t ws; };
+struct FwdPlan { int few, g, nw, gp, tiles, splits, kt; size_t ws; };
+
+// Waves of 16 rows: as few rows as possible beyond R (a wave on rows that do not exist costs as much as one on rows that do)
+int waves_for_rows(int R) {
+    int best = 4, cost = 1 << 30;
+    for (int nw = 4; nw >= 1; nw >>= 1) {
+        const int c = cdiv(R, 16 * nw) * 16 * nw * (nw == 4 ? 8 : nw == 2 ? 9 : 12);      // smaller workgroups copy the tiles more often
+        if (c < cost) { cost = c; best = nw; }
+    }
+    return best;
+}
 
 static FwdPlan fwd_plan(const ekaid_attn_t* a) {
     FwdPlan p;
     const int group = a->H / a->KV;
-    p.gp = a->Lq < 32 && group > 1 && (!a->table || group * (2 * a->reach + 1) <= 8192) ? group : 1;
+    const bool wide32 = a->dtype == EKAID_F32 && a->dh > 128;
+    p.few = a->Lq < 17;
+    p.gp = p.few && group > 1 && (!a->table || group * (2 * a->reach + 1) <= 8192) ? group : 1;
     const int R = a->Lq * p.gp;
-    p.g = R <= 64 || (a->dtype == EKAID_F32 && a->dh > 128) ? 16 : 32;
-    p.nw = R <= 16 ? 1 : R <= 32 && p.g == 16 ? 2 : 4;
-    if (a->dtype == EKAID_F32 && a->dh > 128 && p.nw == 1) p.nw = 2;      // one wave would have to hold a whole staged tile: it spills
-    p.kt = a->dh > 128 ? 32 : 64;
-    if (a->dtype == EKAID_F32 && a->dh > 64) p.kt = 32;
+    if (p.few) {
+        p.g = R <= 64 || wide32 ? 16 : 32;
+        p.nw = R <= 16 ? 1 : R <= 32 && p.g == 16 ? 2 : 4;
+        if (wide32 && p.nw == 1) p.nw = 2;      // one wave would have to hold a whole staged tile: it spills
+        p.kt = a->dh > 128 || (a->dtype == EKAID_F32 && a->dh > 64) ? 32 : 64;
+    } else {
+        p.g = R <= 64 || wide32 ? 16 : 32;
+        p.nw = p.g == 32 ? 4 : waves_for_rows(R);
+        p.kt = attn_kt(a->dtype == EKAID_F32 ? 4 : 2, a->dh, p.g);
+    }
     p.tiles = cdiv(R, p.g * p.nw);
     const long long wgs = (long long)a->B * (a->H / p.gp) * p.tiles;
     const int key_tiles = cdiv(a->Lk, p.kt);
@@ -238,25 +355,35 @@ static FwdPlan fwd_plan(const ekaid_attn_t* a) {
     return p;
 }
 
-template <typename T, int DH, int G, int NW, int KT> static int launch_fwd(const AttnArgs& a, int grid, hipStream_t st) {
+template <typename T, int DH, int G, int NW, int KT> static int launch_few(const AttnArgs& a, int grid, hipStream_t st) {
     constexpr size_t base = (size_t)KT * (Ld<T, DH>::row + Ld<T, DH>::col) * sizeof(T) + KT;
     const size_t lds = base + (a.d.table ? (size_t)a.gp * (2 * a.d.reach + 1) * 4 : 0);
-    const void* fn = (const void*)attn_fwd_kernel<T, DH, G, NW, KT>;
-    if (func_attr_once(fn) && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) {
-        set_error("attn_fwd: cannot raise the LDS limit");
-        return EKAID_ERR_LAUNCH;
-    }
+    if (int rc = attn_lds_limit((const void*)attn_fwd_kernel<T, DH, G, NW, KT>, 160 * 1024)) return rc;
     hipLaunchKernelGGL((attn_fwd_kernel<T, DH, G, NW, KT>), dim3(grid), dim3(64 * NW), lds, st, a);
     return check_launch("attn_fwd");
 }
+template <typename T, int DH, int G, int NW> static int launch_tile(const AttnArgs& a, int grid, hipStream_t st) {
+    constexpr int KT = attn_kt((int)sizeof(T), DH, G);
+    const size_t lds = (a.d.table ? (size_t)(2 * (a.d.reach + BIAS_PAD) + 1) * 4 : 0) + 4 * KT;
+    if (int rc = attn_lds_limit((const void*)attn_tile_fwd_kernel<T, DH, G, NW, KT>, 96 * 1024)) return rc;
+    hipLaunchKernelGGL((attn_tile_fwd_kernel<T, DH, G, NW, KT>), dim3(grid), dim3(64 * NW), lds, st, a);
+    return check_launch("attn_fwd");
+}
 template <typename T, int DH> static int pick_fwd(const AttnArgs& a, const FwdPlan& p, int grid, hipStream_t st) {
-    constexpr int KT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
+    if (p.few) {
+        constexpr int KT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
+        if constexpr (!(sizeof(T) == 4 && DH > 128)) {
+            if (p.g == 32) return launch_few<T, DH, 32, 4, KT>(a, grid, st);
+            if (p.nw == 1) return launch_few<T, DH, 16, 1, KT>(a, grid, st);
+        }
+        if (p.nw == 2) return launch_few<T, DH, 16, 2, KT>(a, grid, st);
+        return launch_few<T, DH, 16, 4, KT>(a, grid, st);
+    }
     if constexpr (!(sizeof(T) == 4 && DH > 128))
-        if (p.g == 32) return launch_fwd<T, DH, 32, 4, KT>(a, grid, st);
-    if constexpr (!(sizeof(T) == 4 && DH > 128))
-        if (p.nw == 1) return launch_fwd<T, DH, 16, 1, KT>(a, grid, st);
-    if (p.nw == 2) return launch_fwd<T, DH, 16, 2, KT>(a, grid, st);
-    return launch_fwd<T, DH, 16, 4, KT>(a, grid, st);
+        if (p.g == 32) return launch_tile<T, DH, 32, 4>(a, grid, st);
+    if (p.nw == 1) return launch_tile<T, DH, 16, 1>(a, grid, st);
+    if (p.nw == 2) return launch_tile<T, DH, 16, 2>(a, grid, st);
+    return launch_tile<T, DH, 16, 4>(a, grid, st);
 }
 template <typename T> static int run_fwd(const AttnArgs& a, const FwdPlan& p, hipStream_t st) {
     const int grid = a.d.B * (a.d.H / p.gp) * p.tiles * p.splits;

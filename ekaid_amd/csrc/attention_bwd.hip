@@ -17,33 +17,38 @@ template <typename T> __device__ __forceinline__ float ds_scale(float norm2) {
     } else return 1.f;
 }
 
+// dq (and the bias table's partial sums): lane = query row.  Units of 32 keys of a tile: scores and dP of a unit, then its share of dq.
 template <typename T, int DH, int G, int NW, int KT, bool REL>
-__global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
-    constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
-    constexpr int LD = Ld<T, DH>::row, nq = Blk<G>::nq, ng = Blk<G>::ng;
+__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void attn_dq_kernel(const AttnArgs a) {
+    constexpr int NT = 64 * NW, U = KT < 32 ? KT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
+    constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng, nv = 4 * nq;
+    __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + KT * LD;
-    unsigned char* kms = reinterpret_cast<unsigned char*>(Vs + KT * LD);
-    float* red = reinterpret_cast<float*>(kms + KT);          // [NW] row-norm maxima
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
-    float* bias = red + NW;                                   // [width]
-    float* dsum = bias + width;                               // [NW][width]: this wave's sums of score gradients by distance
+    float* red = reinterpret_cast<float*>(smem);              // [NW] row-norm maxima
+    float* bias = red + NW;                                   // padded table of the head
+    float* dsum = bias + (REL ? width + 2 * BIAS_PAD : 0);    // [NW][width]: this wave's sums of score gradients by distance
     float* skew = dsum + NW * width + wave * G * (G + 1);     // [NW][G][G + 1]
+    unsigned char* kms = reinterpret_cast<unsigned char*>(dsum + NW * width + (REL ? NW * G * (G + 1) : 0));
     const RowWork w(a);
     const ekaid_attn_t& d = a.d;
-    const int h = w.head0, row0 = (w.tile * NW + wave) * G, i0 = row0 + lane % G;
-    const bool ok = i0 < d.Lq;
-    const int i = ok ? i0 : 0, p0 = query_pos(d, w.b), pos = p0 + i0, len = key_len(d, w.b);
-    int kend = len;
-    if (d.causal) kend = max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G)));
+    const int h = w.head0, row0 = (w.tile * NW + wave) * G;
+    const bool ok = row0 + lane % G < d.Lq, live = row0 < d.Lq;
+    const int i = min(row0 + lane % G, d.Lq - 1), p0 = query_pos(d, w.b), pos = p0 + i, pmin = p0 + min(row0, d.Lq - 1), pmax = p0 + min(row0 + G, d.Lq) - 1;
+    const int len = key_len(d, w.b), kend = d.causal ? max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G))) : len;
     const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
-    const unsigned char* mask = d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr;
     if constexpr (REL) {
-        fill_bias(d, bias, h, 1, tid, NT);
+        fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
         for (int x = tid; x < NW * width; x += NT) dsum[x] = 0.f;
+        __syncthreads();
     }
+    MaskRing<KT> ring;
+    ring.init(d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr, kms, len, t0, tid);
 
+    TileFrag<T, DH, G> tf(lane);
+    TileCopy<T, DH, KT, NW> ck, cv;
+    ck.init(reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh, d.k_row, lane);
+    cv.init(reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh, d.v_row, lane);
     u32x4 qf[NC], gf[NC];
     const long long orow = ((long long)w.b * d.Lq + i) * d.H * d.dh + (long long)h * d.dh;
     const T* qrow = reinterpret_cast<const T*>(d.q) + w.b * d.q_batch + i * d.q_row + (long long)h * d.dh;
@@ -62,6 +67,10 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
             n2 += x * x;
         }
     }
+    if (t0 < t1) {
+        ck.issue(k0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+        cv.issue(v0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+    }
     delta = across_groups_sum<G>(delta);
     n2 = across_groups_sum<G>(n2);
     const long long srow = ((long long)w.b * d.H + h) * d.Lq + i;
@@ -69,69 +78,52 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
     if (ok && g == 0 && w.split == 0) a.delta[srow] = delta;
     const float rs = ds_scale<T>(n2);
     if constexpr (__is_same(T, _Float16)) {
-        float mx = wave_max(n2);
+        const float mx = wave_max(n2);
         if (lane == 0) red[wave] = mx;
     }
-
-    const T* kb = reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh;
-    const T* vb = reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh;
-    Stage<T, DH, KT, NT> sk, sv;
     typename Blk<G>::acc o[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
     float far_back = 0.f, far_ahead = 0.f;
-    if (t0 < t1) {
-        sk.load(kb, d.k_row, t0 * KT, len, d.dh, mask, tid);
-        sv.load(vb, d.v_row, t0 * KT, len, d.dh, mask, tid);
-    }
-    for (int t = t0; t < t1; ++t) {
-        sk.store(Ks, LD, tid);
-        sv.store(Vs, LD, tid);
-        if (mask) for (int j = tid; j < KT; j += NT) kms[j] = t * KT + j < len ? mask[t * KT + j] : 0;
-        __syncthreads();
-        if (t + 1 < t1) {
-            sk.load(kb, d.k_row, (t + 1) * KT, len, d.dh, mask, tid);
-            sv.load(vb, d.v_row, (t + 1) * KT, len, d.dh, mask, tid);
-        }
+    const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
+
+    auto unit = [&](int j0, const T* ks, const T* vs, int r0, const unsigned char* km) __attribute__((always_inline)) {
+        if constexpr (DH * sizeof(T) > 128) tf.refresh();
         typename Blk<G>::acc s[NB], dp[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             s[b] = zero_acc<G>();
             dp[b] = zero_acc<G>();
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s[b] = mma<T, G>(row_frag<T, G>(Ks, LD, b * G, c, lane), qf[c], s[b]);
-                dp[b] = mma<T, G>(row_frag<T, G>(Vs, LD, b * G, c, lane), gf[c], dp[b]);
-            }
         }
-        const bool partial = mask || (t + 1) * KT > len || (d.causal && (t + 1) * KT > p0 + w.tile * NW * G + 1);
-        finish_scores<G, NB>(a, s, t * KT, len, pos, REL ? bias : nullptr, mask ? kms : nullptr, partial, lane);
+        fragment_loop<T, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? vs : ks, r0 + (n / 2 % NB) * G, n / 2 / NB); },
+                                      [&](int n, u32x4 x) __attribute__((always_inline)) {
+                                          const int b = n / 2 % NB, c = n / 2 / NB;
+                                          if (n & 1) dp[b] = mma<T, G>(x, gf[c], dp[b]);
+                                          else s[b] = mma<T, G>(x, qf[c], s[b]);
+                                      });
+        const Affine f = scores_by_row<G, NB>(a, s, j0, len, pos, pmin, pmax, REL ? bias : nullptr, km, lane);
+        const float shift = f.add - lse;
         if (d.drop_p > 0.f) {
-            const uint64_t seed = drop_seed_value(a.seed);
 #pragma unroll
             for (int q = 0; q < NB * nq; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    dp[q / nq][4 * (q % nq) + e] *= drop_keep(a, seed, w.b, h, i, t * KT + 4 * ng * q + 4 * g + e);
+                for (int e = 0; e < 4; ++e) dp[q / nq][4 * (q % nq) + e] *= drop_keep(a, seed, w.b, h, i, j0 + 4 * ng * q + 4 * g + e);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4 * nq; ++r) {
-                const float p = __builtin_amdgcn_exp2f(s[b][r] - lse);
-                s[b][r] = p == 0.f ? 0.f : p * (dp[b][r] - delta);
-            }
+            for (int r = 0; r < nv; ++r) s[b][r] = __builtin_amdgcn_exp2f(s[b][r] * f.mult + shift) * (dp[b][r] - delta);
         if constexpr (REL) {
             // sums over equal distance j - pos: a block that lies wholly beyond the reach goes to one bucket; otherwise the block is written
             // to LDS and lane x adds up diagonal x (rows ascending: a fixed order), whose distance no other lane of the wave holds
             const int prow = p0 + row0;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const int jb = t * KT + b * G;
+                const int jb = j0 + b * G;
                 if (jb + G - 1 - prow <= -d.reach || jb - (prow + G - 1) >= d.reach) {
                     float x = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4 * nq; ++r) x += s[b][r];
+                    for (int r = 0; r < nv; ++r) x += s[b][r];
                     if (jb - prow < 0) far_back += x; else far_ahead += x;
                 } else {
                     wave_fence();
@@ -156,20 +148,38 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
                 }
             }
         }
+        if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4 * nq; ++r) s[b][r] *= rs;
-#pragma unroll
-        for (int c = 0; c < PC; ++c) {
-            const u32x4 sf = score_frag<T, G, NB>(s, c);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o[mt] = mma<T, G>(col_frag<T, G>(Ks, LD, mt * G, c, lane), sf, o[mt]);
+                for (int r = 0; r < nv; ++r) s[b][r] *= rs;
         }
-        __syncthreads();
+        u32x4 sf[PC];
+#pragma unroll
+        for (int c = 0; c < PC; ++c) sf[c] = score_frag<T, G, NB>(s, c);
+        fragment_loop<T, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(ks, (n % MT) * G, r0, n / MT); },
+                                  [&](int n, u32x4 x) __attribute__((always_inline)) { o[n % MT] = mma<T, G>(x, sf[n / MT], o[n % MT]); });
+    };
+    auto tile = [&](int t, const T* ks, const T* vs, T* kn, T* vn) __attribute__((always_inline)) {
+        settle();
+        ring.step(t);
+        if (t + 1 < t1) {
+            ck.issue(kn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+            cv.issue(vn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+        }
+        const unsigned char* km = ring.tile(t);
+#pragma unroll
+        for (int u = 0; u < KT / U; ++u) {
+            const int j0 = t * KT + u * U;
+            if (live && j0 < kend && !(d.causal && j0 > pmax)) unit(j0, ks, vs, u * U, km ? km + u * U : nullptr);
+        }
+    };
+    for (int t = t0; t < t1; t += 2) {
+        tile(t, k0, v0, k1, v1);
+        if (t + 1 < t1) tile(t + 1, k1, v1, k0, v0);
     }
     if constexpr (REL) {
-        __syncthreads();                                      // (a workgroup without a key tile has not met its own zeroing yet)
+        __syncthreads();
         far_back = wave_sum(far_back);
         far_ahead = wave_sum(far_ahead);
         if (lane == 0) {
@@ -203,44 +213,37 @@ __global__ __launch_bounds__(64 * NW) void attn_dq_kernel(const AttnArgs a) {
     }
     if (!ok) return;
     const float f = d.scale / rs;
-    if (a.splits > 1) {
-        float* p = a.po + w.split * ((long long)d.B * d.Lq * d.H * d.dh) + orow;
+    float* part = a.po + w.split * ((long long)d.B * d.Lq * d.H * d.dh) + orow;
+    T* out = reinterpret_cast<T*>(d.dq) + orow;
 #pragma unroll
-        for (int q = 0; q < MT * nq; ++q) {
-            const int col = 4 * ng * q + 4 * g;
-            const auto& x = o[q / nq];
-            if (col < d.dh) store4<float>(p + col, x[4 * (q % nq)] * f, x[4 * (q % nq) + 1] * f, x[4 * (q % nq) + 2] * f, x[4 * (q % nq) + 3] * f);
-        }
-    } else {
-        T* p = reinterpret_cast<T*>(d.dq) + orow;
-#pragma unroll
-        for (int q = 0; q < MT * nq; ++q) {
-            const int col = 4 * ng * q + 4 * g;
-            const auto& x = o[q / nq];
-            if (col < d.dh) store4<T>(p + col, x[4 * (q % nq)] * f, x[4 * (q % nq) + 1] * f, x[4 * (q % nq) + 2] * f, x[4 * (q % nq) + 3] * f);
-        }
+    for (int q = 0; q < MT * nq; ++q) {
+        const int col = 4 * ng * q + 4 * g, r = 4 * (q % nq);
+        const auto& x = o[q / nq];
+        if (col >= d.dh) continue;
+        if (a.splits > 1) store4<float>(part + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
+        else store4<T>(out + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
     }
 }
 
-template <typename T, int DH, int G, int NW, int QT>
-__global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(const AttnArgs a) {
-    constexpr int NT = 64 * NW, NB = QT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = QT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
-    constexpr int LD = Ld<T, DH>::row, nq = Blk<G>::nq, ng = Blk<G>::ng;
+// dk, dv: lane = key; the rows of every head that shares it go by in tiles, in units of 32.  What a lane without a valid key computes stays in
+// that lane and is replaced by zero at the end.
+template <typename T, int DH, int G, int NW, int QT, bool REL>
+__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) void attn_dkv_kernel(const AttnArgs a) {
+    constexpr int NT = 64 * NW, U = QT < 32 ? QT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
+    constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng;
+    __shared__ __attribute__((aligned(16))) T q0s[QT * DH], q1s[QT * DH], g0s[QT * DH], g1s[QT * DH];
+    __shared__ __attribute__((aligned(16))) float l0s[QT], l1s[QT], d0s[QT], d1s[QT];      // log2 denominators, deltas
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Qs = reinterpret_cast<T*>(smem);
-    T* Ds = Qs + QT * LD;
-    float* ls = reinterpret_cast<float*>(Ds + QT * LD);       // [QT] log2 denominators (+inf: no such row)
-    float* dl = ls + QT;                                      // [QT] delta
-    float* bias = dl + QT;
+    float* bias = reinterpret_cast<float*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G;
     const ekaid_attn_t& d = a.d;
-    const int wi = die_order(blockIdx.x, gridDim.x), tile = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
+    const int wi = die_order(blockIdx.x, gridDim.x), tl = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
     const int b = bk / d.KV, kvh = bk % d.KV, group = d.H / d.KV;
-    const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tile * NW * G, j = j0 + wave * G + lane % G;
+    const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tl * NW * G, jw = j0 + wave * G, j = jw + lane % G;
     const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
-    const bool ok = j < len && (!mask || mask[j]);
-    const int qtiles = (d.Lq + QT - 1) / QT, first = d.causal ? min(qtiles, max(0, j0 - p0) / QT) : 0, live = qtiles - first;
-    const int items = j0 < len ? group * live : 0, per = (items + a.splits - 1) / a.splits, t0 = split * per, t1 = min(items, t0 + per);
+    const bool ok = j < len && (!mask || mask[j]), live = jw < len;
+    const int qtiles = (d.Lq + QT - 1) / QT, first = d.causal ? min(qtiles, max(0, j0 - p0) / QT) : 0, run = qtiles - first;
+    const int items = j0 < len ? group * run : 0, per = (items + a.splits - 1) / a.splits, t0 = split * per, t1 = min(items, t0 + per);
 
     u32x4 kf[NC], vf[NC];
     const int jr = ok ? j : 0;
@@ -258,75 +261,138 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(const AttnArgs a) {
         for (int x = lane; x < group * a.dq_parts; x += 64) mx = fmaxf(mx, n[x]);
         rs = ds_scale<T>(wave_max(mx));
     }
-    typename Blk<G>::acc ok_[MT], ov[MT];
+    typename Blk<G>::acc dk[MT], dv[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        ok_[mt] = zero_acc<G>();
-        ov[mt] = zero_acc<G>();
+        dk[mt] = zero_acc<G>();
+        dv[mt] = zero_acc<G>();
     }
-    Stage<T, DH, QT, NT> sq, sd;
-    auto fetch = [&](int t) {
-        const int h = kvh * group + t / live, q0 = (first + t % live) * QT;
-        sq.load(reinterpret_cast<const T*>(d.q) + b * d.q_batch + (long long)h * d.dh, d.q_row, q0, d.Lq, d.dh, nullptr, tid);
-        sd.load(reinterpret_cast<const T*>(d.dout) + (long long)b * d.Lq * d.H * d.dh + (long long)h * d.dh, (long long)d.H * d.dh, q0, d.Lq, d.dh,
-                nullptr, tid);
+    TileFrag<T, DH, G> tf(lane);
+    TileCopy<T, DH, QT, NW> cq, cg;
+    auto fetch = [&](int t, T* qs, T* gs, float* ls, float* ds) __attribute__((always_inline)) {
+        const int h = kvh * group + t / run, r0 = (first + t % run) * QT;
+        cq.init(reinterpret_cast<const T*>(d.q) + b * d.q_batch + (long long)h * d.dh, d.q_row, lane);
+        cg.init(reinterpret_cast<const T*>(d.dout) + (long long)b * d.Lq * d.H * d.dh + (long long)h * d.dh, (long long)d.H * d.dh, lane);
+        cq.issue(qs, r0, d.Lq, d.dh, nullptr, wave);
+        cg.issue(gs, r0, d.Lq, d.dh, nullptr, wave);
+        const long long row = ((long long)b * d.H + h) * d.Lq + min(r0 + lane, d.Lq - 1);
+        if (lane < QT) {
+            if (wave == 0) __builtin_amdgcn_global_load_lds((global_void)(d.lse + row), (lds_void)ls, 4, 0, 0);
+            if (wave == NW - 1) __builtin_amdgcn_global_load_lds((global_void)(a.delta + row), (lds_void)ds, 4, 0, 0);
+        }
     };
-    if (t0 < t1) fetch(t0);
-    int bias_head = -1;
-    for (int t = t0; t < t1; ++t) {
-        const int h = kvh * group + t / live, q0 = (first + t % live) * QT;
-        const long long srow = ((long long)b * d.H + h) * d.Lq;
-        sq.store(Qs, LD, tid);
-        sd.store(Ds, LD, tid);
-        for (int x = tid; x < QT; x += NT) {
-            ls[x] = q0 + x < d.Lq ? d.lse[srow + q0 + x] : POS_INF;
-            dl[x] = q0 + x < d.Lq ? a.delta[srow + q0 + x] : 0.f;
-        }
-        if (d.table && bias_head != h) {
-            fill_bias(d, bias, h, 1, tid, NT);
-            bias_head = h;
-        }
-        __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
+    const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
+    // rows i0 .. i0 + U of head h, at tile row r0
+    auto unit = [&](int h, int i0, int r0, const T* qs, const T* gs, const float* ls, const float* ds) __attribute__((always_inline)) {
+        if constexpr (DH * sizeof(T) > 128) tf.refresh();
         typename Blk<G>::acc s[NB], dp[NB];
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
             s[x] = zero_acc<G>();
             dp[x] = zero_acc<G>();
+        }
+        fragment_loop<T, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? gs : qs, r0 + (n / 2 % NB) * G, n / 2 / NB); },
+                                      [&](int n, u32x4 x) __attribute__((always_inline)) {
+                                          const int y = n / 2 % NB, c = n / 2 / NB;
+                                          if (n & 1) dp[y] = mma<T, G>(x, vf[c], dp[y]);
+                                          else s[y] = mma<T, G>(x, kf[c], s[y]);
+                                      });
+        const int pu = p0 + i0;                               // position of the unit's first row
+        const bool masked = i0 + U > d.Lq || (d.causal && jw + G - 1 > pu);
+        float mult = a.sc2, add = 0.f;
+        if constexpr (REL) {
+            bool near = false;
+            if (jw + G - 1 - pu <= -d.reach) add = bias[BIAS_PAD];
+            else if (jw - (pu + U - 1) >= d.reach) add = bias[2 * d.reach + BIAS_PAD];
+            else near = true;
+            if (near) {
+                const float* bj = bias + (j - pu - 4 * g + d.reach + BIAS_PAD);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s[x] = mma<T, G>(row_frag<T, G>(Qs, LD, x * G, c, lane), kf[c], s[x]);
-                dp[x] = mma<T, G>(row_frag<T, G>(Ds, LD, x * G, c, lane), vf[c], dp[x]);
+                for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[q / nq][4 * (q % nq) + e] = s[q / nq][4 * (q % nq) + e] * mult + bj[-(4 * ng * q + e)];
+                mult = 1.f;
             }
         }
-        const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
 #pragma unroll
         for (int q = 0; q < NB * nq; ++q) {
-            const int iq = 4 * ng * q + 4 * g;
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + iq), d4 = *reinterpret_cast<const f32x4*>(dl + iq);
+            const int iq = r0 + 4 * ng * q + 4 * g;
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + iq), d4 = *reinterpret_cast<const f32x4*>(ds + iq);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = 4 * (q % nq) + e, i = q0 + iq + e, rel = j - (p0 + i);
-                float x = s[q / nq][r] * a.sc2;
-                if (d.table) x += bias[min(max(rel, -d.reach), d.reach) + d.reach];
-                float p = __builtin_amdgcn_exp2f(x - l4[e]);
-                if (!ok || l4[e] == POS_INF || (d.causal && rel > 0)) p = 0.f;
-                float keep = 1.f;
-                if (d.drop_p > 0.f) keep = drop_keep(a, seed, b, h, i, j);
-                dp[q / nq][r] = p == 0.f ? 0.f : p * (dp[q / nq][r] * keep - d4[e]) * rs;
-                s[q / nq][r] = p * keep;
+                const int r = 4 * (q % nq) + e;
+                float x = s[q / nq][r] * mult - l4[e];
+                if constexpr (REL) x += add;
+                s[q / nq][r] = __builtin_amdgcn_exp2f(x);
+                dp[q / nq][r] -= d4[e];
             }
         }
+        if (masked) {
+#pragma unroll
+            for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = 4 * ng * q + 4 * g + e;
+                    if (i0 + k >= d.Lq || (d.causal && j > pu + k)) s[q / nq][4 * (q % nq) + e] = 0.f;
+                }
+        }
+        if (d.drop_p > 0.f) {
+#pragma unroll
+            for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * (q % nq) + e, k = 4 * ng * q + 4 * g + e;
+                    const float keep = drop_keep(a, seed, b, h, i0 + k, j), dl = ds[r0 + k], p = s[q / nq][r];
+                    dp[q / nq][r] = p * ((dp[q / nq][r] + dl) * keep - dl);
+                    s[q / nq][r] = p * keep;
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int r = 0; r < 4 * nq; ++r) dp[x][r] *= s[x][r];
+        }
+        if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int r = 0; r < 4 * nq; ++r) dp[x][r] *= rs;
+        }
+        u32x4 pf[PC], df[PC];
 #pragma unroll
         for (int c = 0; c < PC; ++c) {
-            const u32x4 pf = score_frag<T, G, NB>(s, c), df = score_frag<T, G, NB>(dp, c);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                ov[mt] = mma<T, G>(col_frag<T, G>(Ds, LD, mt * G, c, lane), pf, ov[mt]);
-                ok_[mt] = mma<T, G>(col_frag<T, G>(Qs, LD, mt * G, c, lane), df, ok_[mt]);
+            pf[c] = score_frag<T, G, NB>(s, c);
+            df[c] = score_frag<T, G, NB>(dp, c);
+        }
+        fragment_loop<T, PC * MT * 2>([&](int n) __attribute__((always_inline)) { return tf.cols(n & 1 ? qs : gs, (n / 2 % MT) * G, r0, n / 2 / MT); },
+                                      [&](int n, u32x4 x) __attribute__((always_inline)) {
+                                          const int mt = n / 2 % MT, c = n / 2 / MT;
+                                          if (n & 1) dk[mt] = mma<T, G>(x, df[c], dk[mt]);
+                                          else dv[mt] = mma<T, G>(x, pf[c], dv[mt]);
+                                      });
+    };
+    int bias_head = -1;
+    auto tile = [&](int t, const T* qs, const T* gs, const float* ls, const float* ds, T* qn, T* gn, float* ln, float* dn) __attribute__((always_inline)) {
+        const int h = kvh * group + t / run, i0 = (first + t % run) * QT;
+        settle();
+        if constexpr (REL) {
+            if (bias_head != h) {
+                fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
+                bias_head = h;
+                __syncthreads();
             }
         }
-        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1, qn, gn, ln, dn);
+#pragma unroll
+        for (int u = 0; u < QT / U; ++u) {
+            const int iu = i0 + u * U;
+            if (live && iu < d.Lq && !(d.causal && jw > p0 + iu + U - 1)) unit(h, iu, u * U, qs, gs, ls, ds);
+        }
+    };
+    if (t0 < t1) fetch(t0, q0s, g0s, l0s, d0s);
+    for (int t = t0; t < t1; t += 2) {
+        tile(t, q0s, g0s, l0s, d0s, q1s, g1s, l1s, d1s);
+        if (t + 1 < t1) tile(t + 1, q1s, g1s, l1s, d1s, q0s, g0s, l0s, d0s);
     }
     if (j >= d.Lk) return;
     const float f = d.scale / rs;
@@ -336,14 +402,18 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv_kernel(const AttnArgs a) {
     for (int q = 0; q < MT * nq; ++q) {
         const int col = 4 * ng * q + 4 * g, r = 4 * (q % nq);
         if (col >= d.dh) continue;
-        const auto& x = ok_[q / nq];
-        const auto& y = ov[q / nq];
+        f32x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = ok ? dk[q / nq][r + e] * f : 0.f;
+            y[e] = ok ? dv[q / nq][r + e] : 0.f;
+        }
         if (a.splits > 1) {
-            store4<float>(a.pk + split * n + row + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
-            store4<float>(a.pv + split * n + row + col, y[r], y[r + 1], y[r + 2], y[r + 3]);
+            store4<float>(a.pk + split * n + row + col, x[0], x[1], x[2], x[3]);
+            store4<float>(a.pv + split * n + row + col, y[0], y[1], y[2], y[3]);
         } else {
-            store4<T>(reinterpret_cast<T*>(d.dk) + row + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
-            store4<T>(reinterpret_cast<T*>(d.dv) + row + col, y[r], y[r + 1], y[r + 2], y[r + 3]);
+            store4<T>(reinterpret_cast<T*>(d.dk) + row + col, x[0], x[1], x[2], x[3]);
+            store4<T>(reinterpret_cast<T*>(d.dv) + row + col, y[0], y[1], y[2], y[3]);
         }
     }
 }
@@ -376,18 +446,17 @@ struct BwdPlan {
     int gk, nwk, tk, sk;        // dk / dv
     size_t delta, nrm, tab, po, pk, total;      // float offsets
 };
-static int bwd_tile(const ekaid_attn_t* a) { return a->dh > 128 || (a->dtype == EKAID_F32 && a->dh > 64) ? 32 : 64; }
 static size_t align4(size_t n) { return (n + 3) & ~(size_t)3; }
 
 static BwdPlan bwd_plan(const ekaid_attn_t* a) {
     BwdPlan p;
-    const int kt = bwd_tile(a);
-    p.gq = a->Lq <= 64 || (a->dtype == EKAID_F32 && a->dh > 128) ? 16 : 32;
-    const bool wide = a->dtype == EKAID_F32 && a->dh > 128;       // one wave would have to hold a whole staged tile: it spills
-    p.nwq = wide ? 4 : a->Lq <= 16 ? 1 : a->Lq <= 32 && p.gq == 16 ? 2 : 4;
+    const int esz = a->dtype == EKAID_F32 ? 4 : 2;
+    // blocks of 32 need the registers of one wave a SIMD at 256 wide heads (f32) / 128 wide dk, dv: blocks of 16 there and for few rows
+    p.gq = a->Lq <= 64 || (esz == 4 && a->dh > 128) ? 16 : 32;
+    p.nwq = p.gq == 32 ? 4 : waves_for_rows(a->Lq);
     p.tq = cdiv(a->Lq, p.gq * p.nwq);
     p.gk = a->Lk <= 64 || a->dh > 128 ? 16 : 32;
-    p.nwk = wide ? 4 : a->Lk <= 16 ? 1 : a->Lk <= 32 ? 2 : 4;
+    p.nwk = p.gk == 32 ? 4 : waves_for_rows(a->Lk);
     p.tk = cdiv(a->Lk, p.gk * p.nwk);
     auto split = [](long long wgs, int waves, int work) {
         const long long want = 4 * 512 / waves;
@@ -395,8 +464,8 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
         if (s > (work + 1) / 2) s = (work + 1) / 2;
         return (int)(s < 1 ? 1 : s);
     };
-    p.sq = split((long long)a->B * a->H * p.tq, p.nwq, cdiv(a->Lk, kt));
-    p.sk = split((long long)a->B * a->KV * p.tk, p.nwk, cdiv(a->Lq, kt) * (a->H / a->KV));
+    p.sq = split((long long)a->B * a->H * p.tq, p.nwq, cdiv(a->Lk, attn_kt(esz, a->dh, p.gq)));
+    p.sk = split((long long)a->B * a->KV * p.tk, p.nwk, cdiv(a->Lq, attn_kt(esz, a->dh, p.gk)) * (a->H / a->KV));
     const size_t rows = (size_t)a->B * a->H * a->Lq, bh = (size_t)a->B * a->H;
     const int nb = a->table ? (a->n_border + 1) * (a->bidirectional ? 2 : 1) : 0;
     size_t o = 0;
@@ -410,45 +479,34 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
 }
 size_t attn_bwd_workspace(const ekaid_attn_t* a) { return bwd_plan(a).total; }
 
-static int lds_limit(const void* fn) {
-    if (func_attr_once(fn) && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) {
-        set_error("attn_bwd: cannot raise the LDS limit");
-        return EKAID_ERR_LAUNCH;
-    }
-    return EKAID_OK;
-}
-template <typename T, int DH, int G, int NW, int KT, bool REL> static int launch_dq(const AttnArgs& a, hipStream_t st) {
-    size_t lds = (size_t)2 * KT * Ld<T, DH>::row * sizeof(T) + KT + 4 * NW;
-    if (REL) lds += 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + NW * G * (G + 1));
-    if (int rc = lds_limit((const void*)attn_dq_kernel<T, DH, G, NW, KT, REL>)) return rc;
+template <typename T, int DH, int G, int NW, bool REL> static int launch_dq(const AttnArgs& a, hipStream_t st) {
+    constexpr int KT = attn_kt((int)sizeof(T), DH, G);
+    size_t lds = 4 * NW + 4 * KT;
+    if (REL) lds += 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + 2 * BIAS_PAD + NW * G * (G + 1));
+    if (int rc = attn_lds_limit((const void*)attn_dq_kernel<T, DH, G, NW, KT, REL>, 96 * 1024)) return rc;
     hipLaunchKernelGGL((attn_dq_kernel<T, DH, G, NW, KT, REL>), dim3(a.d.B * a.d.H * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
     return check_launch("attn_dq");
 }
 template <typename T, int DH, bool REL> static int pick_dq(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-    constexpr int KT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
     if constexpr (!(sizeof(T) == 4 && DH > 128))
-        if (p.gq == 32) return launch_dq<T, DH, 32, 4, KT, REL>(a, st);
-    if constexpr (!(sizeof(T) == 4 && DH > 128)) {
-        if (p.nwq == 1) return launch_dq<T, DH, 16, 1, KT, REL>(a, st);
-        if (p.nwq == 2) return launch_dq<T, DH, 16, 2, KT, REL>(a, st);
-    }
-    return launch_dq<T, DH, 16, 4, KT, REL>(a, st);
+        if (p.gq == 32) return launch_dq<T, DH, 32, 4, REL>(a, st);
+    if (p.nwq == 1) return launch_dq<T, DH, 16, 1, REL>(a, st);
+    if (p.nwq == 2) return launch_dq<T, DH, 16, 2, REL>(a, st);
+    return launch_dq<T, DH, 16, 4, REL>(a, st);
 }
-template <typename T, int DH, int G, int NW, int QT> static int launch_dkv(const AttnArgs& a, hipStream_t st) {
-    const size_t lds = (size_t)2 * QT * Ld<T, DH>::row * sizeof(T) + 8 * QT + (a.d.table ? 4 * (2 * a.d.reach + 1) : 0);
-    if (int rc = lds_limit((const void*)attn_dkv_kernel<T, DH, G, NW, QT>)) return rc;
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DH, G, NW, QT>), dim3(a.d.B * a.d.KV * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
+template <typename T, int DH, int G, int NW, bool REL> static int launch_dkv(const AttnArgs& a, hipStream_t st) {
+    constexpr int QT = attn_kt((int)sizeof(T), DH, G);
+    const size_t lds = REL ? 4 * (2 * (a.d.reach + BIAS_PAD) + 1) : 0;
+    if (int rc = attn_lds_limit((const void*)attn_dkv_kernel<T, DH, G, NW, QT, REL>, 92 * 1024)) return rc;
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DH, G, NW, QT, REL>), dim3(a.d.B * a.d.KV * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
     return check_launch("attn_dkv");
 }
-template <typename T, int DH> static int pick_dkv(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-    constexpr int QT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
+template <typename T, int DH, bool REL> static int pick_dkv(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
     if constexpr (DH <= 128)
-        if (p.gk == 32) return launch_dkv<T, DH, 32, 4, QT>(a, st);
-    if constexpr (!(sizeof(T) == 4 && DH > 128)) {
-        if (p.nwk == 1) return launch_dkv<T, DH, 16, 1, QT>(a, st);
-        if (p.nwk == 2) return launch_dkv<T, DH, 16, 2, QT>(a, st);
-    }
-    return launch_dkv<T, DH, 16, 4, QT>(a, st);
+        if (p.gk == 32) return launch_dkv<T, DH, 32, 4, REL>(a, st);
+    if (p.nwk == 1) return launch_dkv<T, DH, 16, 1, REL>(a, st);
+    if (p.nwk == 2) return launch_dkv<T, DH, 16, 2, REL>(a, st);
+    return launch_dkv<T, DH, 16, 4, REL>(a, st);
 }
 template <typename T> static int sum_parts(const float* part, void* out, long long n, int splits, hipStream_t st) {
     hipLaunchKernelGGL(attn_sum_kernel<T>, dim3((int)std::min<long long>((n / 4 + 255) / 256, 4096)), dim3(256), 0, st, part, (T*)out, n, splits);
@@ -475,7 +533,10 @@ template <typename T> static int run_bwd(AttnArgs a, const BwdPlan& p, hipStream
     if (d.Lk == 0) return EKAID_OK;
     a.tiles = p.tk;
     a.splits = p.sk;
-    rc = d.dh <= 64 ? pick_dkv<T, 64>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128>(a, p, st) : pick_dkv<T, 256>(a, p, st);
+    if (d.table)
+        rc = d.dh <= 64 ? pick_dkv<T, 64, true>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128, true>(a, p, st) : pick_dkv<T, 256, true>(a, p, st);
+    else
+        rc = d.dh <= 64 ? pick_dkv<T, 64, false>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128, false>(a, p, st) : pick_dkv<T, 256, false>(a, p, st);
     if (rc || p.sk == 1) return rc;
     const long long n = (long long)d.B * d.Lk * d.KV * d.dh;
     if ((rc = sum_parts<T>(a.pk, d.dk, n, p.sk, st))) return rc;

@@ -8,6 +8,8 @@
 // CONTRACTION, and the other operand is fetched in the same order -- by transposing LDS reads for 16-bit types, by plain reads for f32.
 #pragma once
 #include "common.h"
+#include <type_traits>
+#include <utility>
 #include "../../include/ekaid_hip.h"
 
 namespace ekaid {
@@ -180,6 +182,144 @@ template <typename T, int DH, int ROWS, int NT> struct Stage {
     }
 };
 
+// ---- tiles copied to LDS without passing registers
+// A tile is ROWS rows x DH elements, rows packed (no padding: a wave writes 1 KB in lane order), the 16-byte slots of a row permuted by an
+// exclusive-or with swz(row) so that both kinds of reads spread over the banks: 16 rows at one slot (row fragments), and 4 consecutive
+// rows over 64 bytes (transposing reads) or two rows 4 apart over 128 bytes (f32 columns).  The permutation is applied to the global
+// address.  Rows that do not exist or are masked, and columns beyond dh, are read from a zero vector: NaN or Inf there never arrives.
+__device__ __attribute__((aligned(16))) const uint32_t attn_zero16[4] = {0u, 0u, 0u, 0u};
+typedef __attribute__((address_space(3))) void* lds_void;
+typedef const __attribute__((address_space(1))) void* global_void;
+
+template <typename T, int DH> __device__ __host__ __forceinline__ constexpr int swz(int row) {
+    if constexpr (DH * sizeof(T) == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    else if constexpr (sizeof(T) == 2) return (row & 3) << 2 | ((row >> 2) & 3);
+    else return ((row >> 2) & 1) << 3 | (row & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 3) & 1);
+}
+template <typename T, int DH, int ROWS, int NW> struct TileCopy {
+    static constexpr int epl = Elem<T>::epl, rb = DH * (int)sizeof(T), per = 1024 / rb > 0 ? 1024 / rb : 1, lanes = rb / 16, chunks = ROWS * rb / 1024 / NW;
+    static_assert(rb <= 1024 && chunks >= 1 && chunks * NW * 1024 == ROWS * rb, "");
+    const char* lane_base;                     // row lane / lanes of the matrix
+    long long stride;                          // bytes between rows
+    int lrow, p;
+    __device__ __forceinline__ void init(const void* base, long long row_elems, int lane) {
+        stride = row_elems * (long long)sizeof(T);
+        lrow = lane / lanes;
+        p = lane % lanes;
+        lane_base = (const char*)base + lrow * stride;
+    }
+    // rows r0 .. r0 + ROWS of the matrix; km: this tile's key mask in LDS, or NULL
+    __device__ __forceinline__ void issue(T* lds, int r0, int limit, int dh, const unsigned char* km, int wave) const {
+        const bool whole = r0 + ROWS <= limit && dh == DH && !km;
+#pragma unroll
+        for (int i = 0; i < chunks; ++i) {
+            const int cr = (i * NW + wave) * per, row = cr + lrow, s = p ^ swz<T, DH>(row);
+            const char* src = lane_base + (long long)(r0 + cr) * stride + s * 16;
+            if (!whole) {
+                const bool ok = r0 + row < limit && s * epl < dh && (!km || km[row]);
+                src = ok ? src : (const char*)attn_zero16;
+            }
+            __builtin_amdgcn_global_load_lds((global_void)src, (lds_void)(reinterpret_cast<char*>(lds) + (i * NW + wave) * 1024), 16, 0, 0);
+        }
+    }
+};
+// every copy of this wave has landed and every LDS read of it has returned; then the workgroup meets
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+}
+// Where a lane finds its part of a fragment.  swz() is linear over exclusive-or and tile rows begin at multiples of 16, so an address is
+// (lane part ^ constant) + constant: `row` for fragments of rows, `col` for columns read as rows (contracted in the order of score_frag).
+// refresh() hides the lane parts from the optimizer: one exclusive-or per read instead of dozens of addresses kept in registers.
+template <typename T, int DH, int G> struct TileFrag {
+    static constexpr int ng = Blk<G>::ng, rb = DH * (int)sizeof(T);
+    int row, col;
+    __device__ __forceinline__ explicit TileFrag(int lane) {
+        const int g = lane / G, n = lane % G;
+        row = n * rb + ((g ^ swz<T, DH>(n)) << 4);
+        if constexpr (sizeof(T) == 4) col = 4 * g * rb + (((n >> 2) ^ swz<T, DH>(4 * g)) << 4) + ((n & 3) << 2);
+        else {
+            const int r = 4 * g + ((lane & 15) >> 2), slot = (G == 32 ? (lane & 16) >> 3 : 0) | ((lane & 3) >> 1);
+            col = r * rb + ((slot ^ swz<T, DH>(r)) << 4) + ((lane & 1) << 3);
+        }
+    }
+    __device__ __forceinline__ void refresh() { asm volatile("" : "+v"(row), "+v"(col)); }
+    // rows r0 + n (r0 a multiple of 16), contracted chunk c
+    __device__ __forceinline__ u32x4 rows(const T* X, int r0, int c) const {
+        return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(X) + ((row ^ (c * ng * 16)) + r0 * rb));
+    }
+    // columns m0 + n (m0 a multiple of G), contracted over tile rows r0 + the rows of chunk c
+    __device__ __forceinline__ u32x4 cols(const T* X, int m0, int r0, int c) const {
+        const char* x = reinterpret_cast<const char*>(X);
+        u32x4 f;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = c * 4 * ng + e;              // swz of the constant part of the row
+                f[e] = *reinterpret_cast<const uint32_t*>(x + ((col ^ (((m0 >> 2) ^ swz<T, DH>(r)) << 4)) + (r0 + r) * rb));
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = (2 * c + h) * 4 * ng;
+                typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(x + ((col ^ (((m0 >> 3) ^ swz<T, DH>(r)) << 4)) + (r0 + r) * rb)));
+                const u32x2 w = __builtin_bit_cast(u32x2, v);
+                f[2 * h] = w[0];
+                f[2 * h + 1] = w[1];
+            }
+        }
+        return f;
+    }
+};
+
+template <typename F, int... I> __device__ __forceinline__ void for_each_constant(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+// for n in 0 .. N - 1: use(n, load(n)).  f32: one fragment ahead and no further -- a fragment feeds 4 matrix instructions of 32 / 64 cycles,
+// which cover its LDS latency; left alone, the scheduler fetches dozens of fragments early and spills.  16-bit: the scheduler's order.
+template <typename T, int N, typename Load, typename Use> __device__ __forceinline__ void fragment_loop(Load load, Use use) {
+    if constexpr (sizeof(T) == 4) {
+        auto cur = load(std::integral_constant<int, 0>{});
+        auto step = [&](auto n) __attribute__((always_inline)) {
+            constexpr int k = decltype(n)::value;
+            auto next = load(std::integral_constant<int, (k + 1 < N ? k + 1 : k)>{});
+            use(n, cur);
+            __builtin_amdgcn_sched_barrier(0);
+            cur = next;
+        };
+        for_each_constant(step, std::make_integer_sequence<int, N>{});
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n) use(n, load(n));
+    }
+}
+
+// The key mask of the tiles ahead: a byte per key, a ring of four tiles in LDS.  Read from memory three tiles ahead, written a tile later,
+// needed two tiles later by the copies and three later by the scores: nobody waits for it.
+template <int KT> struct MaskRing {
+    const unsigned char* mask;
+    unsigned char* ring;
+    int len, tid, next;
+    __device__ __forceinline__ int at(int t) const { const int j = t * KT + tid; return tid < KT && j < len ? mask[j] : 0; }
+    // tiles t .. t + 2; the workgroup meets before the first copy
+    __device__ __forceinline__ void init(const unsigned char* m, unsigned char* r, int len_, int t, int tid_) {
+        mask = m; ring = r; len = len_; tid = tid_; next = 0;
+        if (!mask) return;
+        for (int k = 0; k < 3; ++k)
+            if (tid < KT) ring[((t + k) & 3) * KT + tid] = (unsigned char)at(t + k);
+        next = at(t + 3);
+        __syncthreads();
+    }
+    // at tile t, behind the barrier: tile t + 3 into the ring, tile t + 4 under way
+    __device__ __forceinline__ void step(int t) {
+        if (!mask) return;
+        if (tid < KT) ring[((t + 3) & 3) * KT + tid] = (unsigned char)next;
+        next = at(t + 4);
+    }
+    __device__ __forceinline__ const unsigned char* tile(int t) const { return mask ? ring + (t & 3) * KT : nullptr; }
+};
+
+constexpr int BIAS_PAD = 128;          // far values beyond the reach on both sides: a block that touches the reach needs no clamp
 __device__ __forceinline__ long long clamp_index(long long v, long long lo, long long hi) { return v < lo ? lo : v > hi ? hi : v; }
 __device__ __forceinline__ int key_len(const ekaid_attn_t& d, int b) {
     if (!d.k_len) return d.Lk;
@@ -205,10 +345,13 @@ __device__ __forceinline__ float table_at(const ekaid_attn_t& d, int bucket, int
     if (d.table_dtype == EKAID_BF16) return (float)reinterpret_cast<const __bf16*>(d.table)[i];
     return (float)reinterpret_cast<const _Float16*>(d.table)[i];
 }
-// bias of `heads` heads by clamped distance, in units of the power-of-two softmax: bias[h][rel + reach], rel in [-reach, reach]
-__device__ __forceinline__ void fill_bias(const ekaid_attn_t& d, float* bias, int head0, int heads, int tid, int nt) {
-    const int w = 2 * d.reach + 1;
-    for (int i = tid; i < heads * w; i += nt) bias[i] = table_at(d, rel_bucket(d, i % w - d.reach), head0 + i / w) * LOG2E;
+// bias of `heads` heads by distance, in units of the power-of-two softmax: bias[h][rel + reach + pad], rel in [-reach - pad, reach + pad]
+__device__ __forceinline__ void fill_bias(const ekaid_attn_t& d, float* bias, int head0, int heads, int pad, int tid, int nt) {
+    const int w = 2 * (d.reach + pad) + 1;
+    for (int i = tid; i < heads * w; i += nt) {
+        const int rel = i % w - d.reach - pad;
+        bias[i] = table_at(d, rel_bucket(d, min(max(rel, -d.reach), d.reach)), head0 + i / w) * LOG2E;
+    }
 }
 
 // which workgroup works on what: consecutive work items (tiles of one head, which share their keys) on ONE die -- workgroups are dealt
@@ -245,6 +388,40 @@ __device__ __forceinline__ void wave_fence() {
 __device__ __forceinline__ float drop_keep(const AttnArgs& a, uint64_t seed, int b, int h, int i, int j) {
     const uint64_t idx = (((uint64_t)b * a.d.H + h) * a.d.Lq + i) * (uint64_t)a.d.Lk + j;
     return dropout_scale(seed, idx, a.d.drop_p, a.inv_keep);
+}
+
+// How the raw products of a unit become exponents: exponent = score * mult + add.  Where nothing is masked and the bias is one value (none,
+// or all distances beyond the reach) mult / add are that and the scores stay as they are; otherwise they are finished in place (mult 1).
+struct Affine { float mult, add; };
+
+// one unit of NB blocks in the S^T orientation (lane: query row at `pos`; registers: keys j0 + 4 ng quad + 4 g + e).  `pmin`, `pmax`:
+// positions of this wave's rows; `bias`: padded table of the head (NULL: none); `km`: key mask of the unit (NULL: none)
+template <int G, int NB>
+__device__ __forceinline__ Affine scores_by_row(const AttnArgs& a, typename Blk<G>::acc (&s)[NB], int j0, int len, int pos, int pmin, int pmax, const float* bias,
+                                                const unsigned char* km, int lane) {
+    constexpr int ng = Blk<G>::ng, nq = Blk<G>::nq;
+    const int g = lane / G, reach = a.d.reach, jn = j0 + NB * G;
+    const bool masked = km || jn > len || (a.d.causal && jn - 1 > pmin);
+    Affine f = {a.sc2, 0.f};
+    bool near = false;
+    if (bias) {
+        if (jn - 1 - pmin <= -reach) f.add = bias[BIAS_PAD];
+        else if (j0 - pmax >= reach) f.add = bias[2 * reach + BIAS_PAD];
+        else near = true;
+    }
+    if (!masked && !near && a.sc2 >= 0.f) return f;
+    const float* b = near ? bias + (j0 + 4 * g - pos + reach + BIAS_PAD) : nullptr;
+#pragma unroll
+    for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 4 * ng * q + e, j = j0 + 4 * g + k;
+            float x = s[q / nq][4 * (q % nq) + e] * f.mult + f.add;
+            if (near) x += b[k];
+            if (masked && !(j < len && (!km || km[4 * g + k]) && (!a.d.causal || j <= pos))) x = NEG_INF;
+            s[q / nq][4 * (q % nq) + e] = x;
+        }
+    return Affine{1.f, 0.f};
 }
 
 // scores of one key tile, s[sub] = K Q^T (raw products) -> masked, biased, in powers of two.  Lane: one query row (position pos, head
@@ -284,6 +461,10 @@ struct RowWork {                       // one workgroup's share of the forward /
 };
 
 int attn_check(const ekaid_attn_t* a, const char* who);
+int attn_lds_limit(const void* fn, int bytes);      // once per kernel and device: the dynamic LDS it may be launched with
+int waves_for_rows(int R);
+// keys (or rows) a tile of the copying kernels: 16 KB an operand, twice two of them leave room for two workgroups a compute unit
+constexpr int attn_kt(int esize, int dh, int g) { return esize == 4 && dh > 128 ? 16 : g == 16 || dh > 128 || (esize == 4 && dh > 64) ? 32 : 64; }
 size_t attn_bwd_workspace(const ekaid_attn_t* a);
 
 }  // namespace ekaid
