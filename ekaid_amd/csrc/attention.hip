@@ -1,32 +1,8 @@
 // Forward of the attention operators (include/ekaid_hip.h: ekaid_attn_t): one pass over the keys with the running maximum and sum.
 #include "attn.h"
+#include <algorithm>
 
 namespace ekaid {
-
-// running maximum / sum: returns the factor that earlier sums and outputs take
-template <int G, int NB>
-__device__ __forceinline__ float online_softmax(typename Blk<G>::acc (&s)[NB], float& m, float& l) {
-    constexpr int nv = 4 * Blk<G>::nq;
-    float mx = m;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < nv; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = across_groups_max<G>(mx);
-    const float base = mx == NEG_INF ? 0.f : mx;          // nothing valid yet: every power below is 2^-inf = 0
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    float t = 0.f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < nv; ++r) {
-            s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - base);
-            t += s[b][r];
-        }
-    l = l * alpha + t;                                    // this lane's keys only; the lane groups meet at the end
-    m = mx;
-    return alpha;
-}
 
 template <int G, int NB>
 __device__ __forceinline__ void drop_scores(const AttnArgs& a, typename Blk<G>::acc (&s)[NB], int b, int h, int i, int j0, int lane) {
@@ -72,84 +48,191 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const RowWork& w, 
     if (g == 0 && a.d.lse) a.d.lse[row] = l == 0.f ? POS_INF : m + __builtin_amdgcn_logf(l);
 }
 
-// ---- few query rows (a new token; the heads that share keys packed into the rows): key tiles through registers into LDS
-template <typename T, int DH, int G, int NW, int KT>
-__global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs a) {
-    constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
-    constexpr int LDK = Ld<T, DH>::row, LDV = Ld<T, DH>::col;
+// ---- few query rows (a new token; the heads that share keys packed into the rows): 16 rows a workgroup, its NW waves take blocks of keys in
+// turn and are joined at the end.  Nothing is shared before that: keys go from memory to registers as fragments; f32 values likewise (a
+// lane's four columns of a row are its element of four output blocks: columns 64 x + 4 n + t are row n of block 4 x + t), 16-bit values
+// through a buffer of the wave for the transposing read.  One block ahead is under way while a block is worked on.
+template <typename T, int DH> struct FewBlock {
+    static constexpr int KB = sizeof(T) == 4 ? 16 : 32, NB = KB / 16, NC = DH / (Elem<T>::epl * 4), NV = sizeof(T) == 4 ? 4 * (DH / 64) : 0;
+    u32x4 k[NB][NC], v[NV + 1];
+    uint32_t ok[NB];                       // bit i: key i of the block may be attended
+    TileCopy<T, DH, KB, 1> copy;           // (16-bit values)
+    __device__ __forceinline__ void load(const ekaid_attn_t& d, const T* kb, const T* vb, const unsigned char* mask, int j0, int end, T* vs, int lane) {
+        const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int j = j0 + 16 * b + n;
+            const bool valid = j < end && (!mask || mask[j]);
+            ok[b] = (uint32_t)__ballot(valid) & 0xffffu;
+            const T* row = kb + (long long)j * d.k_row;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) k[b][c] = row_frag_global<T, 16>(row, c, d.dh, valid, lane);
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool valid = (ok[0] >> (4 * g + e)) & 1;
+                const T* row = vb + (long long)(j0 + 4 * g + e) * d.v_row;
+#pragma unroll
+                for (int x = 0; x < DH / 64; ++x) {
+                    u32x4 z = {0u, 0u, 0u, 0u};
+                    if (valid && 64 * x + 4 * n < d.dh) z = *reinterpret_cast<const u32x4*>(row + 64 * x + 4 * n);
+                    v[e * (DH / 64) + x] = z;
+                }
+            }
+        } else {
+            uint32_t bits = ok[0];
+            if constexpr (NB > 1) bits |= ok[1] << 16;
+#pragma unroll
+            for (int i = 0; i < TileCopy<T, DH, KB, 1>::chunks; ++i) {
+                const int cr = i * TileCopy<T, DH, KB, 1>::per, row = cr + copy.lrow, s = copy.p ^ swz<T, DH>(row);
+                const char* src = copy.lane_base + (long long)(j0 + cr) * copy.stride + s * 16;
+                src = ((bits >> row) & 1) && s * Elem<T>::epl < d.dh ? src : (const char*)attn_zero16;
+                __builtin_amdgcn_global_load_lds((global_void)src, (lds_void)(reinterpret_cast<char*>(vs) + i * 1024), 16, 0, 0);
+            }
+        }
+    }
+};
+
+template <typename T, int DH, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_few_kernel(const AttnArgs a) {
+    typedef FewBlock<T, DH> Block;
+    constexpr int NT = 64 * NW, NB = Block::NB, NC = Block::NC, KB = Block::KB, MT = DH / 16, nv16 = sizeof(T) == 4 ? 4 : KB * DH;
+    __shared__ __attribute__((aligned(16))) T va[NW][nv16], vb_[NW][nv16];
+    __shared__ float sml[NW][2][16];
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + KT * LDK;
-    unsigned char* kms = reinterpret_cast<unsigned char*>(Vs + KT * LDV);
-    float* bias = reinterpret_cast<float*>(kms + KT);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // [NW][rows][DH] outputs of the waves, 4-column groups permuted by row; 16-bit: over the value buffers, whose work is done by then
+    float* join = sizeof(T) == 4 ? reinterpret_cast<float*>(smem) : reinterpret_cast<float*>(va);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
     const RowWork w(a);
     const ekaid_attn_t& d = a.d;
-    const int R = d.Lq * a.gp, r = (w.tile * NW + wave) * G + lane % G;
-    const bool ok = r < R;
-    const int i = ok ? r / a.gp : 0, hg = ok ? r % a.gp : 0, h = w.head0 + hg;
-    const int p0 = query_pos(d, w.b), pos = p0 + i;
-    const int len = key_len(d, w.b);
-    int kend = len;
-    if (d.causal) {
-        const int last = min(R, (w.tile + 1) * NW * G) - 1;
-        kend = max(0, min(len, p0 + last / a.gp + 1));
-    }
-    const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
+    const int R = d.Lq * a.gp, row0 = w.tile * 16, rows = min(16, R - row0), r = min(row0 + n, R - 1);
+    const bool ok = n < rows;
+    float* bias = reinterpret_cast<float*>(smem) + (sizeof(T) == 4 ? NW * rows * DH : 0);
+    const int i = r / a.gp, hg = r % a.gp, h = w.head0 + hg;
+    const int p0 = query_pos(d, w.b), pos = p0 + i, len = key_len(d, w.b);
+    const int kend = d.causal ? max(0, min(len, p0 + (row0 + rows - 1) / a.gp + 1)) : len;
+    const int nb = (kend + KB - 1) / KB, per = (nb + a.splits - 1) / a.splits, b0 = w.split * per, b1 = min(nb, b0 + per);
     const unsigned char* mask = d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr;
-    if (d.table) fill_bias(d, bias, w.head0, a.gp, 0, tid, NT);
-
+    if (d.table) {
+        fill_bias(d, bias, w.head0, a.gp, 0, tid, NT);
+        __syncthreads();
+    }
+    const float* brow = d.table ? bias + hg * (2 * d.reach + 1) + d.reach : nullptr;
+    const T* kb = reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh;
+    const T* vb = reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh;
     u32x4 qf[NC];
     const T* qrow = reinterpret_cast<const T*>(d.q) + w.b * d.q_batch + i * d.q_row + (long long)h * d.dh;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) qf[c] = row_frag_global<T, G>(qrow, c, d.dh, ok, lane);
-
-    const T* kb = reinterpret_cast<const T*>(d.k) + w.b * d.k_batch + (long long)w.kvh * d.dh;
-    const T* vb = reinterpret_cast<const T*>(d.v) + w.b * d.v_batch + (long long)w.kvh * d.dh;
-    Stage<T, DH, KT, NT> sk, sv;
-    typename Blk<G>::acc o[MT];
+    for (int c = 0; c < NC; ++c) qf[c] = row_frag_global<T, 16>(qrow, c, d.dh, ok, lane);
+    const TileFrag<T, DH, 16> tf(lane);
+    f32x4 o[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
+    for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<16>();
     float m = NEG_INF, l = 0.f;
-    if (t0 < t1) {
-        sk.load(kb, d.k_row, t0 * KT, len, d.dh, mask, tid);
-        sv.load(vb, d.v_row, t0 * KT, len, d.dh, mask, tid);
-    }
-    for (int t = t0; t < t1; ++t) {
-        sk.store(Ks, LDK, tid);
-        sv.store(Vs, LDV, tid);
-        if (mask) for (int j = tid; j < KT; j += NT) kms[j] = t * KT + j < len ? mask[t * KT + j] : 0;
-        __syncthreads();
-        if (t + 1 < t1) {
-            sk.load(kb, d.k_row, (t + 1) * KT, len, d.dh, mask, tid);
-            sv.load(vb, d.v_row, (t + 1) * KT, len, d.dh, mask, tid);
-        }
-        typename Blk<G>::acc s[NB];
+    Block x, y;
+    x.copy.init(vb, d.v_row, lane);
+    y.copy.init(vb, d.v_row, lane);
+    const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
+    const int first = b0 + wave;
+    if (first < b1) x.load(d, kb, vb, mask, first * KB, kend, va[wave], lane);
+    auto block = [&](int t, Block& cur, const T* vs, Block& next, T* vn) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0x0070);                   // this block has arrived, the buffer of the one before is read
+        if (t + NW < b1) next.load(d, kb, vb, mask, (t + NW) * KB, kend, vn, lane);
+        f32x4 s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            s[b] = zero_acc<G>();
+            s[b] = zero_acc<16>();
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s[b] = mma<T, G>(row_frag<T, G>(Ks, LDK, b * G, c, lane), qf[c], s[b]);
+            for (int c = 0; c < NC; ++c) s[b] = mma<T, 16>(cur.k[b][c], qf[c], s[b]);
         }
-        const bool partial = mask || (t + 1) * KT > len || (d.causal && (t + 1) * KT > p0 + (w.tile * NW * G) / a.gp + 1);
-        finish_scores<G, NB>(a, s, t * KT, len, pos, d.table ? bias + hg * (2 * d.reach + 1) : nullptr, mask ? kms : nullptr, partial, lane);
-        const float alpha = online_softmax<G, NB>(s, m, l);
-        if (d.drop_p > 0.f) drop_scores<G, NB>(a, s, w.b, h, i, t * KT, lane);
+        float mx = m;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = t * KB + 16 * b + 4 * g + e;
+                float z = s[b][e] * a.sc2;
+                if (brow) z += brow[min(max(j - pos, -d.reach), d.reach)];
+                if (!((cur.ok[b] >> (4 * g + e)) & 1) || (d.causal && j > pos)) z = NEG_INF;
+                s[b][e] = z;
+                mx = fmaxf(mx, z);
+            }
+        mx = across_groups_max<16>(mx);
+        const float base = mx == NEG_INF ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - base);
+        m = mx;
+        l *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[b][e] = __builtin_amdgcn_exp2f(s[b][e] - base);
+                l += s[b][e];
+                if (d.drop_p > 0.f) s[b][e] *= drop_keep(a, seed, w.b, h, i, t * KB + 16 * b + 4 * g + e);
+            }
         if (__any(alpha != 1.f)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int e = 0; e < 4 * Blk<G>::nq; ++e) o[mt][e] *= alpha;
+                for (int e = 0; e < 4; ++e) o[mt][e] *= alpha;
         }
+        const u32x4 pf = score_frag<T, 16, NB>(s, 0);
 #pragma unroll
-        for (int c = 0; c < PC; ++c) {
-            const u32x4 pf = score_frag<T, G, NB>(s, c);
+        for (int mt = 0; mt < MT; ++mt) {
+            u32x4 f;
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o[mt] = mma<T, G>(col_frag<T, G>(Vs, LDV, mt * G, c, lane), pf, o[mt]);
+                for (int e = 0; e < 4; ++e) f[e] = cur.v[e * (DH / 64) + mt / 4][mt % 4];
+            } else f = tf.cols(vs, mt * 16, 0, 0);
+            o[mt] = mma<T, 16>(f, pf, o[mt]);
         }
-        __syncthreads();
+    };
+    for (int t = first; t < b1; t += 2 * NW) {
+        block(t, x, va[wave], y, vb_[wave]);
+        if (t + NW < b1) block(t + NW, y, vb_[wave], x, va[wave]);
     }
-    write_rows<T, DH, G>(a, w, o, m, l, i, h, ok, lane);
+    // the waves' shares meet: maxima and sums first, then the outputs, each scaled by its wave
+    l = across_groups_sum<16>(l);
+    if (g == 0) {
+        sml[wave][0][n] = m;
+        sml[wave][1][n] = l;
+    }
+    __syncthreads();
+    float M = NEG_INF, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) M = fmaxf(M, sml[k][0][n]);
+    const float base = M == NEG_INF ? 0.f : M;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) sum += sml[k][1][n] * __builtin_amdgcn_exp2f(sml[k][0][n] - base);
+    const float f = __builtin_amdgcn_exp2f(m - base) * (a.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum);
+    const long long row = ((long long)w.b * d.H + h) * d.Lq + i, total = (long long)d.B * d.H * d.Lq;
+    if (ok) {
+        float* p = join + (wave * rows + n) * DH;
+        const int turn = n << 2;
+#pragma unroll
+        for (int q = 0; q < MT; ++q) {
+            if constexpr (sizeof(T) == 4) {                   // q = 4 x + e: columns 64 x + 16 g + 4 e + (block 4 x + t: t)
+                const int x4 = q / 4 * 4, e = q % 4;
+                store4<float>(p + ((16 * x4 + 16 * g + 4 * e) ^ turn), o[x4][e] * f, o[x4 + 1][e] * f, o[x4 + 2][e] * f, o[x4 + 3][e] * f);
+            } else store4<float>(p + ((16 * q + 4 * g) ^ turn), o[q][0] * f, o[q][1] * f, o[q][2] * f, o[q][3] * f);
+        }
+        if (wave == 0 && g == 0) {
+            if (a.splits > 1) {
+                a.pml[2 * (w.split * total + row)] = M;
+                a.pml[2 * (w.split * total + row) + 1] = sum;
+            } else if (d.lse) d.lse[row] = sum == 0.f ? POS_INF : M + __builtin_amdgcn_logf(sum);
+        }
+    }
+    __syncthreads();
+    const int vec = d.dh / 4;
+    for (int k = tid; k < rows * vec; k += NT) {
+        const int rr = k / vec, c = (k % vec) * 4, ri = (row0 + rr) / a.gp, rh = w.head0 + (row0 + rr) % a.gp;
+        f32x4 v = *reinterpret_cast<const f32x4*>(join + rr * DH + (c ^ (rr << 2)));
+#pragma unroll
+        for (int q = 1; q < NW; ++q) v += *reinterpret_cast<const f32x4*>(join + (q * rows + rr) * DH + (c ^ (rr << 2)));
+        if (a.splits > 1) *reinterpret_cast<f32x4*>(a.po + (w.split * total + ((long long)w.b * d.H + rh) * d.Lq + ri) * d.dh + c) = v;
+        else store4<T>(reinterpret_cast<T*>(d.out) + ((long long)w.b * d.Lq + ri) * d.H * d.dh + (long long)rh * d.dh + c, v[0], v[1], v[2], v[3]);
+    }
 }
 
 // ---- many query rows: NW * G rows a workgroup, key tiles copied to LDS one tile ahead of the products
@@ -313,7 +396,7 @@ int attn_check(const ekaid_attn_t* a, const char* who) {
     return EKAID_OK;
 }
 
-struct FwdPlan { int few, g, nw, gp, tiles, splits, kt; size_t ws; };
+struct FwdPlan { int few, g, nw, gp, tiles, splits; size_t ws; };
 
 // Waves of 16 rows: as few rows as possible beyond R (a wave on rows that do not exist costs as much as one on rows that do)
 int waves_for_rows(int R) {
@@ -327,39 +410,39 @@ int waves_for_rows(int R) {
 
 static FwdPlan fwd_plan(const ekaid_attn_t* a) {
     FwdPlan p;
-    const int group = a->H / a->KV;
-    const bool wide32 = a->dtype == EKAID_F32 && a->dh > 128;
-    p.few = a->Lq < 17;
-    p.gp = p.few && group > 1 && (!a->table || group * (2 * a->reach + 1) <= 8192) ? group : 1;
-    const int R = a->Lq * p.gp;
+    const int group = a->H / a->KV, esz = a->dtype == EKAID_F32 ? 4 : 2;
+    // up to 16 query rows a head: the kernel whose waves split the keys; the heads that share keys go into its rows while those fit twice
+    p.few = a->Lq <= 16;
+    p.gp = p.few && a->Lq * group <= 32 && (!a->table || group * (2 * a->reach + 1) <= 7900) ? group : 1;
+    int per_tile, keys;
     if (p.few) {
-        p.g = R <= 64 || wide32 ? 16 : 32;
-        p.nw = R <= 16 ? 1 : R <= 32 && p.g == 16 ? 2 : 4;
-        if (wide32 && p.nw == 1) p.nw = 2;      // one wave would have to hold a whole staged tile: it spills
-        p.kt = a->dh > 128 || (a->dtype == EKAID_F32 && a->dh > 64) ? 32 : 64;
+        p.g = 16;
+        p.nw = 4;
+        per_tile = 16;
+        keys = 4 * (esz == 4 ? 16 : 32);
     } else {
-        p.g = R <= 64 || wide32 ? 16 : 32;
-        p.nw = p.g == 32 ? 4 : waves_for_rows(R);
-        p.kt = attn_kt(a->dtype == EKAID_F32 ? 4 : 2, a->dh, p.g);
+        p.g = a->Lq <= 64 || (esz == 4 && a->dh > 128) ? 16 : 32;
+        p.nw = p.g == 32 ? 4 : waves_for_rows(a->Lq);
+        per_tile = p.g * p.nw;
+        keys = attn_kt(esz, a->dh, p.g);
     }
-    p.tiles = cdiv(R, p.g * p.nw);
+    p.tiles = cdiv(a->Lq * p.gp, per_tile);
     const long long wgs = (long long)a->B * (a->H / p.gp) * p.tiles;
-    const int key_tiles = cdiv(a->Lk, p.kt);
+    const int steps = cdiv(a->Lk, keys);
     long long s = 1;
     const long long want = 4 * 512 / p.nw;
-    if (wgs < want / 2 && key_tiles > 1) s = (want + wgs - 1) / (wgs > 0 ? wgs : 1);
-    if (s > (key_tiles + 1) / 2) s = (key_tiles + 1) / 2;
-    if (s < 1) s = 1;
-    p.splits = (int)s;
+    if (wgs < want / 2 && steps > 1) s = (want + wgs - 1) / (wgs > 0 ? wgs : 1);
+    if (s > (steps + 1) / 2) s = (steps + 1) / 2;
+    p.splits = (int)(s < 1 ? 1 : s);
     p.ws = p.splits > 1 ? (size_t)p.splits * a->B * a->H * a->Lq * (a->dh + 2) * sizeof(float) : 0;
     return p;
 }
 
-template <typename T, int DH, int G, int NW, int KT> static int launch_few(const AttnArgs& a, int grid, hipStream_t st) {
-    constexpr size_t base = (size_t)KT * (Ld<T, DH>::row + Ld<T, DH>::col) * sizeof(T) + KT;
-    const size_t lds = base + (a.d.table ? (size_t)a.gp * (2 * a.d.reach + 1) * 4 : 0);
-    if (int rc = attn_lds_limit((const void*)attn_fwd_kernel<T, DH, G, NW, KT>, 160 * 1024)) return rc;
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DH, G, NW, KT>), dim3(grid), dim3(64 * NW), lds, st, a);
+template <typename T, int DH> static int launch_few(const AttnArgs& a, int grid, hipStream_t st) {
+    const int rows = std::min(16, a.d.Lq * a.gp);
+    const size_t lds = (sizeof(T) == 4 ? (size_t)4 * rows * DH * 4 : 0) + (a.d.table ? (size_t)a.gp * (2 * a.d.reach + 1) * 4 : 0);
+    if (int rc = attn_lds_limit((const void*)attn_few_kernel<T, DH, 4>, sizeof(T) == 4 ? 100 * 1024 : 32 * 1024 - 1024)) return rc;
+    hipLaunchKernelGGL((attn_few_kernel<T, DH, 4>), dim3(grid), dim3(256), lds, st, a);
     return check_launch("attn_fwd");
 }
 template <typename T, int DH, int G, int NW> static int launch_tile(const AttnArgs& a, int grid, hipStream_t st) {
@@ -370,15 +453,7 @@ template <typename T, int DH, int G, int NW> static int launch_tile(const AttnAr
     return check_launch("attn_fwd");
 }
 template <typename T, int DH> static int pick_fwd(const AttnArgs& a, const FwdPlan& p, int grid, hipStream_t st) {
-    if (p.few) {
-        constexpr int KT = DH > 128 || (sizeof(T) == 4 && DH > 64) ? 32 : 64;
-        if constexpr (!(sizeof(T) == 4 && DH > 128)) {
-            if (p.g == 32) return launch_few<T, DH, 32, 4, KT>(a, grid, st);
-            if (p.nw == 1) return launch_few<T, DH, 16, 1, KT>(a, grid, st);
-        }
-        if (p.nw == 2) return launch_few<T, DH, 16, 2, KT>(a, grid, st);
-        return launch_few<T, DH, 16, 4, KT>(a, grid, st);
-    }
+    if (p.few) return launch_few<T, DH>(a, grid, st);
     if constexpr (!(sizeof(T) == 4 && DH > 128))
         if (p.g == 32) return launch_tile<T, DH, 32, 4>(a, grid, st);
     if (p.nw == 1) return launch_tile<T, DH, 16, 1>(a, grid, st);

@@ -112,37 +112,7 @@ template <typename T, int G, int NB> __device__ __forceinline__ u32x4 score_frag
     return f;
 }
 
-// A operand whose rows are the COLUMNS of a row-major LDS tile X[row][ld]: columns m0 .. m0+G, contracted over the tile rows in the
-// order of score_frag(c).  16-bit: ds_read_b64_tr_b16 -- the 16 lanes of a group read 4 rows x 16 columns and each receives one column.
-template <typename T, int G> __device__ __forceinline__ u32x4 col_frag(const T* X, int ld, int m0, int c, int lane) {
-    constexpr int ng = Blk<G>::ng;
-    const int g = lane / G;
-    u32x4 f;
-    if constexpr (sizeof(T) == 4) {
-        const float* p = reinterpret_cast<const float*>(X) + (c * 4 * ng + 4 * g) * ld + m0 + (lane % G);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __builtin_bit_cast(uint32_t, p[e * ld]);
-    } else {
-        const int col = m0 + (G == 32 ? (lane & 16) : 0) + 4 * (lane & 3);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = (2 * c + h) * 4 * ng + 4 * g + ((lane & 15) >> 2);
-            typedef __attribute__((address_space(3))) s16x4* lds_t;
-            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(X + row * ld + col));
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            const u32x2 w = __builtin_bit_cast(u32x2, v);
-            f[2 * h] = w[0];
-            f[2 * h + 1] = w[1];
-        }
-    }
-    return f;
-}
-// A or B operand from a row-major LDS tile: row r0 + lane % G, contracted columns of chunk c
-template <typename T, int G> __device__ __forceinline__ u32x4 row_frag(const T* X, int ld, int r0, int c, int lane) {
-    constexpr int epl = Elem<T>::epl;
-    return *reinterpret_cast<const u32x4*>(X + (r0 + lane % G) * ld + (c * Blk<G>::ng + lane / G) * epl);
-}
-// the same straight from memory (zero beyond column dh, or when the row does not exist)
+// A or B operand straight from memory: this lane's row, contracted chunk c (zero beyond column dh, or when the row does not exist)
 template <typename T, int G> __device__ __forceinline__ u32x4 row_frag_global(const T* row, int c, int dh, bool ok, int lane) {
     constexpr int epl = Elem<T>::epl;
     const int col = (c * Blk<G>::ng + lane / G) * epl;
@@ -150,37 +120,6 @@ template <typename T, int G> __device__ __forceinline__ u32x4 row_frag_global(co
     if (ok && col < dh) z = *reinterpret_cast<const u32x4*>(row + col);
     return z;
 }
-
-// LDS leading dimensions (elements): rows read 16 bytes per lane want an odd number of 16-byte slots; columns read by transposition want
-// consecutive rows 64 bytes apart modulo the 256-byte bank round (16-bit) or an offset of 8 floats (f32, two lane groups)
-template <typename T, int DH> struct Ld {
-    static constexpr int row = DH + 16 / (int)sizeof(T);
-    static constexpr int col = sizeof(T) == 4 ? DH + 8 : DH + 32;
-};
-
-// rows [r0, r0 + ROWS) of a row-major matrix into registers (zero where the row index reaches `limit`, the key mask is 0 or the column
-// is beyond dh), then from registers into an LDS tile.  Masked rows never enter a product: NaN or Inf in them stays there.
-template <typename T, int DH, int ROWS, int NT> struct Stage {
-    static constexpr int epl = Elem<T>::epl, vpr = DH / epl, n = ROWS * vpr, per = (n + NT - 1) / NT;
-    u32x4 r[per];
-    __device__ __forceinline__ void load(const T* base, long long stride, int r0, int limit, int dh, const unsigned char* mask, int tid) {
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            const int id = i * NT + tid, row = id / vpr, col = (id % vpr) * epl;
-            u32x4 z = {0u, 0u, 0u, 0u};
-            const int gr = r0 + row;
-            if (id < n && gr < limit && col < dh && (!mask || mask[gr])) z = *reinterpret_cast<const u32x4*>(base + (long long)gr * stride + col);
-            r[i] = z;
-        }
-    }
-    __device__ __forceinline__ void store(T* lds, int ld, int tid) const {
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            const int id = i * NT + tid;
-            if (id < n) *reinterpret_cast<u32x4*>(lds + (id / vpr) * ld + (id % vpr) * epl) = r[i];
-        }
-    }
-};
 
 // ---- tiles copied to LDS without passing registers
 // A tile is ROWS rows x DH elements, rows packed (no padding: a wave writes 1 KB in lane order), the 16-byte slots of a row permuted by an
@@ -422,27 +361,6 @@ __device__ __forceinline__ Affine scores_by_row(const AttnArgs& a, typename Blk<
             s[q / nq][4 * (q % nq) + e] = x;
         }
     return Affine{1.f, 0.f};
-}
-
-// scores of one key tile, s[sub] = K Q^T (raw products) -> masked, biased, in powers of two.  Lane: one query row (position pos, head
-// row `bias`), registers: keys j0 + 4 ng quad + 4 g + e.
-template <int G, int NB>
-__device__ __forceinline__ void finish_scores(const AttnArgs& a, typename Blk<G>::acc (&s)[NB], int j0, int len, int pos, const float* bias,
-                                              const unsigned char* km, bool partial, int lane) {
-    constexpr int ng = Blk<G>::ng, nq = Blk<G>::nq;
-    const int g = lane / G, reach = a.d.reach;
-#pragma unroll
-    for (int q = 0; q < NB * nq; ++q) {
-        const int jq = 4 * ng * q + 4 * g;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x = s[q / nq][4 * (q % nq) + e] * a.sc2;
-            const int j = j0 + jq + e;
-            if (bias) x += bias[min(max(j - pos, -reach), reach) + reach];
-            if (partial && !(j < len && (!km || km[jq + e]) && (!a.d.causal || j <= pos))) x = NEG_INF;
-            s[q / nq][4 * (q % nq) + e] = x;
-        }
-    }
 }
 
 struct RowWork {                       // one workgroup's share of the forward / dq work list
