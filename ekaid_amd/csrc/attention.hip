@@ -242,7 +242,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) vo
     __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* bias = reinterpret_cast<float*>(smem);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const RowWork w(a);
     const ekaid_attn_t& d = a.d;
     const int row0 = (w.tile * NW + wave) * G, h = w.head0;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) vo
         typename Blk<G>::acc s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) s[b] = zero_acc<G>();
-        fragment_loop<T, NC * NB>([&](int n) __attribute__((always_inline)) { return tf.rows(ks, (n % NB) * G, n / NB); },
+        fragment_loop<T, G, NC * NB>([&](int n) __attribute__((always_inline)) { return tf.rows(ks, (n % NB) * G, n / NB); },
                                   [&](int n, u32x4 x) __attribute__((always_inline)) { s[n % NB] = mma<T, G>(x, qf[n / NB], s[n % NB]); });
         const Affine f = scores_by_row<G, NB>(a, s, t * KT, len, pos, pmin, pmax, d.table ? bias : nullptr, ring.tile(t), lane);
         float mx = s[0][0];
@@ -294,17 +294,17 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) vo
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int r = 0; r < nv; ++r) mx = fmaxf(mx, s[b][r]);
-        const float mn = fmaxf(m, across_groups_max<G>(mx) * f.mult + f.add);      // (mult >= 0)
-        const float base = mn == NEG_INF ? 0.f : mn, shift = f.add - base;
-        if (__any(mn != m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
+        const float mn = across_groups_max<G>(mx) * f.mult + f.add;                // (mult >= 0)
+        if (__any(mn > m + 6.f)) {                        // m need not be the maximum, only near it: powers up to 2^6 lose nothing, and most
+            const float up = fmaxf(m, mn), alpha = __builtin_amdgcn_exp2f(m - (up == NEG_INF ? 0.f : up));      // tiles leave the outputs alone
+            m = up;
             l *= alpha;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int e = 0; e < nv; ++e) o[mt][e] *= alpha;
         }
-        m = mn;
+        const float shift = f.add - (m == NEG_INF ? 0.f : m);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) vo
         u32x4 pf[PC];
 #pragma unroll
         for (int c = 0; c < PC; ++c) pf[c] = score_frag<T, G, NB>(s, c);
-        fragment_loop<T, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(vs, (n % MT) * G, 0, n / MT); },
+        fragment_loop<T, G, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(vs, (n % MT) * G, 0, n / MT); },
                                   [&](int n, u32x4 x) __attribute__((always_inline)) { o[n % MT] = mma<T, G>(x, pf[n / MT], o[n % MT]); });
     };
     for (int t = t0; t < t1; t += 2) {

@@ -24,7 +24,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
     constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng, nv = 4 * nq;
     __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
     float* red = reinterpret_cast<float*>(smem);              // [NW] row-norm maxima
     float* bias = red + NW;                                   // padded table of the head
     float* dsum = bias + (REL ? width + 2 * BIAS_PAD : 0);    // [NW][width]: this wave's sums of score gradients by distance
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
             s[b] = zero_acc<G>();
             dp[b] = zero_acc<G>();
         }
-        fragment_loop<T, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? vs : ks, r0 + (n / 2 % NB) * G, n / 2 / NB); },
+        fragment_loop<T, G, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? vs : ks, r0 + (n / 2 % NB) * G, n / 2 / NB); },
                                       [&](int n, u32x4 x) __attribute__((always_inline)) {
                                           const int b = n / 2 % NB, c = n / 2 / NB;
                                           if (n & 1) dp[b] = mma<T, G>(x, gf[c], dp[b]);
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
         u32x4 sf[PC];
 #pragma unroll
         for (int c = 0; c < PC; ++c) sf[c] = score_frag<T, G, NB>(s, c);
-        fragment_loop<T, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(ks, (n % MT) * G, r0, n / MT); },
+        fragment_loop<T, G, PC * MT>([&](int n) __attribute__((always_inline)) { return tf.cols(ks, (n % MT) * G, r0, n / MT); },
                                   [&](int n, u32x4 x) __attribute__((always_inline)) { o[n % MT] = mma<T, G>(x, sf[n / MT], o[n % MT]); });
     };
     auto tile = [&](int t, const T* ks, const T* vs, T* kn, T* vn) __attribute__((always_inline)) {
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) vo
     __shared__ __attribute__((aligned(16))) float l0s[QT], l1s[QT], d0s[QT], d1s[QT];      // log2 denominators, deltas
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* bias = reinterpret_cast<float*>(smem);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G;
     const ekaid_attn_t& d = a.d;
     const int wi = die_order(blockIdx.x, gridDim.x), tl = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
     const int b = bk / d.KV, kvh = bk % d.KV, group = d.H / d.KV;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) vo
             s[x] = zero_acc<G>();
             dp[x] = zero_acc<G>();
         }
-        fragment_loop<T, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? gs : qs, r0 + (n / 2 % NB) * G, n / 2 / NB); },
+        fragment_loop<T, G, NC * NB * 2>([&](int n) __attribute__((always_inline)) { return tf.rows(n & 1 ? gs : qs, r0 + (n / 2 % NB) * G, n / 2 / NB); },
                                       [&](int n, u32x4 x) __attribute__((always_inline)) {
                                           const int y = n / 2 % NB, c = n / 2 / NB;
                                           if (n & 1) dp[y] = mma<T, G>(x, vf[c], dp[y]);
@@ -327,13 +327,15 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) vo
                 dp[q / nq][r] -= d4[e];
             }
         }
-        if (masked) {
+        if (masked) {                                         // rows of the unit from `from` on, before the last
+            const int from = d.causal ? j - pu : 0, end = d.Lq - i0;
 #pragma unroll
             for (int q = 0; q < NB * nq; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int k = 4 * ng * q + 4 * g + e;
-                    if (i0 + k >= d.Lq || (d.causal && j > pu + k)) s[q / nq][4 * (q % nq) + e] = 0.f;
+                    const float x = s[q / nq][4 * (q % nq) + e];
+                    s[q / nq][4 * (q % nq) + e] = ((k >= from) & (k < end)) ? x : 0.f;
                 }
         }
         if (d.drop_p > 0.f) {
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) vo
             pf[c] = score_frag<T, G, NB>(s, c);
             df[c] = score_frag<T, G, NB>(dp, c);
         }
-        fragment_loop<T, PC * MT * 2>([&](int n) __attribute__((always_inline)) { return tf.cols(n & 1 ? qs : gs, (n / 2 % MT) * G, r0, n / 2 / MT); },
+        fragment_loop<T, G, PC * MT * 2>([&](int n) __attribute__((always_inline)) { return tf.cols(n & 1 ? qs : gs, (n / 2 % MT) * G, r0, n / 2 / MT); },
                                       [&](int n, u32x4 x) __attribute__((always_inline)) {
                                           const int mt = n / 2 % MT, c = n / 2 / MT;
                                           if (n & 1) dk[mt] = mma<T, G>(x, df[c], dk[mt]);
@@ -480,7 +482,7 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
 size_t attn_bwd_workspace(const ekaid_attn_t* a) { return bwd_plan(a).total; }
 
 template <typename T, int DH, int G, int NW, bool REL> static int launch_dq(const AttnArgs& a, hipStream_t st) {
-    constexpr int KT = attn_kt((int)sizeof(T), DH, G);
+    constexpr int KT = attn_kt((int)sizeof(T), DH, G) > 32 && REL ? 32 : attn_kt((int)sizeof(T), DH, G);      // (the sums by distance take LDS too)
     size_t lds = 4 * NW + 4 * KT;
     if (REL) lds += 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + 2 * BIAS_PAD + NW * G * (G + 1));
     if (int rc = attn_lds_limit((const void*)attn_dq_kernel<T, DH, G, NW, KT, REL>, 96 * 1024)) return rc;

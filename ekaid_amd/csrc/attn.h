@@ -214,23 +214,22 @@ template <typename T, int DH, int G> struct TileFrag {
 };
 
 template <typename F, int... I> __device__ __forceinline__ void for_each_constant(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
-// for n in 0 .. N - 1: use(n, load(n)).  f32: one fragment ahead and no further -- a fragment feeds 4 matrix instructions of 32 / 64 cycles,
-// which cover its LDS latency; left alone, the scheduler fetches dozens of fragments early and spills.  16-bit: the scheduler's order.
-template <typename T, int N, typename Load, typename Use> __device__ __forceinline__ void fragment_loop(Load load, Use use) {
-    if constexpr (sizeof(T) == 4) {
-        auto cur = load(std::integral_constant<int, 0>{});
-        auto step = [&](auto n) __attribute__((always_inline)) {
-            constexpr int k = decltype(n)::value;
-            auto next = load(std::integral_constant<int, (k + 1 < N ? k + 1 : k)>{});
-            use(n, cur);
-            __builtin_amdgcn_sched_barrier(0);
-            cur = next;
-        };
-        for_each_constant(step, std::make_integer_sequence<int, N>{});
-    } else {
+// for n in 0 .. N - 1: use(n, load(n)) with the fragments of the next `ahead` steps under way: enough matrix cycles (4 x 64 / 32 in f32, 32 / 16
+// in 16 bits a fragment) to cover a fragment's LDS latency.  The order is pinned: left alone, the scheduler either waits for every
+// fragment right behind its read or fetches dozens early and spills.
+template <typename T, int G, int N, typename Load, typename Use> __device__ __forceinline__ void fragment_loop(Load load, Use use) {
+    constexpr int want = sizeof(T) == 4 ? 64 / G - 1 : 128 / G, ahead = want < N ? want : N;
+    u32x4 buf[ahead];
 #pragma unroll
-        for (int n = 0; n < N; ++n) use(n, load(n));
-    }
+    for (int n = 0; n < ahead; ++n) buf[n] = load(n);
+    auto step = [&](auto c) __attribute__((always_inline)) {
+        constexpr int n = decltype(c)::value;
+        const u32x4 x = buf[n % ahead];
+        if constexpr (n + ahead < N) buf[n % ahead] = load(n + ahead);
+        use(n, x);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for_each_constant(step, std::make_integer_sequence<int, N>{});
 }
 
 // The key mask of the tiles ahead: a byte per key, a ring of four tiles in LDS.  Read from memory three tiles ahead, written a tile later,
@@ -354,12 +353,32 @@ __device__ __forceinline__ Affine scores_by_row(const AttnArgs& a, typename Blk<
     for (int q = 0; q < NB * nq; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int k = 4 * ng * q + e, j = j0 + 4 * g + k;
+            const int k = 4 * ng * q + e;
             float x = s[q / nq][4 * (q % nq) + e] * f.mult + f.add;
             if (near) x += b[k];
-            if (masked && !(j < len && (!km || km[4 * g + k]) && (!a.d.causal || j <= pos))) x = NEG_INF;
             s[q / nq][4 * (q % nq) + e] = x;
         }
+    if (masked) {
+        const int last = a.d.causal ? min(len - 1, pos) : len - 1;        // of this row
+#pragma unroll
+        for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = s[q / nq][4 * (q % nq) + e];
+                s[q / nq][4 * (q % nq) + e] = j0 + 4 * g + 4 * ng * q + e <= last ? x : NEG_INF;
+            }
+        if (km) {
+#pragma unroll
+            for (int q = 0; q < NB * nq; ++q) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(km + 4 * ng * q + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = s[q / nq][4 * (q % nq) + e];
+                    s[q / nq][4 * (q % nq) + e] = (w >> (8 * e)) & 255u ? x : NEG_INF;
+                }
+            }
+        }
+    }
     return Affine{1.f, 0.f};
 }
 
