@@ -488,6 +488,7 @@ extern "C" int ekaid_attn_fwd(const ekaid_attn_t* a, void* workspace, size_t wor
     k.inv_keep = 1.f / (1.f - a->drop_p);
     k.sc2 = a->scale * LOG2E;
     k.gp = p.gp;
+    k.near = !p.few || a->Lk > 512 ? 1 : a->KV % 4 == 0 ? 4 : a->KV % 2 == 0 ? 2 : 1;
     k.tiles = p.tiles;
     k.splits = p.splits;
     k.po = (float*)workspace;

@@ -228,7 +228,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
 // dk, dv: lane = key; the rows of every head that shares it go by in tiles, in units of 32.  What a lane without a valid key computes stays in
 // that lane and is replaced by zero at the end.
 template <typename T, int DH, int G, int NW, int QT, bool REL>
-__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) void attn_dkv_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 16 && sizeof(T) == 2 ? 3 : 2) void attn_dkv_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, U = QT < 32 ? QT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
     constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng;
     __shared__ __attribute__((aligned(16))) T q0s[QT * DH], q1s[QT * DH], g0s[QT * DH], g1s[QT * DH];
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : 2) vo
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G;
     const ekaid_attn_t& d = a.d;
     const int wi = die_order(blockIdx.x, gridDim.x), tl = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
-    const int b = bk / d.KV, kvh = bk % d.KV, group = d.H / d.KV;
+    const int b = bk % d.B, kvh = bk / d.B, group = d.H / d.KV;
     const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tl * NW * G, jw = j0 + wave * G, j = jw + lane % G;
     const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
     const bool ok = j < len && (!mask || mask[j]), live = jw < len;
@@ -453,11 +453,12 @@ static size_t align4(size_t n) { return (n + 3) & ~(size_t)3; }
 static BwdPlan bwd_plan(const ekaid_attn_t* a) {
     BwdPlan p;
     const int esz = a->dtype == EKAID_F32 ? 4 : 2;
-    // blocks of 32 need the registers of one wave a SIMD at 256 wide heads (f32) / 128 wide dk, dv: blocks of 16 there and for few rows
+    // blocks of 32 x 32 halve the LDS reads a product; blocks of 16 x 16 where those of 32 leave registers for one wave a SIMD only (dk, dv of
+    // 128-wide 16-bit heads: 320 -> 275 us for 16 heads x 2048 causal; 64 wide it is 161 against 204 us) and for few rows
     p.gq = a->Lq <= 64 || (esz == 4 && a->dh > 128) ? 16 : 32;
     p.nwq = p.gq == 32 ? 4 : waves_for_rows(a->Lq);
     p.tq = cdiv(a->Lq, p.gq * p.nwq);
-    p.gk = a->Lk <= 64 || a->dh > 128 ? 16 : 32;
+    p.gk = a->Lk <= 64 || a->dh > (esz == 4 ? 128 : 64) ? 16 : 32;
     p.nwk = p.gk == 32 ? 4 : waves_for_rows(a->Lk);
     p.tk = cdiv(a->Lk, p.gk * p.nwk);
     auto split = [](long long wgs, int waves, int work) {
@@ -504,7 +505,7 @@ template <typename T, int DH, int G, int NW, bool REL> static int launch_dkv(con
     return check_launch("attn_dkv");
 }
 template <typename T, int DH, bool REL> static int pick_dkv(const AttnArgs& a, const BwdPlan& p, hipStream_t st) {
-    if constexpr (DH <= 128)
+    if constexpr (DH <= (sizeof(T) == 4 ? 128 : 64))
         if (p.gk == 32) return launch_dkv<T, DH, 32, 4, REL>(a, st);
     if (p.nwk == 1) return launch_dkv<T, DH, 16, 1, REL>(a, st);
     if (p.nwk == 2) return launch_dkv<T, DH, 16, 2, REL>(a, st);
@@ -517,7 +518,7 @@ template <typename T> static int sum_parts(const float* part, void* out, long lo
 template <typename T> static int run_bwd(AttnArgs a, const BwdPlan& p, hipStream_t st) {
     const ekaid_attn_t& d = a.d;
     int rc = EKAID_OK;
-    a.gp = 1;
+    a.gp = a.near = 1;
     a.tiles = p.tq;
     a.splits = p.sq;
     a.dq_parts = p.tq * p.sq;

@@ -32,6 +32,7 @@ struct AttnArgs {
     float inv_keep;
     float sc2;                        // scale * log2(e): the softmax runs on powers of two
     int gp;                           // heads packed into the rows of one workgroup (row r = query r / gp, head r % gp): 1 or H / KV
+    int near;                         // key heads next to each other in the work list (divides KV)
     int tiles;                        // row tiles (forward, dq) / key tiles (dk, dv)
     int splits;                       // workgroups that share a row tile's keys (forward, dq) / a key tile's rows (dk, dv)
     int dq_parts;                     // row-norm words per head that dq wrote (f16)
@@ -382,18 +383,27 @@ __device__ __forceinline__ Affine scores_by_row(const AttnArgs& a, typename Blk<
     return Affine{1.f, 0.f};
 }
 
-struct RowWork {                       // one workgroup's share of the forward / dq work list
+// one workgroup's share of the forward / dq work list.  Order: tile, split, heads that share keys, `near` key heads, sample, the other key
+// heads -- what shares keys is together on a die, and every die sees many samples (dealt sample by sample, the die of the longest one
+// finishes last: 8 ragged samples in training 103 -> 89 us).  near = 4 for few query rows over short states, where latency is the bound
+// and neighbouring heads share pages (64 x 4 heads over 104 f32 states: 16 us, 27 with near = 1), else 1 (32 x 16 heads over a cache of
+// 4096: 83 us, 94 with near = 4).
+struct RowWork {
     int b, head0, kvh, tile, split;
     __device__ __forceinline__ RowWork(const AttnArgs& a) {
-        const int nhg = a.d.H / a.gp, w = die_order(blockIdx.x, gridDim.x);
+        const int w = die_order(blockIdx.x, gridDim.x), group = a.d.H / a.d.KV, shares = group / a.gp;
         tile = w % a.tiles;
         if (a.d.causal) tile = a.tiles - 1 - tile;        // the longest rows first
-        const int rest = w / a.tiles;
+        int rest = w / a.tiles;
         split = rest % a.splits;
-        const int bh = rest / a.splits;
-        b = bh / nhg;
-        head0 = (bh % nhg) * a.gp;
-        kvh = head0 / (a.d.H / a.d.KV);
+        rest /= a.splits;
+        const int share = rest % shares;
+        rest /= shares;
+        const int lo = rest % a.near;
+        rest /= a.near;
+        b = rest % a.d.B;
+        kvh = rest / a.d.B * a.near + lo;
+        head0 = kvh * group + share * a.gp;
     }
 };
 

@@ -1876,11 +1876,6 @@ def lm_loss(logp, target, mask, denom=None):
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # EKAID_F32 / BF16 / F16
 
 
-def _refuse(cond, msg):
-    if cond:
-        raise hip.EkaidError(msg)
-
-
 def _on_device(t):
     """Make ``t``'s device current for the launches inside (kernels run on the device of their tensors, on its current stream)."""
     return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -1954,19 +1949,28 @@ def linear_lm_loss(x, weight, bias, target, mask, denom=None):
     backward.  Rows with mask 0 add nothing and get zero gradients whatever x and target hold there; a target outside the vocabulary in
     a row that counts makes the loss NaN; an all-zero mask gives 0 / 0 (as ``lm_loss``) with zero gradients."""
     require_cuda(x, weight, bias, target, mask, denom)
-    _refuse(x.dim() != 3 or weight.dim() != 2 or weight.shape[1] != x.shape[2] or weight.shape[0] < 1 or x.shape[2] < 1,
-            'linear_lm_loss: x %s and weight %s are (B, T, D) and (V, D)' % (tuple(x.shape), tuple(weight.shape)))
-    _refuse(x.dtype not in _DTYPE_CODE or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype),
-            'linear_lm_loss: x, weight, bias share one of float32, bfloat16, float16 (got %s, %s)' % (x.dtype, weight.dtype))
-    _refuse(x.dtype != torch.float32 and x.shape[2] % 8, 'linear_lm_loss: width %d is not a multiple of 8' % x.shape[2])
-    _refuse(bias is not None and tuple(bias.shape) != (weight.shape[0],), 'linear_lm_loss: bias is (%d,)' % weight.shape[0])
+
+    def refuse(msg, *args):
+        raise hip.EkaidError('linear_lm_loss: ' + msg % args)
+    if x.dim() != 3 or weight.dim() != 2 or weight.shape[1] != x.shape[2] or weight.shape[0] < 1 or x.shape[2] < 1:
+        refuse('x %s and weight %s are (B, T, D) and (V, D)', tuple(x.shape), tuple(weight.shape))
+    if x.dtype not in _DTYPE_CODE or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        refuse('x, weight, bias share one of float32, bfloat16, float16 (got %s, %s)', x.dtype, weight.dtype)
+    if x.dtype != torch.float32 and x.shape[2] % 8:
+        refuse('width %d is not a multiple of 8', x.shape[2])
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        refuse('bias is (%d,)', weight.shape[0])
     for t in (weight, bias, target, mask, denom):
-        _refuse(t is not None and t.device != x.device, 'linear_lm_loss: every tensor must be on %s' % x.device)
+        if t is not None and t.device != x.device:
+            refuse('every tensor must be on %s', x.device)
     B, T = x.shape[:2]
     for name, t, dt in (('target', target, torch.int64), ('mask', mask, torch.float32)):
-        _refuse(t.dim() != 2 or t.dtype != dt or t.shape[0] != B or t.shape[1] < T, 'linear_lm_loss: %s is %s of shape (%d, >= %d)' % (name, dt, B, T))
-    _refuse(denom is not None and (denom.numel() != 1 or denom.dtype != torch.float32), 'linear_lm_loss: denom is a float32 scalar')
-    _refuse(B * T > 1 << 28 or weight.shape[0] > 1 << 28, 'linear_lm_loss: at most 2^28 rows and words')
+        if t.dim() != 2 or t.dtype != dt or t.shape[0] != B or t.shape[1] < T:
+            refuse('%s is %s of shape (%d, >= %d)', name, dt, B, T)
+    if denom is not None and (denom.numel() != 1 or denom.dtype != torch.float32):
+        refuse('denom is a float32 scalar')
+    if B * T > 1 << 28 or weight.shape[0] > 1 << 28:
+        refuse('at most 2^28 rows and words')
     target, mask = (t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous() for t in (target, mask))
     loss = LinearLossFn.apply(x, weight, bias, target, mask, denom)
     assert_finite(loss, 'linear_lm_loss')
@@ -2269,11 +2273,11 @@ _ATTN_MAX_REACH = 1024                                                          
 
 def _vec_rows(t):
     """``t`` (B, L, D) as the attention kernels read it: unit inner stride, whole 16-byte vectors between rows and samples (else a copy)."""
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.clone()
     epl = 16 // t.element_size()
-    if t.numel() == 0:
-        return t.contiguous()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st % epl == 0 for n, st in zip(t.shape[:2], t.stride()[:2]))
-    if ok:
+    sb, sl, sd = t.stride()
+    if sd == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or sb % epl == 0) and (t.shape[1] == 1 or sl % epl == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -2308,23 +2312,25 @@ class AttentionFn(Function):
     (include/ekaid_hip.h: ekaid_attn_t)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, table, cfg):
-        (heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, seed) = cfg
+    def launch(q, k, v, table, cfg, need_lse):
+        """(out, lse or None, the operands as the kernels read them)"""
         q, k, v = _vec_rows(q), _vec_rows(k), _vec_rows(v)
         table = None if table is None else _c(table)
-        B, Lq, D = q.shape
-        out = torch.empty(B, Lq, D, device=q.device, dtype=q.dtype)
-        need = any(ctx.needs_input_grad[:4])
-        lse = torch.empty(B, heads, Lq, device=q.device, dtype=torch.float32) if need else None
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty((q.shape[0], cfg[0], q.shape[1]), device=q.device, dtype=torch.float32) if need_lse else None
         with _on_device(q):
             d = AttentionFn._desc(q, k, v, table, cfg, out, lse)
-            L = hip.lib()
-            nb = L.ekaid_attn_workspace_bytes(ctypes.byref(d), 0)
+            L, r = hip.lib(), ctypes.byref(d)
+            nb = L.ekaid_attn_workspace_bytes(r, 0)
             ws = _scratch(nb, q.device) if nb else None
-            check(L.ekaid_attn_fwd(ctypes.byref(d), ptr(ws), nb, stream()), 'attn_fwd')
-        if need:
-            ctx.cfg = cfg
-            ctx.save_for_backward(q, k, v, table, out, lse, k_len, key_mask, q_pos)
+            check(L.ekaid_attn_fwd(r, ptr(ws), nb, stream()), 'attn_fwd')
+        return out, lse, (q, k, v, table)
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, cfg):
+        out, lse, operands = AttentionFn.launch(q, k, v, table, cfg, any(ctx.needs_input_grad[:4]))
+        ctx.cfg = cfg
+        ctx.save_for_backward(*operands, out, lse, cfg[2], cfg[3], cfg[4])
         return out
 
     @staticmethod
@@ -2374,39 +2380,59 @@ class AttentionFn(Function):
 def _attention(what, q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, training):
     require_cuda(q, k, v, table, k_len, key_mask, q_pos)
     kv_heads = heads if kv_heads is None else kv_heads
-    for t in (q, k, v):
-        _refuse(t.dim() != 3, '%s: q, k, v are (batch, length, heads * width), got %s' % (what, tuple(t.shape)))
-        _refuse(t.dtype not in _DTYPE_CODE or t.dtype != q.dtype, '%s: q, k, v share one of float32, bfloat16, float16 (got %s, %s, %s)' % (what, q.dtype, k.dtype, v.dtype))
+
+    def refuse(msg, *args):
+        raise hip.EkaidError('%s: %s' % (what, msg % args))
+    dtype, dev = q.dtype, q.device
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        refuse('q, k, v are (batch, length, heads * width), got %s, %s, %s', tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    if dtype not in _DTYPE_CODE or k.dtype != dtype or v.dtype != dtype:
+        refuse('q, k, v share one of float32, bfloat16, float16 (got %s, %s, %s)', q.dtype, k.dtype, v.dtype)
     for t in (k, v, table, k_len, key_mask, q_pos):
-        _refuse(t is not None and t.device != q.device, '%s: every tensor must be on %s' % (what, q.device))
+        if t is not None and t.device != dev:
+            refuse('every tensor must be on %s', dev)
     B, Lq, D = q.shape
-    _refuse(heads < 1 or kv_heads < 1 or heads % kv_heads or D % heads, '%s: %d heads, %d key heads, width %d do not divide' % (what, heads, kv_heads, D))
+    Lk = k.shape[1]
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or D % heads:
+        refuse('%d heads, %d key heads, width %d do not divide', heads, kv_heads, D)
     dh = D // heads
-    _refuse(dh % 8 or not 8 <= dh <= 256, '%s: head width %d (a multiple of 8 up to 256)' % (what, dh))
-    _refuse(k.shape != v.shape or k.shape[0] != B or k.shape[2] != kv_heads * dh,
-            '%s: k %s and v %s do not fit q %s with %d of %d heads' % (what, tuple(k.shape), tuple(v.shape), tuple(q.shape), kv_heads, heads))
+    if dh % 8 or not 8 <= dh <= 256:
+        refuse('head width %d (a multiple of 8 up to 256)', dh)
+    if k.shape != v.shape or k.shape[0] != B or k.shape[2] != kv_heads * dh:
+        refuse('k %s and v %s do not fit q %s with %d of %d heads', tuple(k.shape), tuple(v.shape), tuple(q.shape), kv_heads, heads)
     for name, t in (('k_len', k_len), ('q_pos', q_pos)):
-        _refuse(t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,)), '%s: %s is an int32 or int64 tensor of shape (%d,)' % (what, name, B))
+        if t is not None and (t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 or t.shape[0] != B):
+            refuse('%s is an int32 or int64 tensor of shape (%d,)', name, B)
     if key_mask is not None:
-        _refuse(key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, k.shape[1]), '%s: key_mask is a bool tensor of shape %s' % (what, (B, k.shape[1])))
-        if key_mask.stride(1) != 1 and k.shape[1] > 1:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, Lk):
+            refuse('key_mask is a bool tensor of shape %s', (B, Lk))
+        if key_mask.stride(1) != 1 and Lk > 1:
             key_mask = key_mask.contiguous()
-    _refuse(not 0.0 <= p < 1.0, '%s: dropout probability %r' % (what, p))
+    if not 0.0 <= p < 1.0:
+        refuse('dropout probability %r', p)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    _refuse(not math.isfinite(scale), '%s: scale %r' % (what, scale))
+    if not math.isfinite(scale):
+        refuse('scale %r', scale)
     if table is not None:
-        _refuse(table.dim() != 2 or table.shape[1] != heads or table.dtype not in (torch.float32, q.dtype),
-                '%s: table is (buckets, %d), float32 or %s (got %s %s)' % (what, heads, q.dtype, tuple(table.shape), table.dtype))
-        _refuse(bidirectional and table.shape[0] % 2, '%s: %d buckets for two directions' % (what, table.shape[0]))
+        if table.dim() != 2 or table.shape[1] != heads or table.dtype not in (torch.float32, dtype):
+            refuse('table is (buckets, %d), float32 or %s (got %s %s)', heads, dtype, tuple(table.shape), table.dtype)
+        if bidirectional and table.shape[0] % 2:
+            refuse('%d buckets for two directions', table.shape[0])
         side = table.shape[0] // 2 if bidirectional else table.shape[0]
-        _refuse(not 2 <= side <= 128, '%s: 2 to 128 buckets a direction (got %d)' % (what, side))
-        _refuse(int(max_distance) != max_distance or max_distance <= side // 2, '%s: max_distance %r must exceed the %d exact buckets' % (what, max_distance, side // 2))
-        _refuse(relative_borders(side, int(max_distance))[-1] > _ATTN_MAX_REACH, '%s: the last bucket must begin within %d positions' % (what, _ATTN_MAX_REACH))
+        if not 2 <= side <= 128:
+            refuse('2 to 128 buckets a direction (got %d)', side)
+        if int(max_distance) != max_distance or max_distance <= side // 2:
+            refuse('max_distance %r must exceed the %d exact buckets', max_distance, side // 2)
+        if relative_borders(side, int(max_distance))[-1] > _ATTN_MAX_REACH:
+            refuse('the last bucket must begin within %d positions', _ATTN_MAX_REACH)
     p = float(p) if training else 0.0
     cfg = (heads, kv_heads, None if k_len is None else _c(k_len), key_mask, None if q_pos is None else _c(q_pos), bool(causal), bool(bidirectional),
            int(max_distance), scale, p, next_seed() if p > 0.0 else 0)
-    out = AttentionFn.apply(q, k, v, table, cfg)
-    if q.dtype == torch.float32:
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+        out = AttentionFn.apply(q, k, v, table, cfg)
+    else:
+        out = AttentionFn.launch(q, k, v, table, cfg, False)[0]
+    if dtype == torch.float32:
         assert_finite(out, what)
     return out
 
@@ -2428,6 +2454,7 @@ def relative_attention(q, k, v, table, heads, kv_heads=None, k_len=None, key_mas
     share bucket 0.  Per direction the nearest half of the buckets hold one distance each, the others share the distances up to
     ``max_distance`` by logarithm (``relative_borders``), the last takes everything beyond.  The bias is never a (heads, Lq, Lk) tensor;
     its gradient is summed in float32 in a fixed order."""
-    _refuse(table is None, 'relative_attention: table is required')
+    if table is None:
+        raise hip.EkaidError('relative_attention: table is required')
     bidirectional = (not causal) if bidirectional is None else bidirectional
     return _attention('relative_attention', q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, training)
