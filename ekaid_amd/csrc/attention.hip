@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_f
     const int nb = (kend + KB - 1) / KB, per = (nb + a.splits - 1) / a.splits, b0 = w.split * per, b1 = min(nb, b0 + per);
     const unsigned char* mask = d.key_mask ? d.key_mask + w.b * d.mask_batch : nullptr;
     if (d.table) {
-        fill_bias(d, bias, w.head0, a.gp, 0, tid, NT);
+        fill_bias(d, bias, w.head0, a.gp, tid, NT);
         __syncthreads();
     }
     const float* brow = d.table ? bias + hg * (2 * d.reach + 1) + d.reach : nullptr;
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_f
 
 // ---- many query rows: NW * G rows a workgroup, key tiles copied to LDS one tile ahead of the products
 template <typename T, int DH, int G, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) void attn_tile_fwd_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 : 2) void attn_tile_fwd_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, NB = KT / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = KT / (Elem<T>::epl * Blk<G>::ng), MT = DH / G, nv = 4 * Blk<G>::nq;
     __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 8192 ? 1 : 2) vo
     const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
     const int width = d.table ? 2 * (d.reach + BIAS_PAD) + 1 : 0;
     if (d.table) {
-        fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
+        fill_bias_range(d, bias, h, t0 * KT - p0 - min(d.Lq, (w.tile + 1) * NW * G) + 1, t1 * KT - p0 - w.tile * NW * G, tid, NT);
         __syncthreads();
     }
     MaskRing<KT> ring;
@@ -398,11 +398,13 @@ int attn_check(const ekaid_attn_t* a, const char* who) {
 
 struct FwdPlan { int few, g, nw, gp, tiles, splits; size_t ws; };
 
-// Waves of 16 rows: as few rows as possible beyond R (a wave on rows that do not exist costs as much as one on rows that do)
-int waves_for_rows(int R) {
+// Waves of 16 rows a workgroup: as few rows as possible beyond R (a wave on rows that do not exist costs as much as one on rows that do),
+// weighed with what smaller workgroups cost: tiles copied more often; with 64 KB of tiles (`wide`: 256-wide f32 heads) also fewer waves on
+// a compute unit, whose LDS holds two workgroups (64 x 4 heads x 90 x 104: 55 us forward with 4 waves, 82 with 2)
+int waves_for_rows(int R, bool wide) {
     int best = 4, cost = 1 << 30;
     for (int nw = 4; nw >= 1; nw >>= 1) {
-        const int c = cdiv(R, 16 * nw) * 16 * nw * (nw == 4 ? 8 : nw == 2 ? 9 : 12);      // smaller workgroups copy the tiles more often
+        const int c = cdiv(R, 16 * nw) * 16 * nw * (nw == 4 ? 8 : nw == 2 ? (wide ? 14 : 9) : wide ? 24 : 12);
         if (c < cost) { cost = c; best = nw; }
     }
     return best;
@@ -422,7 +424,7 @@ static FwdPlan fwd_plan(const ekaid_attn_t* a) {
         keys = 4 * (esz == 4 ? 16 : 32);
     } else {
         p.g = a->Lq <= 64 || (esz == 4 && a->dh > 128) ? 16 : 32;
-        p.nw = p.g == 32 ? 4 : waves_for_rows(a->Lq);
+        p.nw = p.g == 32 ? 4 : waves_for_rows(a->Lq, esz == 4 && a->dh > 128);
         per_tile = p.g * p.nw;
         keys = attn_kt(esz, a->dh, p.g);
     }

@@ -19,7 +19,7 @@ template <typename T> __device__ __forceinline__ float ds_scale(float norm2) {
 
 // dq (and the bias table's partial sums): lane = query row.  Units of 32 keys of a tile: scores and dP of a unit, then its share of dq.
 template <typename T, int DH, int G, int NW, int KT, bool REL>
-__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void attn_dq_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 : 2) void attn_dq_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, U = KT < 32 ? KT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
     constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng, nv = 4 * nq;
     __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
@@ -37,9 +37,11 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
     const int i = min(row0 + lane % G, d.Lq - 1), p0 = query_pos(d, w.b), pos = p0 + i, pmin = p0 + min(row0, d.Lq - 1), pmax = p0 + min(row0 + G, d.Lq) - 1;
     const int len = key_len(d, w.b), kend = d.causal ? max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G))) : len;
     const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
+    const int rel_lo = t0 * KT - p0 - min(d.Lq, (w.tile + 1) * NW * G) + 1, rel_hi = t1 * KT - p0 - w.tile * NW * G;      // distances this workgroup meets
     if constexpr (REL) {
-        fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
-        for (int x = tid; x < NW * width; x += NT) dsum[x] = 0.f;
+        fill_bias_range(d, bias, h, rel_lo, rel_hi, tid, NT);
+        for (int wv = 0; wv < NW; ++wv)
+            for (int x = max(rel_lo, -d.reach) + tid; x <= min(rel_hi, d.reach); x += NT) dsum[wv * width + x + d.reach] = 0.f;
         __syncthreads();
     }
     MaskRing<KT> ring;
@@ -180,25 +182,31 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) > 256 ? 1 : 2) void at
     }
     if constexpr (REL) {
         __syncthreads();
+        // sums by distance, the waves' in order; then the distances of one bucket in ascending order by one thread
+        const int lo = max(rel_lo, 1 - d.reach), hi = min(rel_hi, d.reach - 1);
+        float* ds = dsum + d.reach;
+        for (int x = lo + tid; x <= hi; x += NT)
+            for (int wv = 1; wv < NW; ++wv) ds[x] += ds[wv * width + x];
         far_back = wave_sum(far_back);
         far_ahead = wave_sum(far_ahead);
         if (lane == 0) {
-            dsum[wave * width] = far_back;
-            dsum[wave * width + 2 * d.reach] = far_ahead;
+            skew[0] = far_back;
+            skew[1] = far_ahead;
         }
         __syncthreads();
-        // distances of one bucket are summed in ascending order by one thread
-        const int nb = (d.n_border + 1) * (d.bidirectional ? 2 : 1);
+        const int side = d.n_border + 1, nb = side * (d.bidirectional ? 2 : 1);
         float* part = a.ptab + ((long long)(w.b * d.H + h) * a.dq_parts + w.tile * a.splits + w.split) * nb;
+        const float* far = dsum + NW * width;
         for (int c = tid; c < nb; c += NT) {
+            const bool ahead = d.bidirectional && c >= side;
+            const int k = c % side, near = k ? d.border[k - 1] : 0, beyond = k == d.n_border ? d.reach : d.border[k];       // distances near .. beyond - 1
             float x = 0.f;
-            const int side = c / (d.n_border + 1), lo = c % (d.n_border + 1) ? d.border[c % (d.n_border + 1) - 1] : 0,
-                      hi = c % (d.n_border + 1) == d.n_border ? d.reach : d.border[c % (d.n_border + 1)] - 1;
+            if (ahead) for (int r = max(max(near, 1), lo); r <= min(beyond - 1, hi); ++r) x += ds[r];
+            else for (int r = max(near, -hi); r <= min(beyond - 1, -lo); ++r) x += ds[-r];
+            if (!d.bidirectional && c == 0) for (int r = max(1, lo); r <= hi; ++r) x += ds[r];
             for (int wv = 0; wv < NW; ++wv) {
-                const float* ds = dsum + wv * width + d.reach;
-                if (d.bidirectional && side) for (int r = max(lo, 1); r <= hi; ++r) x += ds[r];
-                else for (int r = lo; r <= hi; ++r) x += ds[-r];
-                if (!d.bidirectional && c == 0) for (int r = 1; r <= d.reach; ++r) x += ds[r];
+                if (k == d.n_border) x += far[wv * G * (G + 1) + (ahead ? 1 : 0)];
+                if (!d.bidirectional && c == 0) x += far[wv * G * (G + 1) + 1];
             }
             part[c] = x;
         }
@@ -379,7 +387,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
         settle();
         if constexpr (REL) {
             if (bias_head != h) {
-                fill_bias(d, bias, h, 1, BIAS_PAD, tid, NT);
+                fill_bias_range(d, bias, h, j0 - p0 - qtiles * QT, j0 + NW * G - p0, tid, NT);
                 bias_head = h;
                 __syncthreads();
             }
@@ -456,10 +464,10 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
     // blocks of 32 x 32 halve the LDS reads a product; blocks of 16 x 16 where those of 32 leave registers for one wave a SIMD only (dk, dv of
     // 128-wide 16-bit heads: 320 -> 275 us for 16 heads x 2048 causal; 64 wide it is 161 against 204 us) and for few rows
     p.gq = a->Lq <= 64 || (esz == 4 && a->dh > 128) ? 16 : 32;
-    p.nwq = p.gq == 32 ? 4 : waves_for_rows(a->Lq);
+    p.nwq = p.gq == 32 ? 4 : waves_for_rows(a->Lq, esz == 4 && a->dh > 128);
     p.tq = cdiv(a->Lq, p.gq * p.nwq);
     p.gk = a->Lk <= 64 || a->dh > (esz == 4 ? 128 : 64) ? 16 : 32;
-    p.nwk = p.gk == 32 ? 4 : waves_for_rows(a->Lk);
+    p.nwk = p.gk == 32 ? 4 : waves_for_rows(a->Lk, esz == 4 && a->dh > 128);
     p.tk = cdiv(a->Lk, p.gk * p.nwk);
     auto split = [](long long wgs, int waves, int work) {
         const long long want = 4 * 512 / waves;

@@ -284,13 +284,18 @@ __device__ __forceinline__ float table_at(const ekaid_attn_t& d, int bucket, int
     if (d.table_dtype == EKAID_BF16) return (float)reinterpret_cast<const __bf16*>(d.table)[i];
     return (float)reinterpret_cast<const _Float16*>(d.table)[i];
 }
-// bias of `heads` heads by distance, in units of the power-of-two softmax: bias[h][rel + reach + pad], rel in [-reach - pad, reach + pad]
-__device__ __forceinline__ void fill_bias(const ekaid_attn_t& d, float* bias, int head0, int heads, int pad, int tid, int nt) {
-    const int w = 2 * (d.reach + pad) + 1;
-    for (int i = tid; i < heads * w; i += nt) {
-        const int rel = i % w - d.reach - pad;
-        bias[i] = table_at(d, rel_bucket(d, min(max(rel, -d.reach), d.reach)), head0 + i / w) * LOG2E;
-    }
+// bias of `heads` heads by distance, in units of the power-of-two softmax: bias[h][rel + reach], rel in [-reach, reach]
+__device__ __forceinline__ void fill_bias(const ekaid_attn_t& d, float* bias, int head0, int heads, int tid, int nt) {
+    const int w = 2 * d.reach + 1;
+    for (int i = tid; i < heads * w; i += nt) bias[i] = table_at(d, rel_bucket(d, i % w - d.reach), head0 + i / w) * LOG2E;
+}
+
+// the same for one head, padded, and only the distances `lo` .. `hi` a workgroup meets (and the two of everything beyond the reach)
+__device__ __forceinline__ void fill_bias_range(const ekaid_attn_t& d, float* bias, int head, int lo, int hi, int tid, int nt) {
+    lo = max(lo, -d.reach - BIAS_PAD);
+    hi = min(hi, d.reach + BIAS_PAD);
+    for (int rel = lo + tid; rel <= hi; rel += nt) bias[rel + d.reach + BIAS_PAD] = table_at(d, rel_bucket(d, min(max(rel, -d.reach), d.reach)), head) * LOG2E;
+    if (tid < 2) bias[BIAS_PAD + tid * 2 * d.reach] = table_at(d, rel_bucket(d, tid ? d.reach : -d.reach), head) * LOG2E;
 }
 
 // which workgroup works on what: consecutive work items (tiles of one head, which share their keys) on ONE die -- workgroups are dealt
@@ -409,7 +414,7 @@ struct RowWork {
 
 int attn_check(const ekaid_attn_t* a, const char* who);
 int attn_lds_limit(const void* fn, int bytes);      // once per kernel and device: the dynamic LDS it may be launched with
-int waves_for_rows(int R);
+int waves_for_rows(int R, bool wide);
 // keys (or rows) a tile of the copying kernels: 16 KB an operand, twice two of them leave room for two workgroups a compute unit
 constexpr int attn_kt(int esize, int dh, int g) { return esize == 4 && dh > 128 ? 16 : g == 16 || dh > 128 || (esize == 4 && dh > 64) ? 32 : 64; }
 size_t attn_bwd_workspace(const ekaid_attn_t* a);
