@@ -10,6 +10,7 @@
 #include "common.h"
 #include "../../include/ekaid_hip.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace ekaid {
 namespace {
@@ -27,12 +28,13 @@ constexpr float NEG_INF = -__builtin_inff();
 constexpr int BK = 64;
 __device__ __attribute__((aligned(16))) const uint32_t zero16[4] = {0u, 0u, 0u, 0u};
 
-// ---- per-call state: [meta: count | sum mask | max |mask| ...][lse2 N][target logit N][idx N][pos N]
+// ---- per-call state: [meta: count | sum mask | max |mask| ...][lse2 N][target logit N][nll N][idx N][pos N]
 struct State {
     int* count;
-    float* sums;         // [0] sum of the mask, [1] max |mask|
+    float* sums;         // [0] sum of the mask, [1] max |mask|, [2] largest scale of the weight's rows (f32 terms)
     float* lse;          // log2 denominators, by compact row (16-bit) or by row (f32)
     float* tz;           // target logit in powers of two
+    float* nll;          // mask (lse - z_target), by compact row (f32 through ekaid_gemm_f32: by row)
     int* idx;            // compact row -> row
     int* pos;            // row -> compact row, or -1
 };
@@ -43,50 +45,74 @@ State state_of(void* p, long long n) {
     s.sums = (float*)(c + 64);
     s.lse = (float*)(c + 256);
     s.tz = s.lse + n;
-    s.idx = (int*)(s.tz + n);
+    s.nll = s.tz + n;
+    s.idx = (int*)(s.nll + n);
     s.pos = s.idx + n;
     return s;
 }
 
-// the rows that count, in order; sum and largest magnitude of the mask.  One workgroup: thread t owns a run of rows (fixed order).
+// the rows that count, in order; sum and largest magnitude of the mask (thread t: rows t, t + 1024, ...: a fixed order).  One workgroup,
+// 16 x 1024 rows at a time: loads together, then one prefix sum over the 256 wave counts.
 __global__ __launch_bounds__(1024) void ll_rows_kernel(const float* mask, long long ld, int B, int T, State st) {
-    const long long n = (long long)B * T;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const long long per = (n + 1023) / 1024, r0 = min(n, t * per), r1 = min(n, r0 + per);
-    int c = 0;
-    float s = 0.f, mx = 0.f;
-    for (long long r = r0; r < r1; ++r) {
-        const float m = mask[(r / T) * ld + r % T];
-        c += m != 0.f ? 1 : 0;
-        s += m;
-        mx = fmaxf(mx, fabsf(m));
-    }
-    int incl = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += v;
-    }
-    __shared__ int wsum[16];
+    constexpr int U = 16;
+    const int n = B * T, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    __shared__ int cnt[U * 16 + 1];
     __shared__ float ssum[1024], smax[16];
+    int base = 0;
+    float s = 0.f, mx = 0.f;
+    for (int r0 = 0; r0 < n; r0 += U * 1024) {
+        float m[U];
+        unsigned long long on[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int r = r0 + 1024 * k + t;
+            m[k] = r < n ? mask[(long long)(r / T) * ld + r % T] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            s += m[k];
+            mx = fmaxf(mx, fabsf(m[k]));
+            on[k] = __ballot(m[k] != 0.f);
+            if (lane == 0) cnt[k * 16 + wave] = __popcll(on[k]);
+        }
+        __syncthreads();
+        if (wave == 0) {                                       // exclusive prefix sums of 256 counts, four a lane
+            int c[4], sum = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                c[k] = sum;
+                sum += cnt[4 * lane + k];
+            }
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(incl, o, 64);
+                if (lane >= o) incl += v;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) cnt[4 * lane + k] = incl - sum + c[k];
+            if (lane == 63) cnt[U * 16] = incl;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int r = r0 + 1024 * k + t;
+            if (r >= n) continue;
+            const int p = base + cnt[k * 16 + wave] + __popcll(on[k] & ((1ull << lane) - 1));
+            const bool mine = m[k] != 0.f;
+            if (mine) {
+                st.idx[p] = r;
+                st.tz[p] = __builtin_nanf("");                 // stays NaN when the target is no word of the vocabulary
+            }
+            st.pos[r] = mine ? p : -1;
+        }
+        base += cnt[U * 16];
+        __syncthreads();
+    }
     ssum[t] = s;
     mx = wave_max(mx);
-    if (lane == 63) wsum[wave] = incl;
     if (lane == 0) smax[wave] = mx;
     __syncthreads();
-    int base = incl - c, total = 0;
-    for (int w = 0; w < 16; ++w) {
-        if (w < wave) base += wsum[w];
-        total += wsum[w];
-    }
-    for (long long r = r0; r < r1; ++r) {
-        const bool on = mask[(r / T) * ld + r % T] != 0.f;
-        if (on) {
-            st.idx[base] = (int)r;
-            st.tz[base] = __builtin_nanf("");                  // stays NaN when the target is no word of the vocabulary
-        }
-        st.pos[r] = on ? base++ : -1;
-    }
     for (int w = 512; w > 0; w >>= 1) {
         if (t < w) ssum[t] += ssum[t + w];
         __syncthreads();
@@ -94,7 +120,7 @@ __global__ __launch_bounds__(1024) void ll_rows_kernel(const float* mask, long l
     if (t == 0) {
         float m = smax[0];
         for (int w = 1; w < 16; ++w) m = fmaxf(m, smax[w]);
-        st.count[0] = total;
+        st.count[0] = base;
         st.sums[0] = ssum[0];
         st.sums[1] = m;
     }
@@ -115,10 +141,11 @@ template <int R, bool COL, int NW> struct Operand {
     const char* p[chunks];
     int k0[chunks];                       // first contracted element of this lane's vector (COL: its row), or a large value: read zeros
     long long step;                       // bytes per 64 contracted elements
-    __device__ __forceinline__ void issue(char* lds, int kt, int K, int wave) const {
+    long long plane;                      // bytes between the 16-bit planes of an f32 operand
+    __device__ __forceinline__ void issue(char* lds, int kt, int pl, int K, int wave) const {
 #pragma unroll
         for (int i = 0; i < chunks; ++i) {
-            const char* src = kt * BK + k0[i] < K ? p[i] + kt * step : (const char*)zero16;
+            const char* src = kt * BK + k0[i] < K ? p[i] + kt * step + pl * plane : (const char*)zero16;
             __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(lds + (i * NW + wave) * 1024), 16, 0, 0);
         }
     }
@@ -166,16 +193,18 @@ template <int R, bool COL> __device__ __forceinline__ u32x4 operand_frag(const c
     }
 }
 
-// acc[mi][ni] += sum over k in [64 kt0, 64 kt1) of A(m, k) B(n, k); BM x BN per workgroup, WM x WN per wave.  Two LDS buffers: the copies
+// f32 operands come as planes of 16-bit terms; their product is the sum of plane products (largest last):
+//   3 pairs: two f16 terms an operand (rows scaled by powers of two: 22 significant bits), h h + h l + l h
+//   6 pairs: three bf16 terms (exact), the six products above 2^-24
+template <int PAIRS> __device__ __forceinline__ int pair_a(int i) { return PAIRS == 1 ? 0 : PAIRS == 3 ? (i == 0) : (0x201100 >> (4 * (5 - i))) & 15; }
+template <int PAIRS> __device__ __forceinline__ int pair_b(int i) { return PAIRS == 1 ? 0 : PAIRS == 3 ? (i == 1) : (0x021010 >> (4 * (5 - i))) & 15; }
+
+// acc[mi][ni] += sum over k in [64 kt0, 64 kt1) of A(m, k) B(n, k), for every pair of planes; BM x BN per workgroup, WM x WN per wave.  Two LDS buffers: the copies
 // of tile t + 1 are under way while tile t is multiplied; ONE barrier a tile, behind a wait for this wave's copies and LDS reads.
-template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL> struct TileProduct {
-    static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, NT = 64 * NW, MI = WM / 32, NI = WN / 32;
+template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int PAIRS> struct TileProduct {
+    static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, NT = 64 * NW, MI = WM / 32, NI = WN / 32, STAGES = BM == 128 ? 4 : 2;
     typedef Operand<BM, ACOL, NW> A;
     typedef Operand<BN, BCOL, NW> B;
-    static __device__ __forceinline__ void settle() {
-        __builtin_amdgcn_s_waitcnt(0x0070);               // vmcnt 0, lgkmcnt 0
-        __builtin_amdgcn_s_barrier();
-    }
     static __device__ __forceinline__ void step(f32x16 (&acc)[MI][NI], const char* a, const char* b, int wave, int lane) {
         const int m0 = (wave / NWN) * WM, n0 = (wave % NWN) * WN;
 #pragma unroll
@@ -191,9 +220,20 @@ template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL> stru
                 for (int j = 0; j < NI; ++j) acc[i][j] = mma32<T>(fa[i], fb[j], acc[i][j]);
         }
     }
-    // K: contracted elements in all (vectors beyond read as zero)
-    static __device__ __forceinline__ void run(f32x16 (&acc)[MI][NI], const A& oa, const B& ob, int kt0, int kt1, int K, char* a0, char* a1, char* b0, char* b1,
-                                               int wave, int lane) {
+    // how many of this wave's copies may still be under way when `newer` tiles behind the one wanted have been asked for
+    static __device__ __forceinline__ void arrive(int newer) {
+        constexpr int per = A::chunks + B::chunks;            // copies a tile
+        static_assert(per == 8, "");
+        if (newer >= 2) __builtin_amdgcn_s_waitcnt(0x4070);  // vmcnt 16, lgkmcnt 0
+        else if (newer == 1) __builtin_amdgcn_s_waitcnt(0x0078);
+        else __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_barrier();
+    }
+    // K: contracted elements in all (vectors beyond read as zero).  Two buffers where a tile's products (256 x 256: 2 waves a SIMD x 1024
+    // matrix cycles) cover the latency of the next tile's copies, four where they do not (128 x 128: 512 cycles) and the grid is small
+    // anyway; one barrier a tile: behind it the wanted tile is complete and the buffer of the tile before is free.
+    static __device__ __forceinline__ void run(f32x16 (&acc)[MI][NI], const A& oa, const B& ob, int kt0, int kt1, int K, char* a0, char* a1, char* a2, char* a3, char* b0,
+                                               char* b1, char* b2, char* b3, int wave, int lane) {
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -201,30 +241,67 @@ template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL> stru
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
         if (kt0 < kt1) {
-            oa.issue(a0, kt0, K, wave);
-            ob.issue(b0, kt0, K, wave);
-        }
-        for (int kt = kt0; kt < kt1; kt += 2) {
-            settle();
-            if (kt + 1 < kt1) {
-                oa.issue(a1, kt + 1, K, wave);
-                ob.issue(b1, kt + 1, K, wave);
-            }
-            step(acc, a0, b0, wave, lane);
-            if (kt + 1 < kt1) {
-                settle();
-                if (kt + 2 < kt1) {
-                    oa.issue(a0, kt + 2, K, wave);
-                    ob.issue(b0, kt + 2, K, wave);
+            int kt = kt0, pair = 0;                         // of the tile copied next
+            auto copy = [&](char* la, char* lb) __attribute__((always_inline)) {
+                oa.issue(la, kt, pair_a<PAIRS>(pair), K, wave);
+                ob.issue(lb, kt, pair_b<PAIRS>(pair), K, wave);
+                if (++kt == kt1) { kt = kt0; ++pair; }
+            };
+            const int total = PAIRS * (kt1 - kt0);
+            copy(a0, b0);
+            if constexpr (STAGES == 2) {
+                for (int t = 0; t < total; t += 2) {
+                    arrive(0);
+                    if (t + 1 < total) copy(a1, b1);
+                    step(acc, a0, b0, wave, lane);
+                    if (t + 1 < total) {
+                        arrive(0);
+                        if (t + 2 < total) copy(a0, b0);
+                        step(acc, a1, b1, wave, lane);
+                    }
                 }
-                step(acc, a1, b1, wave, lane);
+            } else {
+                if (total > 1) copy(a1, b1);
+                if (total > 2) copy(a2, b2);
+                for (int t = 0; t < total; t += 4) {
+                    arrive(total - 1 - t);
+                    if (t + 3 < total) copy(a3, b3);
+                    step(acc, a0, b0, wave, lane);
+                    if (t + 1 >= total) break;
+                    arrive(total - 2 - t);
+                    if (t + 4 < total) copy(a0, b0);
+                    step(acc, a1, b1, wave, lane);
+                    if (t + 2 >= total) break;
+                    arrive(total - 3 - t);
+                    if (t + 5 < total) copy(a1, b1);
+                    step(acc, a2, b2, wave, lane);
+                    if (t + 3 >= total) break;
+                    arrive(total - 4 - t);
+                    if (t + 6 < total) copy(a2, b2);
+                    step(acc, a3, b3, wave, lane);
+                }
             }
         }
-        settle();                                           // the LDS is free for the epilogue
+        arrive(0);                                          // the LDS is free for the epilogue
     }
 };
-#define LL_LDS(BM, BN)                                                                                                          \
-    __shared__ __attribute__((aligned(16))) char la0[BM * BK * 2], la1[BM * BK * 2], lb0[BN * BK * 2], lb1[BN * BK * 2]
+// (the copies' buffers are arrays of their own, so that the compiler knows which reads a copy under way concerns)
+#define LL_LDS(BM, BN)                                                                                                                                       \
+    __shared__ __attribute__((aligned(16))) char la0[BM * BK * 2], la1[BM * BK * 2], lb0[BN * BK * 2], lb1[BN * BK * 2], la2[BM == 128 ? BM * BK * 2 : 16],   \
+        la3[BM == 128 ? BM * BK * 2 : 16], lb2[BM == 128 ? BN * BK * 2 : 16], lb3[BM == 128 ? BN * BK * 2 : 16]
+#define LL_BUFFERS la0, la1, la2, la3, lb0, lb1, lb2, lb3
+
+// workgroups that share an output tile's contraction: the smallest number that fills the chip's rounds of 256 well, pieces of >= 8 tiles
+__host__ __device__ inline int ll_splits(int tiles, int ksteps, int most) {
+    int best = 1;
+    float filled = 0.f;                                       // (each share writes its own f32 partial tile: no more than needed)
+    for (int s = 1; s <= most && (s == 1 || ksteps / s >= 8); ++s) {
+        const int wg = tiles * s, rounds = (wg + 255) / 256;
+        const float f = rounds ? wg / (256.f * rounds) : 1.f;
+        if (filled < 0.85f && f > filled + 0.05f) { filled = f; best = s; }
+    }
+    return best;
+}
 
 struct LossArgs {
     ekaid_linear_loss_t d;
@@ -235,11 +312,19 @@ struct LossArgs {
     int ldz;
     float2* part;             // [word tiles][nr] per-row (max, sum) of a tile
     unsigned short* dz;       // [nr][ldz]
-    const unsigned short* xc; // [nr][D] the rows that count, zeros behind
+    const unsigned short* xc; // [nr][D] the rows that count, zeros behind (f32: [nr][2][D] f16 terms)
+    const unsigned short* xb; // f32: [nr][3][D] bf16 terms of the rows that count
+    const unsigned short* wp; // the weight (f32: [V][2][D] f16 terms)
+    const float* sx;          // f32: powers of two that take the scale of a row of x / of the weight out again
+    const float* sw;
+    float* up;                // f32: per row, the power of two its dz terms are stored without
+    unsigned short* dzb;      // f32: [nr][3][ldz] bf16 terms of dz (dz: [nr][2][ldz] f16 terms of dz sw, for dx)
     float* pdb;               // [row tiles][ldz] bias partials
     float* pdx;               // [splits][nr][D]
     float* pdw;               // [splits][ldz][D] (splits > 1)
-    int splits;
+    int splits;               // dW: workgroups that share a tile; dx: the most that may
+    int* dx_shares;           // the number dx took
+    int first_vp;             // words of the first piece (every piece is split like it)
     int first;                // first piece: dx partials are written, later ones added
 };
 
@@ -261,9 +346,15 @@ __device__ __forceinline__ float to_f32(const void* p, long long i, int dtype) {
 }
 
 // forward: lanes = rows, registers = words (m), so a row's maximum and sum over the tile are lane-local but for one exchange
+// (T: float means f16 terms of f32 operands)
+template <typename T> struct Term { typedef T type; static constexpr int planes = 1, pairs = 1; };
+template <> struct Term<float> { typedef _Float16 type; static constexpr int planes = 2, pairs = 3; };
+
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(const LossArgs a) {
-    typedef TileProduct<T, BM, BN, WM, WN, false, false> P;
+    typedef TileProduct<typename Term<T>::type, BM, BN, WM, WN, false, false, Term<T>::pairs> P;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NP = Term<T>::planes;
     LL_LDS(BM, BN);
     const int count = a.st.count[0], tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5;
     int rt, wt;
@@ -271,13 +362,21 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(co
     const int w0 = wt * BM, n0 = rt * BN;
     typename P::A oa;
     typename P::B ob;
-    oa.init_rows([&](int r) { return (const char*)a.d.weight + (long long)min(w0 + r, a.d.V - 1) * a.d.D * 2; }, wave, lane);
-    ob.init_rows([&](int r) { return (const char*)a.d.x + a.st.idx[min(n0 + r, count - 1)] * a.d.ldx * 2; }, wave, lane);
+    oa.init_rows([&](int r) { return (const char*)a.wp + (long long)min(w0 + r, a.d.V - 1) * NP * a.d.D * 2; }, wave, lane);
+    ob.init_rows([&](int r) {
+        const int n = min(n0 + r, count - 1);
+        return F32 ? (const char*)a.xc + (long long)n * NP * a.d.D * 2 : (const char*)a.d.x + a.st.idx[n] * a.d.ldx * 2;
+    }, wave, lane);
+    oa.plane = ob.plane = (long long)a.d.D * 2;
     f32x16 acc[P::MI][P::NI];
-    P::run(acc, oa, ob, 0, (a.d.D + BK - 1) / BK, a.d.D, la0, la1, lb0, lb1, wave, lane);
+    P::run(acc, oa, ob, 0, (a.d.D + BK - 1) / BK, a.d.D, LL_BUFFERS, wave, lane);
     float* bias = reinterpret_cast<float*>(la0);               // [BM], -inf behind the vocabulary
+    float* scale = bias + BM;                                  // [BM] f32: of the word's terms, times log2 e
     float2* red = reinterpret_cast<float2*>(la1);              // [BM / WM][BN]
-    for (int i = tid; i < BM; i += P::NT) bias[i] = w0 + i < a.d.V ? (a.d.bias ? to_f32(a.d.bias, w0 + i, a.d.dtype) * LOG2E : 0.f) : NEG_INF;
+    for (int i = tid; i < BM; i += P::NT) {
+        bias[i] = w0 + i < a.d.V ? (a.d.bias ? to_f32(a.d.bias, w0 + i, a.d.dtype) * LOG2E : 0.f) : NEG_INF;
+        if (F32) scale[i] = a.sw[min(w0 + i, a.d.V - 1)] * LOG2E;
+    }
     __syncthreads();
     const int wm = wave / P::NWN, wn = wave % P::NWN;
 #pragma unroll
@@ -287,6 +386,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(co
         const int row = ok ? a.st.idx[n] : 0;
         const long long tg = ok ? a.d.target[(row / a.d.T) * a.d.ld_target + row % a.d.T] : -1;
         const int tl = tg >= w0 && tg < w0 + BM && tg < a.d.V ? (int)(tg - w0) : -1;
+        const float sx = F32 ? a.sx[min(n, count - 1)] : 1.f;
         float mx = NEG_INF, tz = 0.f;
         bool mine = false;
 #pragma unroll
@@ -295,9 +395,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(co
             for (int q = 0; q < 4; ++q) {
                 const int ml = wm * WM + 32 * i + 8 * q + 4 * g;
                 const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias + ml);
+                f32x4 s4 = {LOG2E, LOG2E, LOG2E, LOG2E};
+                if (F32) s4 = *reinterpret_cast<const f32x4*>(scale + ml) * sx;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = acc[i][j][4 * q + e] * LOG2E + b4[e];
+                    const float z = acc[i][j][4 * q + e] * s4[e] + b4[e];
                     acc[i][j][4 * q + e] = z;
                     mx = fmaxf(mx, z);
                     tz = ml + e == tl ? z : tz;
@@ -327,15 +429,15 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(co
     }
 }
 
-// lse of a row from its tiles: 64 rows x 4 strands of tiles a workgroup
-__global__ __launch_bounds__(256) void ll_lse_kernel(const LossArgs a, int tiles) {
-    __shared__ float sm[4][64], sl[4][64];
+// lse of a row from its tiles: 64 rows x 16 strands of tiles a workgroup
+__global__ __launch_bounds__(1024) void ll_lse_kernel(const LossArgs a, int tiles) {
+    __shared__ float sm[16][64], sl[16][64];
     const int r = threadIdx.x & 63, k = threadIdx.x >> 6;
     const long long n = (long long)blockIdx.x * 64 + r;
     const bool ok = n < a.st.count[0];
     float m = NEG_INF, l = 0.f;
     if (ok)
-        for (int t = k; t < tiles; t += 4) {
+        for (int t = k; t < tiles; t += 16) {
             const float2 p = a.part[t * a.nr + n];
             const float mm = fmaxf(m, p.x), base = mm == NEG_INF ? 0.f : mm;
             l = l * __builtin_amdgcn_exp2f(m - base) + p.y * __builtin_amdgcn_exp2f(p.x - base);
@@ -345,22 +447,27 @@ __global__ __launch_bounds__(256) void ll_lse_kernel(const LossArgs a, int tiles
     sl[k][r] = l;
     __syncthreads();
     if (k || !ok) return;
-    for (int i = 1; i < 4; ++i) m = fmaxf(m, sm[i][r]);
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, sm[i][r]);
     const float base = m == NEG_INF ? 0.f : m;
     l = 0.f;
-    for (int i = 0; i < 4; ++i) l += sl[i][r] * __builtin_amdgcn_exp2f(sm[i][r] - base);
-    a.st.lse[n] = m + __builtin_amdgcn_logf(l);
+    for (int i = 0; i < 16; ++i) l += sl[i][r] * __builtin_amdgcn_exp2f(sm[i][r] - base);
+    const float lse = m + __builtin_amdgcn_logf(l);
+    const int row = a.st.idx[n];
+    a.st.lse[n] = lse;
+    a.st.nll[n] = (lse - a.st.tz[n]) * LN2 * a.d.mask[(row / a.d.T) * a.d.ld_mask + row % a.d.T];
 }
 
-// loss = sum mask (lse - z_target) / denom, in double and a fixed order
+// loss = sum nll / denom, in double and a fixed order
 __global__ __launch_bounds__(1024) void ll_loss_kernel(const ekaid_linear_loss_t d, State st, int by_row) {
     __shared__ double s[1024];
     const int count = by_row ? d.B * d.T : st.count[0];
     double x = 0.0;
-    for (int n = threadIdx.x; n < count; n += 1024) {
-        const int row = by_row ? n : st.idx[n];
-        const float m = d.mask[(row / d.T) * d.ld_mask + row % d.T];
-        if (m != 0.f) x += (double)((st.lse[n] - st.tz[n]) * LN2) * m;
+    for (int n0 = 0; n0 < count; n0 += 8192) {                   // eight loads under way
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = n0 + 1024 * k + (int)threadIdx.x < count ? st.nll[n0 + 1024 * k + threadIdx.x] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x += (double)v[k];
     }
     s[threadIdx.x] = x;
     __syncthreads();
@@ -387,37 +494,51 @@ template <typename T> __device__ __forceinline__ unsigned short to_bits(float v)
 // (softmax - onehot) mask / max |mask| lies in [-1, 1]; f16 takes it times 2^14, so that probabilities down to 2^-38 keep a value
 template <typename T> struct DzScale { static constexpr float up = __is_same(T, _Float16) ? 16384.f : 1.f; };
 
-// output tile through LDS: lanes hold columns, registers rows; written as whole 16-byte vectors
-template <typename T, int BM, int BN, int WM, int WN, int MI, int NI, int NT>
-__device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NI], float f, T* out, long long ld, int rows, int cols, char* l0, char* l1, char* l2, char* l3,
-                                           int tid, int wave, int lane) {
-    constexpr int NWN = BN / WN, Q = BM / 4;                   // a quarter of the rows in each of the four operand buffers
-    static_assert(Q * BN <= BM * BK && Q % 32 == 0, "");
+// output tile through LDS: lanes hold columns, registers rows; bits(value) is what is stored, written as whole 16-byte vectors
+template <int BM, int BN, int WM, int WN, int MI, int NI, int NT, typename Bits>
+__device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NI], Bits bits, unsigned short* out, long long ld, int rows, int cols, char* l0, char* l1, char* l2,
+                                           char* l3, int tid, int wave, int lane) {
+    constexpr int NWN = BN / WN, Q = BM / 4, HALF = MI / 2;    // a quarter of the rows in each of the four operand buffers: two a wave
+    static_assert(Q * BN <= BM * BK && WM == 2 * Q && HALF * 32 == Q, "");
     const int wm = wave / NWN, wn = wave % NWN, g = lane >> 5;
-    char* const buf[4] = {l0, l1, l2, l3};
+    const int at = 4 * g * BN + wn * WN + (lane & 31);
+    unsigned short* const lo = reinterpret_cast<unsigned short*>(wm ? l2 : l0) + at;
+    unsigned short* const hi = reinterpret_cast<unsigned short*>(wm ? l3 : l1) + at;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int rb = wm * WM + 32 * i;
-        unsigned short* t = reinterpret_cast<unsigned short*>(buf[rb / Q]) + (rb % Q) * BN;
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t[(8 * (r >> 2) + 4 * g + (r & 3)) * BN + wn * WN + 32 * j + (lane & 31)] = to_bits<T>(acc[i][j][r] * f);
-    }
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * (i % HALF) + 8 * (r >> 2) + (r & 3);
+                (i < HALF ? lo : hi)[row * BN + 32 * j] = bits(acc[i][j][r]);
+            }
     __syncthreads();
     constexpr int vpr = BN / 8;
-    for (int k = tid; k < BM * vpr; k += NT) {
-        const int r = k / vpr, c = (k % vpr) * 8;
-        if (r < rows && c < cols) *reinterpret_cast<u32x4*>(out + r * ld + c) = *reinterpret_cast<const u32x4*>(buf[r / Q] + ((r % Q) * BN + c) * 2);
-    }
+    const auto flush = [&](const char* l, int q) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k0 = 0; k0 < Q * vpr; k0 += NT) {
+            const int k = k0 + tid, r = k / vpr, c = (k % vpr) * 8;
+            if (q * Q + r < rows && c < cols) *reinterpret_cast<u32x4*>(out + (q * Q + r) * ld + c) = *reinterpret_cast<const u32x4*>(l + (r * BN + c) * 2);
+        }
+    };
+    flush(l0, 0);
+    __builtin_amdgcn_sched_barrier(0);                         // (not all sixteen vectors in registers beside the accumulators)
+    flush(l1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    flush(l2, 2);
+    __builtin_amdgcn_sched_barrier(0);
+    flush(l3, 3);
 }
 
 // backward of the logits of one piece: lanes = words, registers = rows
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const LossArgs a) {
-    typedef TileProduct<T, BM, BN, WM, WN, false, false> P;
+    typedef TileProduct<typename Term<T>::type, BM, BN, WM, WN, false, false, Term<T>::pairs> P;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NP = Term<T>::planes;
     LL_LDS(BM, BN);
-    __shared__ float slse[BM], sw[BM], sdb[BM / WM][BN];
+    __shared__ float slse[BM], sw[BM], srow[BM], sdb[BM / WM][BN];
     __shared__ int stg[BM];
     const int count = a.st.count[0], tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5;
     int rt, wt;
@@ -425,8 +546,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
     const int m0 = rt * BM, w0 = a.v0 + wt * BN, end = a.v0 + a.vp;
     typename P::A oa;
     typename P::B ob;
-    oa.init_rows([&](int r) { return (const char*)(a.xc + (long long)(m0 + r) * a.d.D); }, wave, lane);
-    ob.init_rows([&](int r) { return (const char*)a.d.weight + (long long)min(w0 + r, a.d.V - 1) * a.d.D * 2; }, wave, lane);
+    oa.init_rows([&](int r) { return (const char*)(a.xc + (long long)(m0 + r) * NP * a.d.D); }, wave, lane);
+    ob.init_rows([&](int r) { return (const char*)a.wp + (long long)min(w0 + r, a.d.V - 1) * NP * a.d.D * 2; }, wave, lane);
+    oa.plane = ob.plane = (long long)a.d.D * 2;
     const float top = a.st.sums[1];
     for (int i = tid; i < BM; i += P::NT) {
         const bool ok = m0 + i < count;
@@ -435,31 +557,46 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
         slse[i] = ok ? a.st.lse[m0 + i] : __builtin_inff();
         sw[i] = ok ? a.d.mask[(row / a.d.T) * a.d.ld_mask + row % a.d.T] / top : 0.f;
         stg[i] = tg >= w0 && tg < min(w0 + BN, end) ? (int)(tg - w0) : -1;
+        if (F32) srow[i] = ok ? a.sx[m0 + i] * LOG2E : 0.f;
     }
     f32x16 acc[P::MI][P::NI];
-    P::run(acc, oa, ob, 0, (a.d.D + BK - 1) / BK, a.d.D, la0, la1, lb0, lb1, wave, lane);
+    P::run(acc, oa, ob, 0, (a.d.D + BK - 1) / BK, a.d.D, LL_BUFFERS, wave, lane);
     const int wm = wave / P::NWN, wn = wave % P::NWN;
+    float wscale[P::NI], bias[P::NI], sum[P::NI];
+    int word[P::NI];
 #pragma unroll
     for (int j = 0; j < P::NI; ++j) {
-        const int nl = wn * WN + 32 * j + (lane & 31), v = w0 + nl;
-        const float bias = v < end ? (a.d.bias ? to_f32(a.d.bias, v, a.d.dtype) * LOG2E : 0.f) : NEG_INF;
-        float sum = 0.f;
+        word[j] = wn * WN + 32 * j + (lane & 31);
+        const int v = w0 + word[j];
+        bias[j] = v < end ? (a.d.bias ? to_f32(a.d.bias, v, a.d.dtype) * LOG2E : 0.f) : NEG_INF;
+        wscale[j] = F32 ? a.sw[min(v, a.d.V - 1)] : 1.f;
+        sum[j] = 0.f;
+    }
 #pragma unroll
-        for (int i = 0; i < P::MI; ++i)
+    for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int ml = wm * WM + 32 * i + 8 * q + 4 * g;
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(slse + ml), w4 = *reinterpret_cast<const f32x4*>(sw + ml);
+        for (int q = 0; q < 4; ++q) {                         // (rows outside, words inside: what belongs to a row is read once and not kept)
+            const int ml = wm * WM + 32 * i + 8 * q + 4 * g;
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(slse + ml), w4 = *reinterpret_cast<const f32x4*>(sw + ml);
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const i32x4 t4 = *reinterpret_cast<const i32x4*>(stg + ml);
+            f32x4 s4 = {LOG2E, LOG2E, LOG2E, LOG2E};
+            if (F32) s4 = *reinterpret_cast<const f32x4*>(srow + ml);
+#pragma unroll
+            for (int j = 0; j < P::NI; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] * LOG2E + bias - l4[e]);
-                    const float dz = w4[e] == 0.f ? 0.f : (p - (stg[ml + e] == nl ? 1.f : 0.f)) * w4[e];
+                    const float p = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] * (F32 ? s4[e] * wscale[j] : LOG2E) + (bias[j] - l4[e]));
+                    const float dz = w4[e] == 0.f ? 0.f : (p - (t4[e] == word[j] ? 1.f : 0.f)) * w4[e];
                     acc[i][j][4 * q + e] = dz;
-                    sum += dz;
+                    sum[j] += dz;
                 }
-            }
-        sum += __shfl_xor(sum, 32, 64);
-        if (g == 0) sdb[wm][nl] = sum;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+    for (int j = 0; j < P::NI; ++j) {
+        sum[j] += __shfl_xor(sum[j], 32, 64);
+        if (g == 0) sdb[wm][word[j]] = sum[j];
     }
     __syncthreads();
     for (int nl = tid; nl < BN; nl += P::NT) {
@@ -468,8 +605,64 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
         for (int w = 0; w < BM / WM; ++w) s += sdb[w][nl];
         if (wt * BN + nl < a.ldz) a.pdb[(long long)rt * a.ldz + wt * BN + nl] = s;
     }
-    store_tile<T, BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, DzScale<T>::up, (T*)a.dz + (long long)m0 * a.ldz + wt * BN, a.ldz, BM, a.ldz - wt * BN, la0, la1, lb0, lb1, tid,
-                                                       wave, lane);
+    const int cols = a.ldz - wt * BN;
+    if constexpr (!F32) {
+        store_tile<BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, [&](float v) { return to_bits<T>(v * DzScale<T>::up); }, a.dz + (long long)m0 * a.ldz + wt * BN, a.ldz, BM,
+                                                        cols, la0, la1, lb0, lb1, tid, wave, lane);
+    } else {
+        // Two f16 terms of dz times the weight's scale for dx.  |dz| <= (1 - p_target) |mask| in a row: brought to 2^13 against the largest
+        // weight scale, so that a row decided by one word keeps its small values.  Then three bf16 terms of dz for dW.  The values are
+        // scaled and unscaled by powers of two in place, and hidden from the optimizer between the passes: it would keep every
+        // conversion of one pass for the next and spill.
+        const float wtop = a.st.sums[2];
+        for (int i = tid; i < BM; i += P::NT) {
+            float u = 0.f;
+            if (m0 + i < count) {
+                const float miss = fmaxf(1.f - __builtin_amdgcn_exp2f(a.st.tz[m0 + i] - slse[i]), 0x1p-24f);
+                int e;
+                (void)frexpf(fminf(miss, 1.f) * wtop * fabsf(sw[i]), &e);
+                u = ldexpf(1.f, max(min(13 - e, 120), -120));
+                if (wt == 0) a.up[m0 + i] = 1.f / u;
+            }
+            srow[i] = u;
+        }
+        __syncthreads();
+        const auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 u4 = *reinterpret_cast<const f32x4*>(srow + wm * WM + 32 * i + 8 * q + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < P::NI; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = f(acc[i][j][4 * q + e], u4[e], wscale[j]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+            for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+                for (int j = 0; j < P::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
+        };
+        const auto put = [&](auto bits, unsigned short* out, long long ld) __attribute__((always_inline)) {
+            store_tile<BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, bits, out, ld, BM, cols, la0, la1, lb0, lb1, tid, wave, lane);
+            __syncthreads();
+        };
+        unsigned short* f16 = a.dz + (long long)m0 * 2 * a.ldz + wt * BN;
+        unsigned short* b16 = a.dzb + (long long)m0 * 3 * a.ldz + wt * BN;
+        const auto bf = [](float v) { return to_bits<__bf16>(v); };
+        const auto rest = [](float v, float, float) { return v - (float)(__bf16)v; };
+        each([](float v, float u, float w) { return v * (u * w); });
+        put([](float v) { return to_bits<_Float16>(v); }, f16, 2ll * a.ldz);
+        each([](float v, float, float) { return v; });
+        put([](float v) { return to_bits<_Float16>(v - (float)(_Float16)v); }, f16 + a.ldz, 2ll * a.ldz);
+        each([](float v, float u, float w) { return u == 0.f ? 0.f : v * (1.f / (u * w)); });
+        put(bf, b16, 3ll * a.ldz);
+        each(rest);
+        put(bf, b16 + a.ldz, 3ll * a.ldz);
+        each(rest);
+        put(bf, b16 + 2 * a.ldz, 3ll * a.ldz);
+    }
 }
 
 // factor that turns sums of stored dz into gradients: dloss / denom * max |mask| / 2^s (no rows: everything is zero)
@@ -481,7 +674,10 @@ __device__ __forceinline__ float grad_factor(const LossArgs& a, float up) {
 // dW = dz^T x of one piece: lanes = features, registers = words
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dw_kernel(const LossArgs a) {
-    typedef TileProduct<T, BM, BN, WM, WN, true, true> P;
+    // (f32: six products of the exact bf16 terms -- a rare word's whole column of dz is tiny, no row scale serves it)
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NP = F32 ? 3 : 1;
+    typedef TileProduct<std::conditional_t<F32, __bf16, T>, BM, BN, WM, WN, true, true, F32 ? 6 : 1> P;
     LL_LDS(BM, BN);
     const int count = a.st.count[0], tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nm = (a.vp + BM - 1) / BM, nn = (a.d.D + BN - 1) / BN, total = nm * nn * a.splits;
@@ -491,17 +687,25 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dw_kernel(const
     const int kt0 = min(kts, split * per), kt1 = min(kts, kt0 + per);
     typename P::A oa;
     typename P::B ob;
-    oa.init_cols(a.dz, a.ldz, m0, a.ldz, wave, lane);
-    ob.init_cols(a.xc, a.d.D, n0, a.d.D, wave, lane);
+    oa.init_cols(F32 ? a.dzb : a.dz, (long long)NP * a.ldz, m0, a.ldz, wave, lane);
+    ob.init_cols(F32 ? a.xb : a.xc, (long long)NP * a.d.D, n0, a.d.D, wave, lane);
+    oa.plane = 2ll * a.ldz;
+    ob.plane = 2ll * a.d.D;
     f32x16 acc[P::MI][P::NI];
-    P::run(acc, oa, ob, kt0, kt1, kts * BK, la0, la1, lb0, lb1, wave, lane);
-    if (a.splits == 1) {
-        store_tile<T, BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, grad_factor(a, DzScale<T>::up), (T*)a.d.dweight + (long long)(a.v0 + m0) * a.d.D + n0, a.d.D, a.vp - m0,
-                                                           a.d.D - n0, la0, la1, lb0, lb1, tid, wave, lane);
-        return;
+    P::run(acc, oa, ob, kt0, kt1, kts * BK, LL_BUFFERS, wave, lane);
+    if constexpr (!F32) {
+        if (a.splits == 1) {
+            const float f = grad_factor(a, DzScale<T>::up);
+            store_tile<BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, [&](float v) { return to_bits<T>(v * f); },
+                                                            (unsigned short*)a.d.dweight + (long long)(a.v0 + m0) * a.d.D + n0, a.d.D, a.vp - m0, a.d.D - n0, la0, la1, lb0,
+                                                            lb1, tid, wave, lane);
+            return;
+        }
     }
     const int wm = wave / P::NWN, wn = wave % P::NWN, g = lane >> 5;
-    float* out = a.pdw + (long long)split * a.ldz * a.d.D;
+    const bool direct = F32 && a.splits == 1;
+    const float f = direct ? grad_factor(a, 1.f) : 1.f;
+    float* out = direct ? (float*)a.d.dweight + (long long)a.v0 * a.d.D : a.pdw + (long long)split * a.ldz * a.d.D;
 #pragma unroll
     for (int i = 0; i < P::MI; ++i)
 #pragma unroll
@@ -509,7 +713,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dw_kernel(const
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int m = m0 + wm * WM + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3), n = n0 + wn * WN + 32 * j + (lane & 31);
-                if (m < a.vp && n < a.d.D) out[(long long)m * a.d.D + n] = acc[i][j][e];
+                if (m < a.vp && n < a.d.D) out[(long long)m * a.d.D + n] = acc[i][j][e] * f;
             }
 }
 template <typename T> __global__ __launch_bounds__(256) void ll_dw_sum_kernel(const LossArgs a) {
@@ -526,21 +730,25 @@ template <typename T> __global__ __launch_bounds__(256) void ll_dw_sum_kernel(co
 // dx partials of one piece: lanes = features, registers = rows; the words of the piece are cut over `splits` workgroups
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dx_kernel(const LossArgs a) {
-    typedef TileProduct<T, BM, BN, WM, WN, false, true> P;
+    typedef TileProduct<typename Term<T>::type, BM, BN, WM, WN, false, true, Term<T>::pairs> P;
+    constexpr int NP = Term<T>::planes;
     LL_LDS(BM, BN);
     const int count = a.st.count[0], tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int nm = (count + BM - 1) / BM, nn = (a.d.D + BN - 1) / BN, total = nm * nn * a.splits;
+    const int nm = (count + BM - 1) / BM, nn = (a.d.D + BN - 1) / BN, splits = ll_splits(nm * nn, a.first_vp / BK, a.splits), total = nm * nn * splits;
+    if (blockIdx.x == 0 && tid == 0) a.dx_shares[0] = splits;
     if ((int)blockIdx.x >= total) return;
     const int x = blockIdx.x & 7, q = total >> 3, r = total & 7, id = x * q + min(x, r) + (blockIdx.x >> 3);
     const int split = id / (nm * nn), mt = id % (nm * nn) / nn, ntile = id % nn;
-    const int m0 = mt * BM, n0 = ntile * BN, kts = (a.vp + BK - 1) / BK, per = (kts + a.splits - 1) / a.splits;
+    const int m0 = mt * BM, n0 = ntile * BN, kts = (a.vp + BK - 1) / BK, per = (kts + splits - 1) / splits;
     const int kt0 = min(kts, split * per), kt1 = min(kts, kt0 + per);
     typename P::A oa;
     typename P::B ob;
-    oa.init_rows([&](int rr) { return (const char*)(a.dz + (long long)(m0 + rr) * a.ldz); }, wave, lane);
-    ob.init_cols((const unsigned short*)a.d.weight + (long long)a.v0 * a.d.D, a.d.D, n0, a.d.D, wave, lane);
+    oa.init_rows([&](int rr) { return (const char*)(a.dz + (long long)(m0 + rr) * NP * a.ldz); }, wave, lane);
+    ob.init_cols(a.wp + (long long)a.v0 * NP * a.d.D, (long long)NP * a.d.D, n0, a.d.D, wave, lane);
+    oa.plane = 2ll * a.ldz;
+    ob.plane = 2ll * a.d.D;
     f32x16 acc[P::MI][P::NI];
-    P::run(acc, oa, ob, kt0, kt1, a.vp, la0, la1, lb0, lb1, wave, lane);
+    P::run(acc, oa, ob, kt0, kt1, a.vp, LL_BUFFERS, wave, lane);
     const int wm = wave / P::NWN, wn = wave % P::NWN, g = lane >> 5;
     float* out = a.pdx + (long long)split * a.nr * a.d.D;
 #pragma unroll
@@ -558,16 +766,16 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dx_kernel(const
 }
 // dx rows in place: the sum of the partials, or zeros for a row that does not count
 template <typename T> __global__ __launch_bounds__(256) void ll_dx_sum_kernel(const LossArgs a) {
-    const int vec = a.d.D / 8;
+    const int vec = a.d.D / 8, splits = a.dx_shares[0];
     const long long n = (long long)a.d.B * a.d.T * vec;
     const float f0 = grad_factor(a, DzScale<T>::up);
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += 256ll * gridDim.x) {
         const long long row = i / vec;
         const int c = (int)(i % vec) * 8, p = a.st.pos[row];
-        const float f = p >= 0 ? f0 : 0.f;
+        const float f = p >= 0 ? (sizeof(T) == 4 ? f0 * a.up[p] : f0) : 0.f;
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (p >= 0)
-            for (int k = 0; k < a.splits; ++k) {
+            for (int k = 0; k < splits; ++k) {
                 const f32x4* src = reinterpret_cast<const f32x4*>(a.pdx + ((long long)k * a.nr + p) * a.d.D + c);
                 const f32x4 u = src[0], w = src[1];
 #pragma unroll
@@ -576,21 +784,96 @@ template <typename T> __global__ __launch_bounds__(256) void ll_dx_sum_kernel(co
                     s[4 + e] += w[e];
                 }
             }
-        u32x4 o;
+        if constexpr (sizeof(T) == 4) {
+            float* o = (float*)a.d.dx + row * a.d.D + c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = to_bits<T>(s[2 * e] * f) | (uint32_t)to_bits<T>(s[2 * e + 1] * f) << 16;
-        *reinterpret_cast<u32x4*>((T*)a.d.dx + row * a.d.D + c) = o;
+            for (int e = 0; e < 8; ++e) o[e] = s[e] * f;
+        } else {
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = to_bits<T>(s[2 * e] * f) | (uint32_t)to_bits<T>(s[2 * e + 1] * f) << 16;
+            *reinterpret_cast<u32x4*>((T*)a.d.dx + row * a.d.D + c) = o;
+        }
     }
 }
-template <typename T> __global__ __launch_bounds__(256) void ll_db_kernel(const LossArgs a, int BM) {
-    const int v = blockIdx.x * 256 + threadIdx.x, tiles = (a.st.count[0] + BM - 1) / BM;
-    if (v >= a.vp) return;
+// bias gradient: 64 words x 16 strands of row tiles a workgroup
+template <typename T> __global__ __launch_bounds__(1024) void ll_db_kernel(const LossArgs a, int BM) {
+    __shared__ float part[16][64];
+    const int v = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6, tiles = (a.st.count[0] + BM - 1) / BM;
     float s = 0.f;
-    for (int t = 0; t < tiles; ++t) s += a.pdb[(long long)t * a.ldz + v];
+    if (v < a.vp)
+        for (int t = k; t < tiles; t += 16) s += a.pdb[(long long)t * a.ldz + v];
+    part[k][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (k || v >= a.vp) return;
+    for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x & 63];
     ((T*)a.d.dbias)[a.v0 + v] = (T)(s * grad_factor(a, 1.f));
 }
 
-// ---- f32: the products are ekaid_gemm_f32, these are the passes around them
+// ---- f32 operands as 16-bit terms.  One wave a row: the compact rows of x (zeros behind them to a multiple of 256), then the rows of the
+// weight.  f16: the row times a power of two that brings its largest magnitude to [2^13, 2^14), in two terms; its inverse in sx / sw.
+__global__ __launch_bounds__(256) void ll_terms_kernel(const LossArgs a, unsigned short* xp, unsigned short* xb, unsigned short* wp, float* sx, float* sw, int nx) {
+    const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), D = a.d.D, count = a.st.count[0], rows = (count + 255) & ~255;
+    const bool of_x = r < nx;
+    const int v = r - nx;
+    if (of_x ? r >= rows : v >= a.d.V) return;
+    const bool zero = of_x && r >= count;
+    const float* src = of_x ? (const float*)a.d.x + (zero ? 0 : a.st.idx[r]) * a.d.ldx : (const float*)a.d.weight + (long long)v * D;
+    float mx = 0.f;
+    if (!zero)
+        for (int c = 4 * lane; c < D; c += 256) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(src + c);
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        }
+    mx = wave_max(mx);
+    int e = 0;
+    if (mx > 0.f && mx < __builtin_inff()) (void)frexpf(mx, &e);
+    e = max(min(14 - e, 120), -100);
+    const float s = ldexpf(1.f, e);
+    if (lane == 0) (of_x ? sx[r] : sw[v]) = ldexpf(1.f, -e);
+    unsigned short* out = of_x ? xp + (long long)r * 2 * D : wp + (long long)v * 2 * D;
+    for (int c = 8 * lane; c < D; c += 512) {
+        u32x4 h, l, b0, b1, b2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t t[5] = {0, 0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const float x = zero ? 0.f : src[c + 2 * k + w], y = x * s, f = (float)(_Float16)y;
+                const float q = x - (float)(__bf16)x;
+                t[0] |= (uint32_t)to_bits<_Float16>(y) << (16 * w);
+                t[1] |= (uint32_t)to_bits<_Float16>(y - f) << (16 * w);
+                t[2] |= (uint32_t)to_bits<__bf16>(x) << (16 * w);
+                t[3] |= (uint32_t)to_bits<__bf16>(q) << (16 * w);
+                t[4] |= (uint32_t)to_bits<__bf16>(q - (float)(__bf16)q) << (16 * w);
+            }
+            h[k] = t[0]; l[k] = t[1]; b0[k] = t[2]; b1[k] = t[3]; b2[k] = t[4];
+        }
+        *reinterpret_cast<u32x4*>(out + c) = h;
+        *reinterpret_cast<u32x4*>(out + D + c) = l;
+        if (of_x && xb) {
+            unsigned short* o = xb + (long long)r * 3 * D + c;
+            *reinterpret_cast<u32x4*>(o) = b0;
+            *reinterpret_cast<u32x4*>(o + D) = b1;
+            *reinterpret_cast<u32x4*>(o + 2 * D) = b2;
+        }
+    }
+}
+// sums[2] = largest scale of the weight's rows
+__global__ __launch_bounds__(1024) void ll_scale_top_kernel(const float* sw, int V, float* out) {
+    __shared__ float part[16];
+    float m = 0.f;
+    for (int v = threadIdx.x; v < V; v += 1024) m = fmaxf(m, sw[v]);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) m = fmaxf(m, part[w]);
+        out[0] = m;
+    }
+}
+
+// ---- f32 in the other arithmetics: the products are ekaid_gemm_f32, these are the passes around them
 __global__ __launch_bounds__(256) void ll_fill_kernel(float* p, long long n, float v) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += 256ll * gridDim.x) p[i] = v;
 }
@@ -600,7 +883,11 @@ __global__ __launch_bounds__(256) void ll32_stats_kernel(const ekaid_linear_loss
     const int lane = threadIdx.x & 63;
     if (row >= n) return;
     const long long b = row / d.T, t = row % d.T;
-    if (d.mask[b * d.ld_mask + t] == 0.f) return;
+    const float mask = d.mask[b * d.ld_mask + t];
+    if (mask == 0.f) {
+        if (lane == 0 && last) st.nll[row] = 0.f;
+        return;
+    }
     const float* zp = z + row * ldz;
     const float* bias = (const float*)d.bias;
     float m = NEG_INF, l = 0.f;
@@ -619,8 +906,11 @@ __global__ __launch_bounds__(256) void ll32_stats_kernel(const ekaid_linear_loss
     const long long tg = d.target[b * d.ld_target + t];
     if (first) st.tz[row] = __builtin_nanf("");
     if (tg >= v0 && tg < v0 + vp) st.tz[row] = (zp[tg - v0] + (bias ? bias[tg] : 0.f)) * LOG2E;
-    if (last) st.lse[row] = M + __builtin_amdgcn_logf(s);
-    else {
+    if (last) {
+        const float lse = M + __builtin_amdgcn_logf(s);
+        st.lse[row] = lse;
+        st.nll[row] = (lse - st.tz[row]) * LN2 * mask;
+    } else {
         run[2 * row] = M;
         run[2 * row + 1] = s;
     }
@@ -642,15 +932,19 @@ __global__ __launch_bounds__(256) void ll32_dz_kernel(const ekaid_linear_loss_t 
         z[i] = g;
     }
 }
-__global__ __launch_bounds__(256) void ll32_clean_kernel(const ekaid_linear_loss_t d, float* xc) {
-    const long long n = (long long)d.B * d.T * d.D;
+// x with the rows that do not count zeroed; VEC floats at a time
+template <int VEC> __global__ __launch_bounds__(256) void ll32_clean_kernel(const ekaid_linear_loss_t d, float* xc) {
+    const int per = d.D / VEC;
+    const long long n = (long long)d.B * d.T * per;
     const float* x = (const float*)d.x;
+    typedef float vec __attribute__((ext_vector_type(VEC)));
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += 256ll * gridDim.x) {
-        const long long row = i / d.D;
-        xc[i] = d.mask[(row / d.T) * d.ld_mask + row % d.T] == 0.f ? 0.f : x[row * d.ldx + i % d.D];
+        const int row = (int)(i / per), c = (int)(i % per) * VEC;
+        vec v = *reinterpret_cast<const vec*>(x + row * d.ldx + c);
+        if (d.mask[(row / d.T) * d.ld_mask + row % d.T] == 0.f) v = 0.f;
+        *reinterpret_cast<vec*>(xc + (long long)row * d.D + c) = v;
     }
 }
-
 // column sums (a bias gradient without the weight's product to ride on): 64 columns x 16 strands of rows a workgroup, fixed order
 __global__ __launch_bounds__(1024) void ll32_db_kernel(const float* z, long long n, int vp, int ldz, float* out) {
     __shared__ float part[16][64];
@@ -679,15 +973,18 @@ int ll_check(const ekaid_linear_loss_t* a, const char* who) {
     if (((uintptr_t)a->x | (uintptr_t)a->weight | (uintptr_t)a->dx | (uintptr_t)a->dweight) & (al - 1)) { set_error("%s: operands must be %d-byte aligned", who, al); return EKAID_ERR_ARG; }
     return EKAID_OK;
 }
-constexpr size_t PIECE_BYTES = size_t(256) << 20;              // dz (or f32 logits) of one piece: what the 256 MB last-level cache can hold
+constexpr size_t PIECE_BYTES = size_t(512) << 20;              // dz (or f32 logits) of one piece
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 struct LossPlan {
+    int terms;                     // f32 as 16-bit terms through the tile kernels
     int big;                       // 256 x 256 tiles
     long long n, nr;
     int vp, pieces, ldz;           // words a piece
-    int sx, sw;                    // splits of dx, dW
+    int sx, sw;                    // splits of dx (at most), dW
+    int dx_grid;
     size_t part, dz, xc, pdb, pdx, pdw, total;        // byte offsets
+    size_t wp, xb, xscale, wscale, up, dzb;           // f32 terms
     // f32
     size_t z, run, clean, bnd, gws, gws_bytes;
     int bounds;
@@ -712,7 +1009,9 @@ LossPlan loss_plan(const ekaid_linear_loss_t* a, int backward) {
     p.n = (long long)a->B * a->T;
     p.nr = (p.n + 255) & ~255ll;
     size_t o = 0;
-    if (a->dtype == EKAID_F32) {
+    // (below 2^31 products of a matrix the few tiles are bound by latency, and ekaid_gemm_f32 with its splits is level or ahead)
+    p.terms = a->dtype == EKAID_F32 && a->arith == EKAID_GEMM_F16X2 && (double)p.n * a->V * a->D >= 2147483648.0 && a->D % 8 == 0 && a->ldx % 4 == 0 && !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
+    if (a->dtype == EKAID_F32 && !p.terms) {
         long long vp = (long long)(PIECE_BYTES / 4) / std::max(1ll, p.n);
         vp = std::max(256ll, vp & ~255ll);
         p.vp = (int)std::min<long long>(a->V, vp);
@@ -745,29 +1044,38 @@ LossPlan loss_plan(const ekaid_linear_loss_t* a, int backward) {
     }
     p.big = (p.nr / 256) * (long long)cdiv(a->V, 256) >= 128;
     const int bt = p.big ? 256 : 128;
+    if (p.terms) {
+        p.wp = o; o += up256((size_t)a->V * a->D * 4);
+        p.wscale = o; o += up256((size_t)a->V * 4);
+        p.xscale = o; o += up256((size_t)p.nr * 4);
+        p.xc = o; o += up256((size_t)p.nr * a->D * 4);
+        p.xb = o; o += backward ? up256((size_t)p.nr * a->D * 6) : 0;
+        p.up = o; o += backward ? up256((size_t)p.nr * 4) : 0;
+    }
     if (!backward) {
         p.part = o; o += up256((size_t)cdiv(a->V, bt) * p.nr * 8);
         p.total = o;
         return p;
     }
-    long long vp = (long long)(PIECE_BYTES / 2) / std::max(1ll, p.nr);
+    const int per = p.terms ? 10 : 2;      // bytes of dz a logit
+    long long vp = (long long)(PIECE_BYTES / per) / std::max(1ll, p.nr);
     vp = std::max(1024ll, vp & ~255ll);
     p.pieces = cdiv(a->V, std::min<long long>(a->V, vp));
     p.vp = (int)std::min<long long>(a->V, ((a->V + p.pieces - 1) / p.pieces + 255) & ~255);          // even pieces
     p.pieces = cdiv(a->V, p.vp);
-    p.ldz = (p.vp + 63) & ~63;
-    auto split = [](long long tiles, int ksteps) {
-        long long s = tiles >= 192 ? 1 : (256 + tiles - 1) / std::max(1ll, tiles);
-        return (int)std::max(1ll, std::min<long long>(s, ksteps / 8));
-    };
-    p.sx = split(p.nr / bt * cdiv(a->D, bt), p.vp / BK);
-    p.sw = split((long long)cdiv(p.vp, bt) * cdiv(a->D, bt), (int)(p.nr / BK));
-    p.dz = o; o += up256((size_t)p.nr * p.ldz * 2);
-    p.xc = o; o += up256((size_t)p.nr * a->D * 2);
+    p.ldz = ((p.vp + 63) & ~63) + 64;      // (rows a power of two apart would meet in the same memory channels)
+    const size_t dx_bytes = (size_t)p.nr * a->D * 4;
+    p.sx = (int)std::max<size_t>(1, std::min<size_t>(16, (size_t(1) << 29) / std::max<size_t>(1, dx_bytes)));
+    p.sw = ll_splits(cdiv(p.vp, bt) * cdiv(a->D, bt), (int)(p.nr / BK) * (p.terms ? 6 : 1), 32);
+    p.dz = o; o += up256((size_t)p.nr * p.ldz * (p.terms ? 4 : 2));
+    p.dzb = o; o += p.terms ? up256((size_t)p.nr * p.ldz * 6) : 0;
+    if (!p.terms) { p.xc = o; o += up256((size_t)p.nr * a->D * 2); }
     p.pdb = o; o += up256((size_t)(p.nr / bt) * p.ldz * 4);
     p.pdx = o; o += up256((size_t)p.sx * p.nr * a->D * 4);
     p.pdw = o; o += p.sw > 1 ? up256((size_t)p.sw * p.ldz * a->D * 4) : 0;
-    p.total = o;
+    p.total = o + 256;
+    const int nn = cdiv(a->D, bt);
+    for (int nm = 1; nm <= p.nr / bt; ++nm) p.dx_grid = std::max(p.dx_grid, nm * nn * ll_splits(nm * nn, p.vp / BK, p.sx));      // for any number of rows
     return p;
 }
 int blocks(long long n) { return (int)std::max(1ll, std::min<long long>((n + 255) / 256, 8192)); }
@@ -797,7 +1105,8 @@ int bwd32(const ekaid_linear_loss_t* a, const LossPlan& p, State st, char* ws, h
     float* xr = (float*)(ws + p.bnd);
     const long long n4 = (p.n + 3) & ~3ll, v4 = (a->V + 3) & ~3;
     float *wr = xr + n4, *xcol = wr + v4, *wcol = xcol + ((a->D + 3) & ~3), *zr = wcol + ((a->D + 3) & ~3), *zcol = zr + n4;
-    hipLaunchKernelGGL(ll32_clean_kernel, dim3(blocks(p.n * a->D)), dim3(256), 0, s, *a, xc);
+    if (a->D % 4 == 0 && a->ldx % 4 == 0 && !((uintptr_t)a->x & 15)) hipLaunchKernelGGL(ll32_clean_kernel<4>, dim3(blocks(p.n * (a->D / 4))), dim3(256), 0, s, *a, xc);
+    else hipLaunchKernelGGL(ll32_clean_kernel<1>, dim3(blocks(p.n * a->D)), dim3(256), 0, s, *a, xc);
     if (a->dbias) hipLaunchKernelGGL(ll_fill_kernel, dim3(blocks(a->V)), dim3(256), 0, s, (float*)a->dbias, (long long)a->V, 0.f);
     if (p.bounds) {
         hipLaunchKernelGGL(ll_fill_kernel, dim3(blocks(zr - xr)), dim3(256), 0, s, xr, (long long)(zr - xr), 0.f);
@@ -835,18 +1144,25 @@ int bwd32(const ekaid_linear_loss_t* a, const LossPlan& p, State st, char* ws, h
     return check_launch("linear_loss_bwd");
 }
 
+void launch_terms(const LossArgs& a, const LossPlan& p, hipStream_t s) {
+    hipLaunchKernelGGL(ll_terms_kernel, dim3(cdiv(p.nr + a.d.V, 4)), dim3(256), 0, s, a, (unsigned short*)a.xc, (unsigned short*)a.xb, (unsigned short*)a.wp, (float*)a.sx,
+                       (float*)a.sw, (int)p.nr);
+    if (a.xb) hipLaunchKernelGGL(ll_scale_top_kernel, dim3(1), dim3(1024), 0, s, a.sw, a.d.V, a.st.sums + 2);
+}
 template <typename T, int BT, int WM, int WN> int fwd16(LossArgs a, const LossPlan& p, hipStream_t s) {
     constexpr int NT = (BT / WM) * (BT / WN) * 64;
     const int tiles = cdiv(a.d.V, BT);
+    if constexpr (sizeof(T) == 4) launch_terms(a, p, s);
     hipLaunchKernelGGL((ll_stats_kernel<T, BT, BT, WM, WN>), dim3((int)(p.nr / BT) * tiles), dim3(NT), 0, s, a);
-    hipLaunchKernelGGL(ll_lse_kernel, dim3(cdiv(p.n, 64)), dim3(256), 0, s, a, tiles);
+    hipLaunchKernelGGL(ll_lse_kernel, dim3(cdiv(p.n, 64)), dim3(1024), 0, s, a, tiles);
     return check_launch("linear_loss_fwd");
 }
 template <typename T, int BT, int WM, int WN> int bwd16(LossArgs a, const LossPlan& p, hipStream_t s) {
     constexpr int NT = (BT / WM) * (BT / WN) * 64;
     const ekaid_linear_loss_t& d = a.d;
     const int rt = (int)(p.nr / BT), dt = cdiv(d.D, BT);
-    hipLaunchKernelGGL(ll_gather_kernel, dim3(blocks(p.nr * (d.D / 8))), dim3(256), 0, s, a, (unsigned short*)a.xc);
+    if constexpr (sizeof(T) == 4) launch_terms(a, p, s);
+    else hipLaunchKernelGGL(ll_gather_kernel, dim3(blocks(p.nr * (d.D / 8))), dim3(256), 0, s, a, (unsigned short*)a.xc);
     for (int k = 0; k < p.pieces; ++k) {
         a.v0 = k * p.vp;
         a.vp = std::min(p.vp, d.V - a.v0);
@@ -857,28 +1173,38 @@ template <typename T, int BT, int WM, int WN> int bwd16(LossArgs a, const LossPl
             hipLaunchKernelGGL((ll_dw_kernel<T, BT, BT, WM, WN>), dim3(cdiv(a.vp, BT) * dt * p.sw), dim3(NT), 0, s, a);
             if (p.sw > 1) hipLaunchKernelGGL(ll_dw_sum_kernel<T>, dim3(blocks((long long)a.vp * d.D)), dim3(256), 0, s, a);
         }
-        if (d.dbias) hipLaunchKernelGGL(ll_db_kernel<T>, dim3(cdiv(a.vp, 256)), dim3(256), 0, s, a, BT);
+        if (d.dbias) hipLaunchKernelGGL(ll_db_kernel<T>, dim3(cdiv(a.vp, 64)), dim3(1024), 0, s, a, BT);
         if (d.dx) {
             a.splits = p.sx;
-            hipLaunchKernelGGL((ll_dx_kernel<T, BT, BT, WM, WN>), dim3(rt * dt * p.sx), dim3(NT), 0, s, a);
+            hipLaunchKernelGGL((ll_dx_kernel<T, BT, BT, WM, WN>), dim3(p.dx_grid), dim3(NT), 0, s, a);
         }
     }
     a.splits = p.sx;
     if (d.dx) hipLaunchKernelGGL(ll_dx_sum_kernel<T>, dim3(blocks(p.n * (d.D / 8))), dim3(256), 0, s, a);
     return check_launch("linear_loss_bwd");
 }
-LossArgs loss_args(const ekaid_linear_loss_t* a, const LossPlan& p, char* ws) {
+LossArgs loss_args(const ekaid_linear_loss_t* a, const LossPlan& p, char* ws, bool backward) {
     LossArgs k = {};
     k.d = *a;
     k.st = state_of(a->state, p.n);
     k.nr = p.nr;
-    k.vp = p.vp;
+    k.vp = k.first_vp = p.vp;
     k.ldz = p.ldz;
     k.part = (float2*)(ws + p.part);
     k.dz = (unsigned short*)(ws + p.dz);
     k.xc = (const unsigned short*)(ws + p.xc);
+    k.wp = (const unsigned short*)a->weight;
+    if (p.terms) {
+        k.wp = (const unsigned short*)(ws + p.wp);
+        k.sx = (const float*)(ws + p.xscale);
+        k.sw = (const float*)(ws + p.wscale);
+        k.xb = backward ? (const unsigned short*)(ws + p.xb) : nullptr;
+        k.up = (float*)(ws + p.up);
+        k.dzb = (unsigned short*)(ws + p.dzb);
+    }
     k.pdb = (float*)(ws + p.pdb);
     k.pdx = (float*)(ws + p.pdx);
+    k.dx_shares = (int*)(ws + p.total - 256);
     k.pdw = (float*)(ws + p.pdw);
     return k;
 }
@@ -887,7 +1213,7 @@ LossArgs loss_args(const ekaid_linear_loss_t* a, const LossPlan& p, char* ws) {
 
 extern "C" size_t ekaid_linear_loss_state_bytes(const ekaid_linear_loss_t* a) {
     if (ekaid::ll_check(a, "linear_loss_state_bytes")) return 0;
-    return 256 + (size_t)a->B * a->T * 16;
+    return 256 + (size_t)a->B * a->T * 20;
 }
 extern "C" size_t ekaid_linear_loss_workspace_bytes(const ekaid_linear_loss_t* a, int backward) {
     if (ekaid::ll_check(a, "linear_loss_workspace_bytes")) return 0;
@@ -904,15 +1230,16 @@ extern "C" int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspa
     hipLaunchKernelGGL(ll_rows_kernel, dim3(1), dim3(1024), 0, s, a->mask, a->ld_mask, a->B, a->T, st);
     int rc = check_launch("linear_loss_fwd");
     if (rc == EKAID_OK && p.n) {
-        if (a->dtype == EKAID_F32) rc = fwd32(a, p, st, (char*)workspace, s);
+        if (a->dtype == EKAID_F32 && !p.terms) rc = fwd32(a, p, st, (char*)workspace, s);
         else {
-            const LossArgs k = loss_args(a, p, (char*)workspace);
-            if (a->dtype == EKAID_BF16) rc = p.big ? fwd16<__bf16, 256, 128, 64>(k, p, s) : fwd16<__bf16, 128, 64, 64>(k, p, s);
+            const LossArgs k = loss_args(a, p, (char*)workspace, false);
+            if (a->dtype == EKAID_F32) rc = p.big ? fwd16<float, 256, 128, 64>(k, p, s) : fwd16<float, 128, 64, 64>(k, p, s);
+            else if (a->dtype == EKAID_BF16) rc = p.big ? fwd16<__bf16, 256, 128, 64>(k, p, s) : fwd16<__bf16, 128, 64, 64>(k, p, s);
             else rc = p.big ? fwd16<_Float16, 256, 128, 64>(k, p, s) : fwd16<_Float16, 128, 64, 64>(k, p, s);
         }
     }
     if (rc) return rc;
-    hipLaunchKernelGGL(ll_loss_kernel, dim3(1), dim3(1024), 0, s, *a, st, a->dtype == EKAID_F32);
+    hipLaunchKernelGGL(ll_loss_kernel, dim3(1), dim3(1024), 0, s, *a, st, a->dtype == EKAID_F32 && !p.terms);
     return check_launch("linear_loss_fwd");
 }
 extern "C" int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -923,8 +1250,9 @@ extern "C" int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspa
     if (!a->dloss || !a->state || !a->x || !a->weight || !a->target || !a->mask) { set_error("linear_loss_bwd: null operand"); return EKAID_ERR_ARG; }
     if (workspace_bytes < p.total || !workspace) { set_error("linear_loss_bwd: workspace of %zu bytes needed", p.total); return EKAID_ERR_ARG; }
     hipStream_t s = (hipStream_t)stream;
-    if (a->dtype == EKAID_F32) return bwd32(a, p, state_of(a->state, p.n), (char*)workspace, s);
-    const LossArgs k = loss_args(a, p, (char*)workspace);
+    if (a->dtype == EKAID_F32 && !p.terms) return bwd32(a, p, state_of(a->state, p.n), (char*)workspace, s);
+    const LossArgs k = loss_args(a, p, (char*)workspace, true);
+    if (a->dtype == EKAID_F32) return p.big ? bwd16<float, 256, 128, 64>(k, p, s) : bwd16<float, 128, 64, 64>(k, p, s);
     if (a->dtype == EKAID_BF16) return p.big ? bwd16<__bf16, 256, 128, 64>(k, p, s) : bwd16<__bf16, 128, 64, 64>(k, p, s);
     return p.big ? bwd16<_Float16, 256, 128, 64>(k, p, s) : bwd16<_Float16, 128, 64, 64>(k, p, s);
 }

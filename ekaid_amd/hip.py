@@ -108,7 +108,7 @@ class Attn(Structure):
 
 class LinearLoss(Structure):
     """ekaid_linear_loss_t."""
-    _fields_ = ([('x', c_void_p), ('weight', c_void_p), ('bias', c_void_p)] + [(n, c_int) for n in ('dtype', 'B', 'T', 'D', 'V')] +
+    _fields_ = ([('x', c_void_p), ('weight', c_void_p), ('bias', c_void_p)] + [(n, c_int) for n in ('dtype', 'B', 'T', 'D', 'V', 'arith')] +
                 [('ldx', c_longlong), ('target', c_void_p), ('ld_target', c_longlong), ('mask', c_void_p), ('ld_mask', c_longlong)] +
                 [(n, c_void_p) for n in ('denom', 'loss', 'state', 'dloss', 'dx', 'dweight', 'dbias')])
 

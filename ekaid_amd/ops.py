@@ -1893,15 +1893,16 @@ class LinearLossFn(Function):
     def forward(ctx, x, weight, bias, target, mask, denom):
         shape = x.shape
         x2, ld = _rows2d(x)
-        if x2.dtype != torch.float32 and x2.numel() and (ld % 8 or x2.data_ptr() % 16):
+        if x2.numel() and (ld * x2.element_size() % 16 or x2.data_ptr() % 16):          # whole 16-byte vectors, else a copy
             x2, ld = x2.clone(memory_format=torch.contiguous_format), shape[2]
         weight, bias = _c(weight), (None if bias is None else _c(bias))
-        if weight.data_ptr() % 16 and weight.dtype != torch.float32:
+        if weight.data_ptr() % 16:
             weight = weight.clone()
         loss = torch.empty((), device=x.device, dtype=torch.float32)
         L = hip.lib()
         with _on_device(x):
-            d = LinearLossFn._desc(x2, ld, shape, weight, bias, target, mask, denom)
+            ctx.arith = get_gemm_mode()
+            d = LinearLossFn._desc(x2, ld, shape, weight, bias, target, mask, denom, ctx.arith)
             state = _scratch(L.ekaid_linear_loss_state_bytes(ctypes.byref(d)), x.device)
             nb = L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 0)
             ws = _scratch(nb, x.device)
@@ -1912,10 +1913,11 @@ class LinearLossFn(Function):
         return loss
 
     @staticmethod
-    def _desc(x2, ld, shape, weight, bias, target, mask, denom):
+    def _desc(x2, ld, shape, weight, bias, target, mask, denom, arith):
         d = hip.LinearLoss()
         d.x, d.weight, d.bias, d.dtype = x2.data_ptr(), weight.data_ptr(), ptr(bias), _DTYPE_CODE[x2.dtype]
         d.B, d.T, d.D, d.V, d.ldx = shape[0], shape[1], shape[2], weight.shape[0], max(ld, shape[2])
+        d.arith = arith
         d.target, d.ld_target, d.mask, d.ld_mask = target.data_ptr(), target.stride(0), mask.data_ptr(), mask.stride(0)
         d.denom = ptr(denom)
         return d
@@ -1934,7 +1936,7 @@ class LinearLossFn(Function):
         dloss = _c(dloss)
         L = hip.lib()
         with _on_device(x2):
-            d = LinearLossFn._desc(x2, ctx.ld, ctx.shape, weight, bias, target, mask, denom)
+            d = LinearLossFn._desc(x2, ctx.ld, ctx.shape, weight, bias, target, mask, denom, ctx.arith)
             d.state, d.dloss, d.dx, d.dweight, d.dbias = state.data_ptr(), dloss.data_ptr(), ptr(dx), ptr(dw), ptr(db)
             nb = L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 1)
             ws = _scratch(nb, x2.device)

@@ -735,8 +735,9 @@ int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_byte
  * nothing whatever x and target hold there (16-bit types leave them out of the products as well); a target outside [0, V) in a row that
  * counts makes the loss NaN.  All-zero mask: loss 0/0, gradients 0.
  * state (ekaid_linear_loss_state_bytes) is written by fwd and read by bwd.  dloss: device scalar.  dx [B T][D], dweight [V][D],
- * dbias [V] contiguous, any may be NULL.  f32 products run as ekaid_gemm_f32 in the selected arithmetic; 16-bit products accumulate in
- * f32, logit gradients are rounded to the type (scaled by an exact power of two) where they enter a product.  No float atomics.
+ * dbias [V] contiguous, any may be NULL.  f32 products run in the arithmetic `arith`: two f16 terms with row scales for z and dx and the
+ * exact three bf16 terms for dweight (EKAID_GEMM_F16X2; D % 8 == 0 and 16-byte aligned x, weight), else as ekaid_gemm_f32; 16-bit
+ * products accumulate in f32, logit gradients are rounded to the type (scaled by an exact power of two) where they enter a product.  No float atomics.
  * ref: DynamicSpeaker.logit + log_softmax (dynamic_speaker_change_pos.py:163,238) + LanguageModelCriterion (utils/utils.py:204-216).
  * ------------------------------------------------------------------------------------------ */
 typedef struct ekaid_linear_loss {
@@ -745,6 +746,7 @@ typedef struct ekaid_linear_loss {
     const void* bias;
     int dtype;
     int B, T, D, V;
+    int arith;              /* f32: EKAID_GEMM_* of its products; bwd takes the value fwd was given */
     long long ldx;
     const int64_t* target;
     long long ld_target;

@@ -113,7 +113,7 @@ def test_f32_arithmetics_and_odd_widths(mode):
     old = ops.get_gemm_mode()
     ops.set_gemm_mode(dict(f32=ops.GEMM_F32_MFMA, bf16x3=ops.GEMM_BF16_SPLIT, f16x2=ops.GEMM_F16X2)[mode])
     try:
-        for shape in ((2, 21, 37, 203), (8, 256, 512, 6001)):
+        for shape in ((2, 21, 37, 203), (8, 256, 512, 6001), (8, 256, 516, 6001)):
             t = make(F32, *shape)
             compare(run(t), reference(t), str(shape))
     finally:
@@ -121,9 +121,27 @@ def test_f32_arithmetics_and_odd_widths(mode):
 
 
 @gpu
-@pytest.mark.parametrize('dtype', [F32, BF16], ids=['f32', 'bf16'])
-def test_vocabulary_in_several_pieces(dtype):
-    t = make(dtype, 4, 4100, 16, 9001 if dtype == BF16 else 8300)
+@pytest.mark.parametrize('dtype,V,mode', [(F32, 8300, None), (F32, 8300, 1), (BF16, 9001, None), (BF16, 17001, None)], ids=['f32', 'f32-bf16x3', 'bf16', 'bf16-2'])
+def test_vocabulary_in_several_pieces(dtype, V, mode):
+    from ekaid_amd import ops
+    old = ops.get_gemm_mode()
+    ops.set_gemm_mode(old if mode is None else mode)
+    try:
+        t = make(dtype, 4, 4100, 16, V)
+        compare(run(t), reference(t))
+    finally:
+        ops.set_gemm_mode(old)
+
+
+@gpu
+@pytest.mark.parametrize('xs', [1.0, 25.0])
+def test_f32_terms_of_uneven_magnitudes(xs):
+    """Rows and words whose magnitudes differ by powers of ten, rows decided by one word: every output element within its own bound."""
+    t = make(F32, 6, 200, 256, 8111, xs=xs)
+    g = torch.Generator().manual_seed(12)
+    t['x'] = t['x'] * (10.0 ** torch.randint(-4, 1, (6, 200, 1), generator=g)).to(DEV)
+    t['weight'] = t['weight'] * (10.0 ** torch.randint(-3, 1, (8111, 1), generator=g)).to(DEV)
+    t['weight'][5] = 0
     compare(run(t), reference(t))
 
 
