@@ -43,7 +43,11 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const RowWork& w, 
     for (int q = 0; q < DH / G * nq; ++q) {
         const int col = 4 * ng * q + 4 * g;
         const auto& t = o[q / nq];
-        if (col < a.d.dh) store4<T>(p + col, t[4 * (q % nq)] * inv, t[4 * (q % nq) + 1] * inv, t[4 * (q % nq) + 2] * inv, t[4 * (q % nq) + 3] * inv);
+        if (col < a.d.dh) {
+            const float x0 = t[4 * (q % nq)] * inv, x1 = t[4 * (q % nq) + 1] * inv, x2 = t[4 * (q % nq) + 2] * inv, x3 = t[4 * (q % nq) + 3] * inv;
+            store4<T>(p + col, x0, x1, x2, x3);
+            if (sizeof(T) == 2 && a.d.out32) store4<float>(a.d.out32 + (p - reinterpret_cast<T*>(a.d.out)) + col, x0, x1, x2, x3);
+        }
     }
     if (g == 0 && a.d.lse) a.d.lse[row] = l == 0.f ? POS_INF : m + __builtin_amdgcn_logf(l);
 }
@@ -231,7 +235,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_f
 #pragma unroll
         for (int q = 1; q < NW; ++q) v += *reinterpret_cast<const f32x4*>(join + (q * rows + rr) * DH + (c ^ (rr << 2)));
         if (a.splits > 1) *reinterpret_cast<f32x4*>(a.po + (w.split * total + ((long long)w.b * d.H + rh) * d.Lq + ri) * d.dh + c) = v;
-        else store4<T>(reinterpret_cast<T*>(d.out) + ((long long)w.b * d.Lq + ri) * d.H * d.dh + (long long)rh * d.dh + c, v[0], v[1], v[2], v[3]);
+        else {
+            const long long at = ((long long)w.b * d.Lq + ri) * d.H * d.dh + (long long)rh * d.dh + c;
+            store4<T>(reinterpret_cast<T*>(d.out) + at, v[0], v[1], v[2], v[3]);
+            if (sizeof(T) == 2 && d.out32) store4<float>(d.out32 + at, v[0], v[1], v[2], v[3]);
+        }
     }
 }
 
@@ -351,7 +359,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] += f * v[e];
         }
-        store4<T>(out + c, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        acc *= inv;
+        store4<T>(out + c, acc[0], acc[1], acc[2], acc[3]);
+        if (sizeof(T) == 2 && d.out32) store4<float>(d.out32 + (out - reinterpret_cast<T*>(d.out)) + c, acc[0], acc[1], acc[2], acc[3]);
     }
     if (lane == 0 && d.lse) d.lse[row] = l == 0.f ? POS_INF : m + __builtin_amdgcn_logf(l);
 }

@@ -17,19 +17,20 @@ template <typename T> __device__ __forceinline__ float ds_scale(float norm2) {
     } else return 1.f;
 }
 
-// dq (and the bias table's partial sums): lane = query row.  Units of 32 keys of a tile: scores and dP of a unit, then its share of dq.
+// dq: lane = query row.  Units of 32 keys of a tile: scores and dP of a unit, then its share of dq.
+// With a bias table the kernel also sums every row's score gradients: with delta = sum_j P dP they would be zero, so what they are is the
+// error of <dout, out> against it (out was formed from probabilities rounded to the type).  Added to delta, it makes the score gradients of
+// dk / dv and the table's long sums exact to f32.
 template <typename T, int DH, int G, int NW, int KT, bool REL>
 __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 : 2) void attn_dq_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, U = KT < 32 ? KT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
     constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng, nv = 4 * nq;
     __shared__ __attribute__((aligned(16))) T k0[KT * DH], k1[KT * DH], v0[KT * DH], v1[KT * DH];
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G, width = REL ? 2 * (a.d.reach + BIAS_PAD) + 1 : 0;
     float* red = reinterpret_cast<float*>(smem);              // [NW] row-norm maxima
     float* bias = red + NW;                                   // padded table of the head
-    float* dsum = bias + (REL ? width + 2 * BIAS_PAD : 0);    // [NW][width]: this wave's sums of score gradients by distance
-    float* skew = dsum + NW * width + wave * G * (G + 1);     // [NW][G][G + 1]
-    unsigned char* kms = reinterpret_cast<unsigned char*>(dsum + NW * width + (REL ? NW * G * (G + 1) : 0));
+    unsigned char* kms = reinterpret_cast<unsigned char*>(bias + width);
     const RowWork w(a);
     const ekaid_attn_t& d = a.d;
     const int h = w.head0, row0 = (w.tile * NW + wave) * G;
@@ -37,11 +38,8 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     const int i = min(row0 + lane % G, d.Lq - 1), p0 = query_pos(d, w.b), pos = p0 + i, pmin = p0 + min(row0, d.Lq - 1), pmax = p0 + min(row0 + G, d.Lq) - 1;
     const int len = key_len(d, w.b), kend = d.causal ? max(0, min(len, p0 + min(d.Lq, (w.tile + 1) * NW * G))) : len;
     const int nt = (kend + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits, t0 = w.split * per, t1 = min(nt, t0 + per);
-    const int rel_lo = t0 * KT - p0 - min(d.Lq, (w.tile + 1) * NW * G) + 1, rel_hi = t1 * KT - p0 - w.tile * NW * G;      // distances this workgroup meets
     if constexpr (REL) {
-        fill_bias_range(d, bias, h, rel_lo, rel_hi, tid, NT);
-        for (int wv = 0; wv < NW; ++wv)
-            for (int x = max(rel_lo, -d.reach) + tid; x <= min(rel_hi, d.reach); x += NT) dsum[wv * width + x + d.reach] = 0.f;
+        fill_bias_range(d, bias, h, t0 * KT - p0 - min(d.Lq, (w.tile + 1) * NW * G) + 1, t1 * KT - p0 - w.tile * NW * G, tid, NT);
         __syncthreads();
     }
     MaskRing<KT> ring;
@@ -61,13 +59,22 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     for (int c = 0; c < NC; ++c) {
         qf[c] = row_frag_global<T, G>(qrow, c, d.dh, ok, lane);
         gf[c] = row_frag_global<T, G>(grow, c, d.dh, ok, lane);
-        const u32x4 y = row_frag_global<T, G>(yrow, c, d.dh, ok, lane);
+        if (sizeof(T) == 2 && d.out32) {
+            const int col = (c * ng + g) * Elem<T>::epl;
+            f32x4 y0 = {0.f, 0.f, 0.f, 0.f}, y1 = y0;
+            if (ok && col < d.dh) {
+                y0 = *reinterpret_cast<const f32x4*>(d.out32 + orow + col);
+                y1 = *reinterpret_cast<const f32x4*>(d.out32 + orow + col + 4);
+            }
 #pragma unroll
-        for (int e = 0; e < Elem<T>::epl; ++e) {
-            const float x = elem<T>(gf[c], e);
-            delta += x * elem<T>(y, e);
-            n2 += x * x;
+            for (int e = 0; e < 4; ++e) delta += elem<T>(gf[c], e) * y0[e] + elem<T>(gf[c], (4 + e) % Elem<T>::epl) * y1[e];
+        } else {
+            const u32x4 y = row_frag_global<T, G>(yrow, c, d.dh, ok, lane);
+#pragma unroll
+            for (int e = 0; e < Elem<T>::epl; ++e) delta += elem<T>(gf[c], e) * elem<T>(y, e);
         }
+#pragma unroll
+        for (int e = 0; e < Elem<T>::epl; ++e) n2 += elem<T>(gf[c], e) * elem<T>(gf[c], e);
     }
     if (t0 < t1) {
         ck.issue(k0, t0 * KT, len, d.dh, ring.tile(t0), wave);
@@ -77,7 +84,7 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     n2 = across_groups_sum<G>(n2);
     const long long srow = ((long long)w.b * d.H + h) * d.Lq + i;
     const float lse = ok ? d.lse[srow] : POS_INF;
-    if (ok && g == 0 && w.split == 0) a.delta[srow] = delta;
+    if (ok && g == 0 && w.split == 0 && (!REL || a.splits > 1)) a.delta[srow] = delta;
     const float rs = ds_scale<T>(n2);
     if constexpr (__is_same(T, _Float16)) {
         const float mx = wave_max(n2);
@@ -86,7 +93,7 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     typename Blk<G>::acc o[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
-    float far_back = 0.f, far_ahead = 0.f;
+    float rowsum = 0.f;
     const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
 
     auto unit = [&](int j0, const T* ks, const T* vs, int r0, const unsigned char* km) __attribute__((always_inline)) {
@@ -116,39 +123,10 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
 #pragma unroll
             for (int r = 0; r < nv; ++r) s[b][r] = __builtin_amdgcn_exp2f(s[b][r] * f.mult + shift) * (dp[b][r] - delta);
         if constexpr (REL) {
-            // sums over equal distance j - pos: a block that lies wholly beyond the reach goes to one bucket; otherwise the block is written
-            // to LDS and lane x adds up diagonal x (rows ascending: a fixed order), whose distance no other lane of the wave holds
-            const int prow = p0 + row0;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int jb = j0 + b * G;
-                if (jb + G - 1 - prow <= -d.reach || jb - (prow + G - 1) >= d.reach) {
-                    float x = 0.f;
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int r = 0; r < nv; ++r) x += s[b][r];
-                    if (jb - prow < 0) far_back += x; else far_ahead += x;
-                } else {
-                    wave_fence();
-#pragma unroll
-                    for (int q = 0; q < nq; ++q)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) skew[(lane % G) * (G + 1) + 4 * ng * q + 4 * g + e] = s[b][4 * q + e];
-                    wave_fence();
-                    if (lane < 2 * G - 1) {
-                        const int off = lane - (G - 1);
-                        float x = 0.f;
-#pragma unroll 8
-                        for (int r = 0; r < G; ++r) {
-                            const int c = r + off;
-                            x += (c >= 0 && c < G) ? skew[r * (G + 1) + c] : 0.f;
-                        }
-                        const int rel = jb - prow + off;
-                        if (rel <= -d.reach) far_back += x;
-                        else if (rel >= d.reach) far_ahead += x;
-                        else dsum[wave * width + rel + d.reach] += x;
-                    }
-                }
-            }
+                for (int r = 0; r < nv; ++r) rowsum += s[b][r];
         }
         if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
@@ -181,34 +159,10 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
         if (t + 1 < t1) tile(t + 1, k1, v1, k0, v0);
     }
     if constexpr (REL) {
-        __syncthreads();
-        // sums by distance, the waves' in order; then the distances of one bucket in ascending order by one thread
-        const int lo = max(rel_lo, 1 - d.reach), hi = min(rel_hi, d.reach - 1);
-        float* ds = dsum + d.reach;
-        for (int x = lo + tid; x <= hi; x += NT)
-            for (int wv = 1; wv < NW; ++wv) ds[x] += ds[wv * width + x];
-        far_back = wave_sum(far_back);
-        far_ahead = wave_sum(far_ahead);
-        if (lane == 0) {
-            skew[0] = far_back;
-            skew[1] = far_ahead;
-        }
-        __syncthreads();
-        const int side = d.n_border + 1, nb = side * (d.bidirectional ? 2 : 1);
-        float* part = a.ptab + ((long long)(w.b * d.H + h) * a.dq_parts + w.tile * a.splits + w.split) * nb;
-        const float* far = dsum + NW * width;
-        for (int c = tid; c < nb; c += NT) {
-            const bool ahead = d.bidirectional && c >= side;
-            const int k = c % side, near = k ? d.border[k - 1] : 0, beyond = k == d.n_border ? d.reach : d.border[k];       // distances near .. beyond - 1
-            float x = 0.f;
-            if (ahead) for (int r = max(max(near, 1), lo); r <= min(beyond - 1, hi); ++r) x += ds[r];
-            else for (int r = max(near, -hi); r <= min(beyond - 1, -lo); ++r) x += ds[-r];
-            if (!d.bidirectional && c == 0) for (int r = max(1, lo); r <= hi; ++r) x += ds[r];
-            for (int wv = 0; wv < NW; ++wv) {
-                if (k == d.n_border) x += far[wv * G * (G + 1) + (ahead ? 1 : 0)];
-                if (!d.bidirectional && c == 0) x += far[wv * G * (G + 1) + 1];
-            }
-            part[c] = x;
+        rowsum = across_groups_sum<G>(rowsum);
+        if (ok && g == 0) {
+            if (a.splits > 1) a.eps[(long long)w.split * d.B * d.H * d.Lq + srow] = rowsum;
+            else a.delta[srow] = delta + rowsum;
         }
     }
     if constexpr (__is_same(T, _Float16)) {
@@ -236,14 +190,18 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
 // dk, dv: lane = key; the rows of every head that shares it go by in tiles, in units of 32.  What a lane without a valid key computes stays in
 // that lane and is replaced by zero at the end.
 template <typename T, int DH, int G, int NW, int QT, bool REL>
-__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 16 && sizeof(T) == 2 ? 3 : 2) void attn_dkv_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 16 && sizeof(T) == 2 && !(REL && DH > 64) ? 3 : 2) void attn_dkv_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, U = QT < 32 ? QT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;
     constexpr int nq = Blk<G>::nq, ng = Blk<G>::ng;
     __shared__ __attribute__((aligned(16))) T q0s[QT * DH], q1s[QT * DH], g0s[QT * DH], g1s[QT * DH];
     __shared__ __attribute__((aligned(16))) float l0s[QT], l1s[QT], d0s[QT], d1s[QT];      // log2 denominators, deltas
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* bias = reinterpret_cast<float*>(smem);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane / G, width = REL ? 2 * a.d.reach + 1 : 0;
+    float* bias = reinterpret_cast<float*>(smem);             // padded table of the head
+    float* dsum = bias + (REL ? width + 2 * BIAS_PAD : 0);    // [NW][width]: this wave's sums of score gradients by distance
+    float* far = dsum + NW * width;                           // [NW][2]
+    constexpr int DIAG = U + G - 1, DP = U + 4;               // diagonals of a unit; places of a diagonal (one a row)
+    float* skew = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(far + 2 * NW) + 15) & ~(uintptr_t)15) + wave * DIAG * DP;      // [NW][DIAG][DP]
     const ekaid_attn_t& d = a.d;
     const int wi = die_order(blockIdx.x, gridDim.x), tl = wi % a.tiles, split = (wi / a.tiles) % a.splits, bk = wi / a.tiles / a.splits;
     const int b = bk % d.B, kvh = bk / d.B, group = d.H / d.KV;
@@ -289,6 +247,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
             if (wave == NW - 1) __builtin_amdgcn_global_load_lds((global_void)(a.delta + row), (lds_void)ds, 4, 0, 0);
         }
     };
+    float far_back = 0.f, far_ahead = 0.f;
     const uint64_t seed = d.drop_p > 0.f ? drop_seed_value(a.seed) : 0;
     // rows i0 .. i0 + U of head h, at tile row r0
     auto unit = [&](int h, int i0, int r0, const T* qs, const T* gs, const float* ls, const float* ds) __attribute__((always_inline)) {
@@ -362,6 +321,39 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
 #pragma unroll
                 for (int r = 0; r < 4 * nq; ++r) dp[x][r] *= s[x][r];
         }
+        if constexpr (REL) {
+            // sums over equal distance j - pos: a unit that lies wholly beyond the reach goes to one bucket; otherwise it is written to LDS by
+            // diagonals and lane x adds up diagonal x (rows ascending: a fixed order), whose distance no other lane of the wave holds.
+            // Places of a diagonal that the unit does not have stay zero from the start.
+            if (jw + G - 1 - pu <= -d.reach || jw - (pu + U - 1) >= d.reach) {
+                float z = 0.f;
+#pragma unroll
+                for (int x = 0; x < NB; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4 * nq; ++r) z += dp[x][r];
+                z = ok ? z : 0.f;
+                if (jw < pu) far_back += z; else far_ahead += z;
+            } else {
+                wave_fence();
+                float* at = skew + (lane % G + U - 1) * DP - (DP - 1) * 4 * g;        // (row r, key c) at diagonal c - r + U - 1, place r
+#pragma unroll
+                for (int q = 0; q < NB * nq; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) at[-(DP - 1) * (4 * ng * q + e)] = ok ? dp[q / nq][4 * (q % nq) + e] : 0.f;
+                wave_fence();
+                if (lane < DIAG) {
+                    const float* row = skew + lane * DP;
+                    f32x4 z4 = *reinterpret_cast<const f32x4*>(row);
+#pragma unroll
+                    for (int r = 4; r < U; r += 4) z4 += *reinterpret_cast<const f32x4*>(row + r);
+                    const float z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
+                    const int rel = jw - pu + lane - (U - 1);
+                    if (rel <= -d.reach) far_back += z;
+                    else if (rel >= d.reach) far_ahead += z;
+                    else dsum[wave * width + rel + d.reach] += z;
+                }
+            }
+        }
         if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
             for (int x = 0; x < NB; ++x)
@@ -381,28 +373,73 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
                                           else dv[mt] = mma<T, G>(x, pf[c], dv[mt]);
                                       });
     };
-    int bias_head = -1;
+    // a head's sums: the waves' in order, then the distances of one bucket in ascending order by one thread
+    const int rel_lo = j0 - p0 - qtiles * QT, rel_hi = j0 + NW * G - p0;      // distances this workgroup meets
+    const int side = d.n_border + 1, nbuckets = side * (d.bidirectional ? 2 : 1);
+    auto part_of = [&](int h) { return a.ptab + (((long long)b * d.H + h) * a.tiles * a.splits + tl * a.splits + split) * nbuckets; };
+    auto flush = [&](int h) __attribute__((always_inline)) {
+        const int lo = max(rel_lo, 1 - d.reach), hi = min(rel_hi, d.reach - 1);
+        float* ds = dsum + d.reach;
+        far_back = wave_sum(far_back);
+        far_ahead = wave_sum(far_ahead);
+        if (lane == 0) {
+            far[2 * wave] = far_back;
+            far[2 * wave + 1] = far_ahead;
+        }
+        far_back = far_ahead = 0.f;
+        __syncthreads();
+        for (int x = lo + tid; x <= hi; x += NT)
+            for (int wv = 1; wv < NW; ++wv) ds[x] += ds[wv * width + x];
+        __syncthreads();
+        float* part = part_of(h);
+        for (int c = tid; c < nbuckets; c += NT) {
+            const bool ahead = d.bidirectional && c >= side;
+            const int k = c % side, near = k ? d.border[k - 1] : 0, beyond = k == d.n_border ? d.reach : d.border[k];       // distances near .. beyond - 1
+            float x = 0.f;
+            if (ahead) for (int r = max(max(near, 1), lo); r <= min(beyond - 1, hi); ++r) x += ds[r];
+            else for (int r = max(near, -hi); r <= min(beyond - 1, -lo); ++r) x += ds[-r];
+            if (!d.bidirectional && c == 0) for (int r = max(1, lo); r <= hi; ++r) x += ds[r];
+            for (int wv = 0; wv < NW; ++wv) {
+                if (k == d.n_border) x += far[2 * wv + (ahead ? 1 : 0)];
+                if (!d.bidirectional && c == 0) x += far[2 * wv + 1];
+            }
+            part[c] = x;
+        }
+        __syncthreads();
+    };
+    int end = t0;                                             // items before it are copied ahead
     auto tile = [&](int t, const T* qs, const T* gs, const float* ls, const float* ds, T* qn, T* gn, float* ln, float* dn) __attribute__((always_inline)) {
         const int h = kvh * group + t / run, i0 = (first + t % run) * QT;
         settle();
-        if constexpr (REL) {
-            if (bias_head != h) {
-                fill_bias_range(d, bias, h, j0 - p0 - qtiles * QT, j0 + NW * G - p0, tid, NT);
-                bias_head = h;
-                __syncthreads();
-            }
-        }
-        if (t + 1 < t1) fetch(t + 1, qn, gn, ln, dn);
+        if (t + 1 < end) fetch(t + 1, qn, gn, ln, dn);
 #pragma unroll
         for (int u = 0; u < QT / U; ++u) {
             const int iu = i0 + u * U;
             if (live && iu < d.Lq && !(d.causal && jw > p0 + iu + U - 1)) unit(h, iu, u * U, qs, gs, ls, ds);
         }
     };
-    if (t0 < t1) fetch(t0, q0s, g0s, l0s, d0s);
-    for (int t = t0; t < t1; t += 2) {
-        tile(t, q0s, g0s, l0s, d0s, q1s, g1s, l1s, d1s);
-        if (t + 1 < t1) tile(t + 1, q1s, g1s, l1s, d1s, q0s, g0s, l0s, d0s);
+    if constexpr (REL) {
+        for (int x = lane; x < DIAG * DP; x += 64) skew[x] = 0.f;       // (this wave's own; the first unit is behind a barrier)
+    }
+    for (int seg = t0; seg < t1; seg = end) {                 // with a bias table head by head: the table and the sums are a head's
+        end = REL ? min(t1, (seg / run + 1) * run) : t1;
+        if constexpr (REL) {
+            fill_bias_range(d, bias, kvh * group + seg / run, rel_lo, rel_hi, tid, NT);
+            for (int wv = 0; wv < NW; ++wv)
+                for (int x = max(rel_lo, -d.reach) + tid; x <= min(rel_hi, d.reach); x += NT) dsum[wv * width + x + d.reach] = 0.f;
+            __syncthreads();
+        }
+        fetch(seg, q0s, g0s, l0s, d0s);
+        for (int t = seg; t < end; t += 2) {
+            tile(t, q0s, g0s, l0s, d0s, q1s, g1s, l1s, d1s);
+            if (t + 1 < end) tile(t + 1, q1s, g1s, l1s, d1s, q0s, g0s, l0s, d0s);
+        }
+        if constexpr (REL) flush(kvh * group + seg / run);
+    }
+    if constexpr (REL) {
+        for (int h = kvh * group; h < (kvh + 1) * group; ++h)        // heads this share has not met
+            if (t0 >= t1 || h < kvh * group + t0 / run || h > kvh * group + (t1 - 1) / run)
+                for (int c = tid; c < nbuckets; c += NT) part_of(h)[c] = 0.f;
     }
     if (j >= d.Lk) return;
     const float f = d.scale / rs;
@@ -437,12 +474,20 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, T* out
         store4<T>(out + x, s[0], s[1], s[2], s[3]);
     }
 }
-// dtable[c][h] = sum over samples and row blocks, one wave per entry, fixed order
+// delta += the shares of its correction, in order
+__global__ __launch_bounds__(256) void attn_delta_kernel(const float* eps, float* delta, long long n, int splits) {
+    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < n; x += 256ll * gridDim.x) {
+        float s = delta[x];
+        for (int k = 0; k < splits; ++k) s += eps[k * n + x];
+        delta[x] = s;
+    }
+}
+// dtable[c][h] = sum over samples and key blocks, one wave per entry, fixed order
 __global__ __launch_bounds__(64) void attn_table_kernel(const AttnArgs a, int nb) {
-    const int c = blockIdx.x % nb, h = blockIdx.x / nb, lane = threadIdx.x;
+    const int c = blockIdx.x % nb, h = blockIdx.x / nb, lane = threadIdx.x, parts = a.tiles * a.splits;
     float s = 0.f;
-    const long long n = (long long)a.d.B * a.dq_parts;
-    for (long long x = lane; x < n; x += 64) s += a.ptab[(((x / a.dq_parts) * a.d.H + h) * a.dq_parts + x % a.dq_parts) * nb + c];
+    const int n = a.d.B * parts;
+    for (int x = lane; x < n; x += 64) s += a.ptab[(((long long)(x / parts) * a.d.H + h) * parts + x % parts) * nb + c];
     s = wave_sum(s);
     if (lane) return;
     const long long o = (long long)c * a.d.H + h;
@@ -454,7 +499,7 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const AttnArgs a, int nb
 struct BwdPlan {
     int gq, nwq, tq, sq;        // dq: block edge, waves, row tiles, splits
     int gk, nwk, tk, sk;        // dk / dv
-    size_t delta, nrm, tab, po, pk, total;      // float offsets
+    size_t delta, nrm, eps, tab, po, pk, total;      // float offsets
 };
 static size_t align4(size_t n) { return (n + 3) & ~(size_t)3; }
 
@@ -482,7 +527,8 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
     size_t o = 0;
     p.delta = o; o += align4(rows);
     p.nrm = o; o += align4(bh * p.tq * p.sq);
-    p.tab = o; o += align4(bh * p.tq * p.sq * nb);
+    p.eps = o; o += a->table && p.sq > 1 ? align4(rows * p.sq) : 0;
+    p.tab = o; o += align4(bh * p.tk * p.sk * nb);
     p.po = o; o += p.sq > 1 ? p.sq * rows * a->dh : 0;
     p.pk = o; o += p.sk > 1 ? 2 * p.sk * (size_t)a->B * a->Lk * a->KV * a->dh : 0;
     p.total = o * sizeof(float);
@@ -491,9 +537,8 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
 size_t attn_bwd_workspace(const ekaid_attn_t* a) { return bwd_plan(a).total; }
 
 template <typename T, int DH, int G, int NW, bool REL> static int launch_dq(const AttnArgs& a, hipStream_t st) {
-    constexpr int KT = attn_kt((int)sizeof(T), DH, G) > 32 && REL ? 32 : attn_kt((int)sizeof(T), DH, G);      // (the sums by distance take LDS too)
-    size_t lds = 4 * NW + 4 * KT;
-    if (REL) lds += 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + 2 * BIAS_PAD + NW * G * (G + 1));
+    constexpr int KT = attn_kt((int)sizeof(T), DH, G);
+    const size_t lds = 4 * NW + 4 * KT + (REL ? 4 * (2 * (a.d.reach + BIAS_PAD) + 1) : 0);
     if (int rc = attn_lds_limit((const void*)attn_dq_kernel<T, DH, G, NW, KT, REL>, 96 * 1024)) return rc;
     hipLaunchKernelGGL((attn_dq_kernel<T, DH, G, NW, KT, REL>), dim3(a.d.B * a.d.H * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
     return check_launch("attn_dq");
@@ -507,7 +552,8 @@ template <typename T, int DH, bool REL> static int pick_dq(const AttnArgs& a, co
 }
 template <typename T, int DH, int G, int NW, bool REL> static int launch_dkv(const AttnArgs& a, hipStream_t st) {
     constexpr int QT = attn_kt((int)sizeof(T), DH, G);
-    const size_t lds = REL ? 4 * (2 * (a.d.reach + BIAS_PAD) + 1) : 0;
+    constexpr int U = QT < 32 ? QT : 32;
+    const size_t lds = REL ? 4 * ((size_t)(NW + 1) * (2 * a.d.reach + 1) + 2 * BIAS_PAD + 2 * NW + 4 + NW * (U + G - 1) * (U + 4)) : 0;
     if (int rc = attn_lds_limit((const void*)attn_dkv_kernel<T, DH, G, NW, QT, REL>, 92 * 1024)) return rc;
     hipLaunchKernelGGL((attn_dkv_kernel<T, DH, G, NW, QT, REL>), dim3(a.d.B * a.d.KV * a.tiles * a.splits), dim3(64 * NW), lds, st, a);
     return check_launch("attn_dkv");
@@ -536,19 +582,29 @@ template <typename T> static int run_bwd(AttnArgs a, const BwdPlan& p, hipStream
         rc = d.dh <= 64 ? pick_dq<T, 64, false>(a, p, st) : d.dh <= 128 ? pick_dq<T, 128, false>(a, p, st) : pick_dq<T, 256, false>(a, p, st);
     if (rc) return rc;
     if (p.sq > 1 && (rc = sum_parts<T>(a.po, d.dq, (long long)d.B * d.Lq * d.H * d.dh, p.sq, st))) return rc;
-    if (d.table) {
-        const int nb = (d.n_border + 1) * (d.bidirectional ? 2 : 1);
+    if (d.table && p.sq > 1) {
+        const long long n = (long long)d.B * d.H * d.Lq;
+        hipLaunchKernelGGL(attn_delta_kernel, dim3((int)std::min<long long>((n + 255) / 256, 4096)), dim3(256), 0, st, a.eps, a.delta, n, p.sq);
+        if ((rc = check_launch("attn_delta"))) return rc;
+    }
+    const int nb = (d.n_border + 1) * (d.bidirectional ? 2 : 1);
+    a.tiles = p.tk;                                           // (no keys: no key tiles, the table's sums are of nothing)
+    a.splits = p.sk;
+    if (d.table && d.Lk == 0) {
         hipLaunchKernelGGL(attn_table_kernel, dim3(nb * d.H), dim3(64), 0, st, a, nb);
-        if ((rc = check_launch("attn_table"))) return rc;
+        return check_launch("attn_table");
     }
     if (d.Lk == 0) return EKAID_OK;
-    a.tiles = p.tk;
-    a.splits = p.sk;
     if (d.table)
         rc = d.dh <= 64 ? pick_dkv<T, 64, true>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128, true>(a, p, st) : pick_dkv<T, 256, true>(a, p, st);
     else
         rc = d.dh <= 64 ? pick_dkv<T, 64, false>(a, p, st) : d.dh <= 128 ? pick_dkv<T, 128, false>(a, p, st) : pick_dkv<T, 256, false>(a, p, st);
-    if (rc || p.sk == 1) return rc;
+    if (rc) return rc;
+    if (d.table) {
+        hipLaunchKernelGGL(attn_table_kernel, dim3(nb * d.H), dim3(64), 0, st, a, nb);
+        if ((rc = check_launch("attn_table"))) return rc;
+    }
+    if (p.sk == 1) return EKAID_OK;
     const long long n = (long long)d.B * d.Lk * d.KV * d.dh;
     if ((rc = sum_parts<T>(a.pk, d.dk, n, p.sk, st))) return rc;
     return sum_parts<T>(a.pv, d.dv, n, p.sk, st);
@@ -563,7 +619,7 @@ extern "C" int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t wor
         set_error("attn_bwd: null operand");
         return EKAID_ERR_ARG;
     }
-    if (((uintptr_t)a->dout | (uintptr_t)a->out) & 15) { set_error("attn_bwd: operands must be 16-byte aligned"); return EKAID_ERR_ARG; }
+    if (((uintptr_t)a->dout | (uintptr_t)a->out | (uintptr_t)a->out32) & 15) { set_error("attn_bwd: operands must be 16-byte aligned"); return EKAID_ERR_ARG; }
     const BwdPlan p = bwd_plan(a);
     if (!workspace || workspace_bytes < p.total) { set_error("attn_bwd: workspace of %zu bytes needed", p.total); return EKAID_ERR_ARG; }
     AttnArgs k = {};
@@ -574,6 +630,7 @@ extern "C" int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t wor
     float* w = (float*)workspace;
     k.delta = w + p.delta;
     k.nrm = w + p.nrm;
+    k.eps = w + p.eps;
     k.ptab = w + p.tab;
     k.po = w + p.po;
     k.pk = w + p.pk;

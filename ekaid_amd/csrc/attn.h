@@ -40,7 +40,8 @@ struct AttnArgs {
     float* pml;                       // their (max, sum) pairs
     float* delta;                     // [B][H][Lq]
     float* nrm;                       // [B * H][dq_parts]
-    float* ptab;                      // [B * H][dq_parts][nb]
+    float* eps;                       // [splits][B][H][Lq] shares of delta's correction (split dq with a bias table)
+    float* ptab;                      // [B * H][key tiles * splits][nb]
     float* pk;                        // partial dk, dv
     float* pv;
 };

@@ -103,7 +103,7 @@ class Attn(Structure):
                  ('key_mask', c_void_p), ('mask_batch', c_longlong), ('table', c_void_p)] +
                 [(n, c_int) for n in ('table_dtype', 'bidirectional', 'n_border', 'reach')] +
                 [('border', c_int * 128), ('causal', c_int), ('drop_p', c_float), ('drop_seed', c_uint64)] +
-                [(n, c_void_p) for n in ('out', 'lse', 'dout', 'dq', 'dk', 'dv', 'dtable')])
+                [(n, c_void_p) for n in ('out', 'lse', 'out32', 'dout', 'dq', 'dk', 'dv', 'dtable')])
 
 
 class LinearLoss(Structure):

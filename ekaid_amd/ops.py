@@ -2315,28 +2315,29 @@ class AttentionFn(Function):
 
     @staticmethod
     def launch(q, k, v, table, cfg, need_lse):
-        """(out, lse or None, the operands as the kernels read them)"""
+        """(out, lse and the unrounded out or None, the operands as the kernels read them)"""
         q, k, v = _vec_rows(q), _vec_rows(k), _vec_rows(v)
         table = None if table is None else _c(table)
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         lse = torch.empty((q.shape[0], cfg[0], q.shape[1]), device=q.device, dtype=torch.float32) if need_lse else None
+        out32 = torch.empty(q.shape, device=q.device, dtype=torch.float32) if need_lse and q.dtype != torch.float32 else None
         with _on_device(q):
-            d = AttentionFn._desc(q, k, v, table, cfg, out, lse)
+            d = AttentionFn._desc(q, k, v, table, cfg, out, lse, out32)
             L, r = hip.lib(), ctypes.byref(d)
             nb = L.ekaid_attn_workspace_bytes(r, 0)
             ws = _scratch(nb, q.device) if nb else None
             check(L.ekaid_attn_fwd(r, ptr(ws), nb, stream()), 'attn_fwd')
-        return out, lse, (q, k, v, table)
+        return out, (lse, out32), (q, k, v, table)
 
     @staticmethod
     def forward(ctx, q, k, v, table, cfg):
-        out, lse, operands = AttentionFn.launch(q, k, v, table, cfg, any(ctx.needs_input_grad[:4]))
+        out, stats, operands = AttentionFn.launch(q, k, v, table, cfg, any(ctx.needs_input_grad[:4]))
         ctx.cfg = cfg
-        ctx.save_for_backward(*operands, out, lse, cfg[2], cfg[3], cfg[4])
+        ctx.save_for_backward(*operands, out, *stats, cfg[2], cfg[3], cfg[4])
         return out
 
     @staticmethod
-    def _desc(q, k, v, table, cfg, out, lse):
+    def _desc(q, k, v, table, cfg, out, lse, out32):
         (heads, kv_heads, k_len, key_mask, q_pos, causal, bidirectional, max_distance, scale, p, seed) = cfg
         d = hip.Attn()
         d.q, d.k, d.v, d.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[q.dtype]
@@ -2353,13 +2354,13 @@ class AttentionFn(Function):
             d.border[:len(borders)] = borders
         d.causal = int(causal)
         d.drop_p, d.drop_seed = p, seed
-        d.out, d.lse = out.data_ptr(), ptr(lse)
+        d.out, d.lse, d.out32 = out.data_ptr(), ptr(lse), ptr(out32)
         return d
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, out, lse, k_len, key_mask, q_pos = ctx.saved_tensors
+        q, k, v, table, out, lse, out32, k_len, key_mask, q_pos = ctx.saved_tensors
         dout = _c(dout)
         if dout.data_ptr() % 16:
             dout = dout.clone()
@@ -2370,7 +2371,7 @@ class AttentionFn(Function):
         if q.shape[0] == 0 or q.shape[1] == 0:
             return dq, dk.zero_(), dv.zero_(), (dtable.zero_() if table is not None else None), None
         with _on_device(q):
-            d = AttentionFn._desc(q, k, v, table, ctx.cfg, out, lse)
+            d = AttentionFn._desc(q, k, v, table, ctx.cfg, out, lse, out32)
             d.dout, d.dq, d.dk, d.dv, d.dtable = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(dtable)
             L = hip.lib()
             nb = L.ekaid_attn_workspace_bytes(ctypes.byref(d), 1)

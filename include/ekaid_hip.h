@@ -715,6 +715,8 @@ typedef struct ekaid_attn {
     uint64_t drop_seed;
     void* out;
     float* lse;
+    float* out32;           /* 16-bit types, optional: out before its rounding, [B][Lq][H dh] f32, written by fwd and read by bwd for <dout, out>:
+                               the rounding of out would enter every score gradient of the row, and the bias table's sums add it up */
     const void* dout;
     void* dq;
     void* dk;

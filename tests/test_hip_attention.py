@@ -3,7 +3,8 @@
 Every bound is derived, none is fitted: u = 2^-24 for arithmetic in f32, h = half a step of the tensors' type where a value is rounded to
 it.  A score carries (dh + 3) u S (S = scale * sum |q||k|), a probability twice that plus (Lk + 8) u relative; probabilities and score
 gradients are rounded to the type (h relative; f16 also 2^-25 absolute below its normal range, score gradients after their power-of-two
-scaling) where they enter a product; delta = <dout, out> uses the rounded output (h relative per term); the result is rounded once (h)."""
+scaling) where they enter a product; delta = <dout, out> uses the output before its rounding -- formed from rounded probabilities, which reaches dq; with a bias table the rest of the
+backward takes delta as the f32 sum of P dP -- and the result is rounded once (h)."""
 import ctypes
 import math
 
@@ -85,16 +86,19 @@ def reference(t, H, KV, dh, k_len=None, key_mask=None, q_pos=None, causal=False,
     # the largest magnitude of a score decides the rounding of the power of two's argument
     ep = 2 * (dh + 6) * u * (S.amax(3, keepdim=True) if Lk else m * 0) + (Lk + 8) * u
     o = pd @ v
-    eo = (pd * (ep + hp) + tiny * keep) @ v.abs() + h * o.abs()
+    eo32 = (pd * (ep + hp) + tiny * keep) @ v.abs()               # before the result is rounded
+    eo = eo32 + h * o.abs()
     dpr = do @ v.transpose(2, 3)
     delta = (do * o).sum(3, keepdim=True)
-    edelta = (do.abs() * (eo + u * dh * o.abs())).sum(3, keepdim=True)
+    edelta = (do.abs() * (eo32 + u * (dh + 1) * o.abs())).sum(3, keepdim=True)
     ds = p * (dpr * keep - delta)
     absd = p * ((do.abs() @ v.abs().transpose(2, 3)) * keep + (do.abs() * o.abs()).sum(3, keepdim=True))
     nrm = do.norm(dim=3, keepdim=True)
     under = tiny * nrm / 8
     eds = absd * (ep + 2 * dh * u) + p * edelta                   # of ds in f32
     edq = scale * ((eds + hp * ds.abs() + under) @ k.abs())
+    if 'table' in t:
+        eds = absd * (ep + 2 * dh * u) + p * (absd * (ep + 2 * dh * u + Lk * u)).sum(3, keepdim=True)
     dq = scale * (ds @ k)
     share = lambda x: x.view(B, KV, G, Lk, dh).sum(2)               # noqa: E731
     dk = share(scale * (ds.transpose(2, 3) @ q))
