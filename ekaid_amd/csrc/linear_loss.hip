@@ -959,6 +959,226 @@ __global__ __launch_bounds__(1024) void ll32_db_kernel(const float* z, long long
     out[c] = s;
 }
 
+// ---- f32, few words: products on the f32 matrix instructions, whole rows of logits in one workgroup, logits kept for the backward
+//
+// z[row][word] = (x W^T + bias) log2 e, -infinity behind the last word.  A workgroup takes 16 of the rows that count, its waves every fourth 16
+// words; lanes read 16 bytes along the width (four matrix instructions), one 64-wide block ahead.  Workgroups start at different blocks: rows
+// of the weight a power of two apart share a few channels of the second-level cache, which all workgroups at one block would wait for.
+template <int TW> __global__ __launch_bounds__(256) void ll_narrow_fwd_kernel(const ekaid_linear_loss_t d, State st, float* z, int ldz) {
+    __shared__ float sm[4][16], sl[4][16], stz[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, kq = lane >> 4;
+    const int count = st.count[0], row = blockIdx.x * 16 + j;
+    if ((int)blockIdx.x * 16 >= count) return;
+    const int rc = st.idx[min(row, count - 1)];
+    const float *xp = (const float*)d.x + (long long)rc * d.ldx + 4 * kq, *wp[TW];
+#pragma unroll
+    for (int u = 0; u < TW; ++u) wp[u] = (const float*)d.weight + (long long)min(16 * (wave + 4 * u) + j, d.V - 1) * d.D + 4 * kq;
+    f32x4 acc[TW];
+#pragma unroll
+    for (int u = 0; u < TW; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 x0[4], x1[4], w0[4][TW], w1[4][TW];
+    auto fetch = [&](int k0, f32x4* xf, f32x4 (*wf)[TW]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int k = k0 + 16 * s;
+            const bool in = k + 4 * kq < d.D;
+            const int o = in ? k : 0;                          // behind the width: zeros (x and the weight alike, an infinite weight is none here)
+            xf[s] = *reinterpret_cast<const f32x4*>(xp + (in ? k : -4 * kq));
+            if (!in) xf[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < TW; ++u) {
+                wf[s][u] = *reinterpret_cast<const f32x4*>(wp[u] + (in ? o : -4 * kq));
+                if (!in) wf[s][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    };
+    auto multiply = [&](const f32x4* xf, const f32x4 (*wf)[TW]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int u = 0; u < TW; ++u) acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[s][u][c], xf[s][c], acc[u], 0, 0, 0);
+    };
+    const int blocks = (d.D + 63) >> 6, turn = blockIdx.x % blocks;
+    auto at = [&](int k) { return 64 * (k + turn < blocks ? k + turn : k + turn - blocks); };
+    fetch(at(0), x0, w0);
+    for (int k = 0; k < blocks; k += 2) {
+        if (k + 1 < blocks) fetch(at(k + 1), x1, w1);
+        multiply(x0, w0);
+        if (k + 1 >= blocks) break;
+        if (k + 2 < blocks) fetch(at(k + 2), x0, w0);
+        multiply(x1, w1);
+    }
+    const long long target = d.target[(rc / d.T) * d.ld_target + rc % d.T];
+    const float* bias = (const float*)d.bias;
+    float m = NEG_INF, l = 0.f;
+#pragma unroll
+    for (int u = 0; u < TW; ++u) {
+        const int v0 = 16 * (wave + 4 * u) + 4 * kq;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = v0 + i;
+            acc[u][i] = v < d.V ? (acc[u][i] + (bias ? bias[min(v, d.V - 1)] : 0.f)) * LOG2E : NEG_INF;
+            m = fmaxf(m, acc[u][i]);
+            if (v == target && v < d.V) stz[j] = acc[u][i];
+        }
+        if (row < count && v0 < ldz) *reinterpret_cast<f32x4*>(z + (long long)row * ldz + v0) = acc[u];
+    }
+    if (wave == 0 && kq == 0 && (target < 0 || target >= d.V)) stz[j] = __builtin_nanf("");
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float base = m == NEG_INF ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < TW; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(acc[u][i] - base);
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (kq == 0) {
+        sm[wave][j] = m;
+        sl[wave][j] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16 || row >= count) return;
+    const float M = fmaxf(fmaxf(sm[0][j], sm[1][j]), fmaxf(sm[2][j], sm[3][j])), B = M == NEG_INF ? 0.f : M;
+    float s = 0.f;
+    for (int k = 0; k < 4; ++k) s += sl[k][j] * __builtin_amdgcn_exp2f((sm[k][j] == NEG_INF ? 0.f : sm[k][j]) - B);
+    const float lse = M + __builtin_amdgcn_logf(s);
+    st.lse[row] = lse;
+    st.nll[row] = (lse - stz[j]) * LN2 * d.mask[(rc / d.T) * d.ld_mask + rc % d.T];
+}
+
+// dz of the rows row0 .. last - 1 (at most ROWS, counted among those that count) from their kept logits into dst[..][stride], zeros behind
+// them: 256 / ROWS threads a row, 16 bytes each
+template <int ROWS> __device__ __forceinline__ void narrow_dz(const ekaid_linear_loss_t& d, const State& st, const float* z, int ldz, int row0, int last, float f, float* dst, int stride) {
+    constexpr int PER = 256 / ROWS;
+    const int r = threadIdx.x / PER, c = threadIdx.x % PER, k = min(row0 + r, last - 1), row = st.idx[k];
+    const float w = row0 + r < last ? d.mask[(row / d.T) * d.ld_mask + row % d.T] * f : 0.f, lse = st.lse[k];
+    const long long target = d.target[(row / d.T) * d.ld_target + row % d.T];
+    for (int v = 4 * c; v < ldz; v += 4 * PER) {
+        const f32x4 q = *reinterpret_cast<const f32x4*>(z + (long long)k * ldz + v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[r * stride + v + i] = row0 + r < last ? (__builtin_amdgcn_exp2f(q[i] - lse) - (target == v + i ? 1.f : 0.f)) * w : 0.f;
+    }
+}
+// Both gradients in one launch.  Workgroups below nx: 16 rows of dx, dz (LDS) times the weight, the waves take the width 2 x 64 apart; and
+// zeros for those of 16 rows of x that do not count.  The others: one of `parts` shares of the rows of dz^T x over 64 of the width, 32 rows
+// at a time, the waves take the words; shares joined by ll_narrow_sum.
+template <int TW> __global__ __launch_bounds__(256, 3) void ll_narrow_bwd_kernel(const ekaid_linear_loss_t d, State st, const float* z, int ldz, int nx, int nd, int parts, float* pdw, float* pdb) {
+    __shared__ __attribute__((aligned(16))) float dz[32 * (64 * TW + 16)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, kq = lane >> 4;
+    const int count = st.count[0];
+    const float f = d.dloss[0] / (d.denom ? d.denom[0] : st.sums[0]);
+    if ((int)blockIdx.x < nx) {
+        for (int r = 16 * blockIdx.x + wave; r < min(d.B * d.T, 16 * (int)blockIdx.x + 16); r += 4)
+            if (st.pos[r] < 0)
+                for (int c = 4 * lane; c < d.D; c += 256) *reinterpret_cast<f32x4*>((float*)d.dx + (long long)r * d.D + c) = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int r0 = blockIdx.x * 16, stride = ldz + 2;     // (16 rows two words apart in the banks)
+        if (r0 >= count) return;
+        narrow_dz<16>(d, st, z, ldz, r0, count, f, dz, stride);
+        __syncthreads();
+        const float* mine = dz + j * stride + kq;
+        for (int d0 = 128 * wave; d0 < d.D; d0 += 512) {
+            f32x4 acc[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[h][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const float *wp0 = (const float*)d.weight + min(d0 + 4 * j, d.D - 4), *wp1 = (const float*)d.weight + min(d0 + 64 + 4 * j, d.D - 4);
+            f32x4 a0[4][2], a1[4][2];
+            auto fetch = [&](int v0, f32x4 (*a)[2]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const long long o = (long long)min(v0 + 4 * s + kq, d.V - 1) * d.D;
+                    a[s][0] = *reinterpret_cast<const f32x4*>(wp0 + o);
+                    a[s][1] = *reinterpret_cast<const f32x4*>(wp1 + o);
+                }
+            };
+            auto multiply = [&](int v0, const f32x4 (*a)[2]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const float g = mine[v0 + 4 * s];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[h][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s][h][c], g, acc[h][c], 0, 0, 0);
+                }
+            };
+            fetch(0, a0);
+            for (int v0 = 0; v0 < ldz; v0 += 32) {
+                if (v0 + 16 < ldz) fetch(v0 + 16, a1);
+                multiply(v0, a0);
+                if (v0 + 16 >= ldz) break;
+                if (v0 + 32 < ldz) fetch(v0 + 32, a0);
+                multiply(v0 + 16, a1);
+            }
+            if (r0 + j >= count) continue;
+            float* out = (float*)d.dx + (long long)st.idx[r0 + j] * d.D;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = d0 + 64 * h + 16 * kq + 4 * i;
+                    if (c < d.D) *reinterpret_cast<f32x4*>(out + c) = f32x4{acc[h][0][i], acc[h][1][i], acc[h][2][i], acc[h][3][i]};
+                }
+        }
+        return;
+    }
+    const int q = blockIdx.x - nx, d0 = (q % nd) * 64, part = q / nd, share = ((count + parts - 1) / parts + 31) & ~31, first = min(count, part * share), last = min(count, first + share);
+    const int stride = ldz | 16;                               // (four rows half the banks apart)
+    const float* xp = (const float*)d.x + min(d0 + 4 * j, d.D - 4);
+    f32x4 acc[TW][4];
+#pragma unroll
+    for (int u = 0; u < TW; ++u)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[u][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (int r0 = first; r0 < last; r0 += 32) {
+        f32x4 xf[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) xf[s] = *reinterpret_cast<const f32x4*>(xp + (long long)st.idx[min(r0 + 4 * s + kq, last - 1)] * d.ldx);
+        narrow_dz<32>(d, st, z, ldz, r0, last, f, dz, stride);
+        __syncthreads();
+        if (d0 == 0 && (int)threadIdx.x < ldz)
+            for (int r = 0; r < 32; ++r) sum += dz[r * stride + threadIdx.x];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+#pragma unroll
+            for (int u = 0; u < TW; ++u) {
+                const float g = dz[(4 * s + kq) * stride + min(16 * (wave + 4 * u), ldz - 16) + j];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[u][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(g, xf[s][c], acc[u][c], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+    if (pdb && d0 == 0 && (int)threadIdx.x < ldz) pdb[(long long)part * ldz + threadIdx.x] = sum;
+    if (!pdw || d0 + 4 * j >= d.D) return;
+#pragma unroll
+    for (int u = 0; u < TW; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = 16 * (wave + 4 * u) + 4 * kq + i;
+            if (v < d.V) *reinterpret_cast<f32x4*>(pdw + ((long long)part * d.V + v) * d.D + d0 + 4 * j) = f32x4{acc[u][0][i], acc[u][1][i], acc[u][2][i], acc[u][3][i]};
+        }
+}
+// parts of dweight (16 bytes a thread) and of dbias (behind them), added in order
+__global__ __launch_bounds__(256) void ll_narrow_sum_kernel(const ekaid_linear_loss_t d, const float* pdw, const float* pdb, int ldz, int parts) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, nw = d.dweight ? (long long)d.V * d.D / 4 : 0;
+    if (i < nw) {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int k = 0; k < parts; ++k) s += reinterpret_cast<const f32x4*>(pdw)[k * nw + i];
+        reinterpret_cast<f32x4*>(d.dweight)[i] = s;
+    } else if (d.dbias && i - nw < d.V) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < parts; ++k) s += pdb[(long long)k * ldz + (i - nw)];
+        ((float*)d.dbias)[i - nw] = s;
+    }
+}
+
 // ---- host side
 int ll_check(const ekaid_linear_loss_t* a, const char* who) {
     if (!a) { set_error("%s: null descriptor", who); return EKAID_ERR_ARG; }
@@ -968,6 +1188,7 @@ int ll_check(const ekaid_linear_loss_t* a, const char* who) {
         return EKAID_ERR_ARG;
     }
     const int al = a->dtype == EKAID_F32 ? 4 : 16;
+    if ((uintptr_t)a->state & 15) { set_error("%s: the state must be 16-byte aligned", who); return EKAID_ERR_ARG; }
     if (a->dtype != EKAID_F32 && (a->D % 8 || a->ldx % 8)) { set_error("%s: width %d / row stride %lld must be multiples of 8", who, a->D, a->ldx); return EKAID_ERR_UNSUPPORTED; }
     if (a->ldx < a->D || a->ldx > (1 << 30)) { set_error("%s: row stride %lld", who, a->ldx); return EKAID_ERR_ARG; }
     if (((uintptr_t)a->x | (uintptr_t)a->weight | (uintptr_t)a->dx | (uintptr_t)a->dweight) & (al - 1)) { set_error("%s: operands must be %d-byte aligned", who, al); return EKAID_ERR_ARG; }
@@ -976,7 +1197,16 @@ int ll_check(const ekaid_linear_loss_t* a, const char* who) {
 constexpr size_t PIECE_BYTES = size_t(512) << 20;              // dz (or f32 logits) of one piece
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Few words (f32): one launch forms the logits, their statistics and the losses, one both gradients, and the logits, no larger than x
+// itself, stay in the state.  A rule of sizes alone, since it says what the state holds.  5760 rows of width 512, 148 words, against the
+// route through ekaid_gemm_f32: NARROW_FIGURES
+bool few_words(const ekaid_linear_loss_t* a) {
+    return a->dtype == EKAID_F32 && a->V <= 256 && a->V <= a->D && a->D % 4 == 0 && (double)a->B * a->T * a->V * a->D < 2147483648.0;
+}
+size_t kept_offset(const ekaid_linear_loss_t* a) { return (256 + (size_t)a->B * a->T * 20 + 255) & ~size_t(255); }
 struct LossPlan {
+    int narrow;                    // few words, and operands in whole 16 bytes
+    int parts;                     // shares of dW
     int terms;                     // f32 as 16-bit terms through the tile kernels
     int big;                       // 256 x 256 tiles
     long long n, nr;
@@ -1009,6 +1239,15 @@ LossPlan loss_plan(const ekaid_linear_loss_t* a, int backward) {
     p.n = (long long)a->B * a->T;
     p.nr = (p.n + 255) & ~255ll;
     size_t o = 0;
+    p.narrow = few_words(a) && a->ldx % 4 == 0 && !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
+    if (p.narrow) {
+        p.ldz = (a->V + 15) & ~15;
+        p.parts = (int)std::max(1ll, std::min<long long>(320 / std::max(1, std::min(320, cdiv(a->D, 64))), (p.n + 63) / 64));        // about 320 workgroups, 64 rows or more each
+        p.pdw = o; o += backward ? up256((size_t)p.parts * a->V * a->D * 4) : 0;
+        p.pdb = o; o += backward ? up256((size_t)p.parts * p.ldz * 4) : 0;
+        p.total = o;
+        return p;
+    }
     // (below 2^31 products of a matrix the few tiles are bound by latency, and ekaid_gemm_f32 with its splits is level or ahead)
     p.terms = a->dtype == EKAID_F32 && a->arith == EKAID_GEMM_F16X2 && (double)p.n * a->V * a->D >= 2147483648.0 && a->D % 8 == 0 && a->ldx % 4 == 0 && !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
     if (a->dtype == EKAID_F32 && !p.terms) {
@@ -1144,6 +1383,27 @@ int bwd32(const ekaid_linear_loss_t* a, const LossPlan& p, State st, char* ws, h
     return check_launch("linear_loss_bwd");
 }
 
+template <int TW> int narrow(const ekaid_linear_loss_t* a, const LossPlan& p, State st, char* ws, bool backward, hipStream_t s) {
+    float* z = (float*)((char*)a->state + kept_offset(a));
+    if (!backward) {
+        hipLaunchKernelGGL(ll_narrow_fwd_kernel<TW>, dim3(cdiv(p.n, 16)), dim3(256), 0, s, *a, st, z, p.ldz);
+        return check_launch("linear_loss_fwd");
+    }
+    float *pdw = a->dweight ? (float*)(ws + p.pdw) : nullptr, *pdb = a->dbias ? (float*)(ws + p.pdb) : nullptr;
+    const int nx = a->dx ? cdiv(p.n, 16) : 0, nd = a->dweight ? cdiv(a->D, 64) : 1, nw = a->dweight || a->dbias ? nd * p.parts : 0;
+    if (nx + nw) hipLaunchKernelGGL(ll_narrow_bwd_kernel<TW>, dim3(nx + nw), dim3(256), 0, s, *a, st, z, p.ldz, nx, nd, p.parts, pdw, pdb);
+    if (nw) hipLaunchKernelGGL(ll_narrow_sum_kernel, dim3(cdiv((a->dweight ? (long long)a->V * a->D / 4 : 0) + a->V, 256)), dim3(256), 0, s, *a, pdw, pdb, p.ldz, p.parts);
+    return check_launch("linear_loss_bwd");
+}
+int narrow(const ekaid_linear_loss_t* a, const LossPlan& p, State st, char* ws, bool backward, hipStream_t s) {
+    switch (cdiv(a->V, 64)) {
+        case 1: return narrow<1>(a, p, st, ws, backward, s);
+        case 2: return narrow<2>(a, p, st, ws, backward, s);
+        case 3: return narrow<3>(a, p, st, ws, backward, s);
+        default: return narrow<4>(a, p, st, ws, backward, s);
+    }
+}
+
 void launch_terms(const LossArgs& a, const LossPlan& p, hipStream_t s) {
     hipLaunchKernelGGL(ll_terms_kernel, dim3(cdiv(p.nr + a.d.V, 4)), dim3(256), 0, s, a, (unsigned short*)a.xc, (unsigned short*)a.xb, (unsigned short*)a.wp, (float*)a.sx,
                        (float*)a.sw, (int)p.nr);
@@ -1213,7 +1473,7 @@ LossArgs loss_args(const ekaid_linear_loss_t* a, const LossPlan& p, char* ws, bo
 
 extern "C" size_t ekaid_linear_loss_state_bytes(const ekaid_linear_loss_t* a) {
     if (ekaid::ll_check(a, "linear_loss_state_bytes")) return 0;
-    return 256 + (size_t)a->B * a->T * 20;
+    return ekaid::kept_offset(a) + (ekaid::few_words(a) ? (size_t)a->B * a->T * ((a->V + 15) & ~15) * 4 : 0);
 }
 extern "C" size_t ekaid_linear_loss_workspace_bytes(const ekaid_linear_loss_t* a, int backward) {
     if (ekaid::ll_check(a, "linear_loss_workspace_bytes")) return 0;
@@ -1230,7 +1490,8 @@ extern "C" int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspa
     hipLaunchKernelGGL(ll_rows_kernel, dim3(1), dim3(1024), 0, s, a->mask, a->ld_mask, a->B, a->T, st);
     int rc = check_launch("linear_loss_fwd");
     if (rc == EKAID_OK && p.n) {
-        if (a->dtype == EKAID_F32 && !p.terms) rc = fwd32(a, p, st, (char*)workspace, s);
+        if (p.narrow) rc = narrow(a, p, st, (char*)workspace, false, s);
+        else if (a->dtype == EKAID_F32 && !p.terms) rc = fwd32(a, p, st, (char*)workspace, s);
         else {
             const LossArgs k = loss_args(a, p, (char*)workspace, false);
             if (a->dtype == EKAID_F32) rc = p.big ? fwd16<float, 256, 128, 64>(k, p, s) : fwd16<float, 128, 64, 64>(k, p, s);
@@ -1239,7 +1500,7 @@ extern "C" int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspa
         }
     }
     if (rc) return rc;
-    hipLaunchKernelGGL(ll_loss_kernel, dim3(1), dim3(1024), 0, s, *a, st, a->dtype == EKAID_F32 && !p.terms);
+    hipLaunchKernelGGL(ll_loss_kernel, dim3(1), dim3(1024), 0, s, *a, st, a->dtype == EKAID_F32 && !p.terms && !p.narrow);
     return check_launch("linear_loss_fwd");
 }
 extern "C" int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1250,6 +1511,8 @@ extern "C" int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspa
     if (!a->dloss || !a->state || !a->x || !a->weight || !a->target || !a->mask) { set_error("linear_loss_bwd: null operand"); return EKAID_ERR_ARG; }
     if (workspace_bytes < p.total || !workspace) { set_error("linear_loss_bwd: workspace of %zu bytes needed", p.total); return EKAID_ERR_ARG; }
     hipStream_t s = (hipStream_t)stream;
+    if (p.narrow && (((uintptr_t)a->dx | (uintptr_t)a->dweight) & 15)) { set_error("linear_loss_bwd: dx and dweight must be 16-byte aligned"); return EKAID_ERR_ARG; }
+    if (p.narrow) return narrow(a, p, state_of(a->state, p.n), (char*)workspace, true, s);
     if (a->dtype == EKAID_F32 && !p.terms) return bwd32(a, p, state_of(a->state, p.n), (char*)workspace, s);
     const LossArgs k = loss_args(a, p, (char*)workspace, true);
     if (a->dtype == EKAID_F32) return p.big ? bwd16<float, 256, 128, 64>(k, p, s) : bwd16<float, 128, 64, 64>(k, p, s);

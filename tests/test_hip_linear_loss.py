@@ -106,6 +106,36 @@ def test_loss_and_gradients(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('shape', [(1, 1, 4, 1), (3, 7, 4, 4), (2, 33, 60, 60), (2, 40, 68, 65), (7, 97, 132, 129), (3, 50, 256, 256), (64, 90, 512, 148), (5, 61, 1028, 200)],
+                         ids=lambda s: 'x'.join(map(str, s)))
+def test_few_words(shape):
+    """No more words than the width (f32: whole rows of logits in one workgroup): whatever stands in rows that do not count, weighted rows, whole
+    workgroups of them without a counting row; each gradient alone is the one of the full call; x that is no whole vector takes the other route."""
+    from ekaid_amd import ops
+    B, T, D, V = shape
+    t = make(F32, *shape)
+    t['mask'] = t['mask'] * (torch.arange(B * T, device=DEV).view(B, T) % 5 + 1) / 4
+    if B > 1:
+        t['mask'][:B // 2 + 1].mul_(torch.tensor(0.0, device=DEV))
+    off = t['mask'] == 0
+    t['x'][off] = float('nan')
+    t['target'][off] = 10 ** 12
+    want = reference(t, dloss=0.5)
+    got = run(t, dloss=0.5)
+    if off.all():                                             # nothing counts (two samples, both masked): loss 0 / 0, gradients 0
+        assert torch.isnan(want[0][0]) and torch.isnan(got[0])
+        assert all(float(g.abs().max()) == 0 for g in got[1:])
+    else:
+        compare(got, want)
+    for k, name in enumerate(('x', 'weight', 'bias')):
+        leaf = {n: t[n].detach().requires_grad_(n == name) for n in ('x', 'weight', 'bias')}
+        loss = ops.linear_lm_loss(leaf['x'], leaf['weight'], leaf['bias'], t['target'], t['mask'])
+        assert torch.equal(torch.autograd.grad(loss, leaf[name], torch.tensor(0.5, device=DEV))[0], got[1 + k]), name
+    t['weight'][V // 2, 0] = float('inf')
+    assert not torch.isfinite(run(t)[0])
+
+
+@gpu
 @pytest.mark.parametrize('mode', ['f32', 'bf16x3', 'f16x2'])
 def test_f32_arithmetics_and_odd_widths(mode):
     """Every product arithmetic, a width that is no whole vector, a size that takes the operand bounds of the two-term split."""
