@@ -131,6 +131,14 @@ def test_few_words(shape):
         leaf = {n: t[n].detach().requires_grad_(n == name) for n in ('x', 'weight', 'bias')}
         loss = ops.linear_lm_loss(leaf['x'], leaf['weight'], leaf['bias'], t['target'], t['mask'])
         assert torch.equal(torch.autograd.grad(loss, leaf[name], torch.tensor(0.5, device=DEV))[0], got[1 + k]), name
+    flat = torch.zeros(V * D + 1, device=DEV)                 # the weight's gradient into a slot of a flat buffer that is no whole vector
+    ops._grad_slots[t['weight'].data_ptr()] = (t['weight'], flat, 1, V * D, (V, D))
+    try:
+        run(t, dloss=0.5)
+    finally:
+        del ops._grad_slots[t['weight'].data_ptr()]
+        ops._grad_claimed.discard(t['weight'].data_ptr())
+    assert torch.equal(flat[1:].view(V, D), got[2])
     t['weight'][V // 2, 0] = float('inf')
     assert not torch.isfinite(run(t)[0])
 
