@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
         }
         if constexpr (REL) {
             // sums over equal distance j - pos: a unit that lies wholly beyond the reach goes to one bucket; otherwise it is written to LDS by
-            // diagonals and lane x adds up diagonal x (rows ascending: a fixed order), whose distance no other lane of the wave holds.
+            // diagonals and lane x adds up diagonal x (in a fixed order), whose distance no other lane of the wave holds.
             // Places of a diagonal that the unit does not have stay zero from the start.
             if (jw + G - 1 - pu <= -d.reach || jw - (pu + U - 1) >= d.reach) {
                 float z = 0.f;
@@ -335,11 +335,12 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
                 if (jw < pu) far_back += z; else far_ahead += z;
             } else {
                 wave_fence();
-                float* at = skew + (lane % G + U - 1) * DP - (DP - 1) * 4 * g;        // (row r, key c) at diagonal c - r + U - 1, place r
+                // (row r, key c) at diagonal c - r + U - 1, group of places r / 4, place (c + U - 1) % 4: the 64 writes of a value meet 64 banks
+                float* at = skew + (lane % G + U - 1 - 4 * g) * DP + 4 * g + ((lane + U - 1) & 3);
 #pragma unroll
                 for (int q = 0; q < NB * nq; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) at[-(DP - 1) * (4 * ng * q + e)] = ok ? dp[q / nq][4 * (q % nq) + e] : 0.f;
+                    for (int e = 0; e < 4; ++e) at[4 * ng * q - DP * (4 * ng * q + e)] = ok ? dp[q / nq][4 * (q % nq) + e] : 0.f;
                 wave_fence();
                 if (lane < DIAG) {
                     const float* row = skew + lane * DP;

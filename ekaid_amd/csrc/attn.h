@@ -126,16 +126,20 @@ template <typename T, int G> __device__ __forceinline__ u32x4 row_frag_global(co
 // ---- tiles copied to LDS without passing registers
 // A tile is ROWS rows x DH elements, rows packed (no padding: a wave writes 1 KB in lane order), the 16-byte slots of a row permuted by an
 // exclusive-or with swz(row) so that both kinds of reads spread over the banks: 16 rows at one slot (row fragments), and 4 consecutive
-// rows over 64 bytes (transposing reads) or two rows 4 apart over 128 bytes (f32 columns).  The permutation is applied to the global
+// rows over 64 or 32 bytes (transposing reads), two rows 4 apart over 128 bytes or four over 64 (f32 columns).  16-byte reads go to the banks
+// in groups of lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31: with blocks of 16 rows, where lanes 16 on read the next slot, rows whose
+// swz() differ by 1 must lie in one group (dk / dv of 128-wide 16-bit heads: 2 extra cycles of every 8 otherwise).  The permutation is
+// applied to the global
 // address.  Rows that do not exist or are masked, and columns beyond dh, are read from a zero vector: NaN or Inf there never arrives.
 __device__ __attribute__((aligned(16))) const uint32_t attn_zero16[4] = {0u, 0u, 0u, 0u};
 typedef __attribute__((address_space(3))) void* lds_void;
 typedef const __attribute__((address_space(1))) void* global_void;
 
 template <typename T, int DH> __device__ __host__ __forceinline__ constexpr int swz(int row) {
-    if constexpr (DH * sizeof(T) == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
-    else if constexpr (sizeof(T) == 2) return (row & 3) << 2 | ((row >> 2) & 3);
-    else return ((row >> 2) & 1) << 3 | (row & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 3) & 1);
+    const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b3 = (row >> 3) & 1;
+    if constexpr (DH * sizeof(T) == 128) return b1 << 2 | (b2 ^ b3) << 1 | b3;
+    else if constexpr (sizeof(T) == 2) return b0 << 2 | b1 << 3 | (b2 ^ b3) << 1 | b3;
+    else return b2 << 3 | b3 << 2 | b1 << 1 | b0;
 }
 template <typename T, int DH, int ROWS, int NW> struct TileCopy {
     static constexpr int epl = Elem<T>::epl, rb = DH * (int)sizeof(T), per = 1024 / rb > 0 ? 1024 / rb : 1, lanes = rb / 16, chunks = ROWS * rb / 1024 / NW;
