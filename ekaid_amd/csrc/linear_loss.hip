@@ -133,7 +133,7 @@ template <typename T> __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, 
 }
 
 // One operand tile: R rows (or columns) x 64 contracted elements, 1 KB per wave and instruction straight into LDS.
-//   contracted index contiguous (COL = false): LDS [R][64], the 16-byte slots of row r permuted by ^ (r & 7);
+//   contracted index contiguous (COL = false): LDS [R][64], the 16-byte slots of row r permuted by ^ (r / 2 & 7): 16 rows at one slot fill 64 banks;
 //   contracted index strided   (COL = true):  LDS [64][R], the 64-byte groups of row k permuted by ^ (k & 3)
 // -- so that fragment reads meet few bank conflicts; the permutation is applied to the GLOBAL address, LDS is written in lane order.
 template <int R, bool COL, int NW> struct Operand {
@@ -155,7 +155,7 @@ template <int R, bool COL, int NW> struct Operand {
         step = BK * 2;
 #pragma unroll
         for (int i = 0; i < chunks; ++i) {
-            const int r = (i * NW + wave) * 8 + (lane >> 3), s = (lane & 7) ^ (r & 7);
+            const int r = (i * NW + wave) * 8 + (lane >> 3), s = (lane & 7) ^ ((r >> 1) & 7);
             p[i] = (const char*)row(r) + s * 16;
             k0[i] = s * 8;
         }
@@ -177,7 +177,7 @@ template <int R, bool COL> __device__ __forceinline__ u32x4 operand_frag(const c
     const int g = lane >> 5;
     if constexpr (!COL) {
         const int r = r0 + (lane & 31);
-        return *reinterpret_cast<const u32x4*>(lds + r * 128 + (((c * 2 + g) ^ (r & 7)) << 4));
+        return *reinterpret_cast<const u32x4*>(lds + r * 128 + (((c * 2 + g) ^ ((r >> 1) & 7)) << 4));
     } else {
         u32x4 f;
 #pragma unroll
