@@ -748,14 +748,19 @@ __global__ __launch_bounds__(256) void process_matrix_kernel(const T* adj, int B
 }
 
 // ------------------------------------------------------------------ Adam
+// The order of roundings is written out: fused where it says fmaf, every other product and sum rounded, whatever the compiler packs (an
+// update of 1e-4 on a weight of 1 shows each of them).  FUSED: the denominator's product and sum in one rounding (the by-value form).
+template <bool FUSED> __device__ __forceinline__ void adam_element(float& p, float gr, float& m, float& v, float lr_bc1, float beta1, float beta2, float eps, float inv_sqrt_bc2) {
+#pragma clang fp contract(off)
+    const float mi = fmaf(1.f - beta1, gr, beta1 * m);
+    const float vi = beta2 * v + (1.f - beta2) * gr * gr;
+    m = mi; v = vi;
+    p -= lr_bc1 * mi / (FUSED ? fmaf(sqrtf(vi), inv_sqrt_bc2, eps) : sqrtf(vi) * inv_sqrt_bc2 + eps);
+}
 __global__ __launch_bounds__(256) void adam_kernel(float* p, const float* g, float* m, float* v, long long n, float lr_bc1,
                                                    float beta1, float beta2, float eps, float inv_sqrt_bc2, float gscale) {
     GS_LOOP(i, n) {
-        const float gr = g[i] * gscale;
-        const float mi = beta1 * m[i] + (1.f - beta1) * gr;
-        const float vi = beta2 * v[i] + (1.f - beta2) * gr * gr;
-        m[i] = mi; v[i] = vi;
-        p[i] -= lr_bc1 * mi / (sqrtf(vi) * inv_sqrt_bc2 + eps);
+        adam_element<true>(p[i], g[i] * gscale, m[i], v[i], lr_bc1, beta1, beta2, eps, inv_sqrt_bc2);
     }
 }
 
@@ -779,11 +784,7 @@ __global__ __launch_bounds__(256) void adam_dev_kernel(float* p, const float* g,
     if (derived[2] != 0.f) return;            // (uniform over the grid: the whole update is skipped)
     const float lr_bc1 = derived[0], inv_sqrt_bc2 = derived[1], beta1 = hyper[1], beta2 = hyper[2], eps = hyper[3], gscale = hyper[4];
     GS_LOOP(i, n) {
-        const float gr = g[i] * gscale;
-        const float mi = beta1 * m[i] + (1.f - beta1) * gr;
-        const float vi = beta2 * v[i] + (1.f - beta2) * gr * gr;
-        m[i] = mi; v[i] = vi;
-        p[i] -= lr_bc1 * mi / (sqrtf(vi) * inv_sqrt_bc2 + eps);
+        adam_element<false>(p[i], g[i] * gscale, m[i], v[i], lr_bc1, beta1, beta2, eps, inv_sqrt_bc2);
     }
 }
 
