@@ -1204,7 +1204,7 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // words, against the route through ekaid_gemm_f32 with its 13 launches: kernels 125 -> 71 us (16 rows a workgroup, bound by the latency of
 // the second-level cache and of three dependent stages, not by the f32 matrix rate: 5 of the 22 us of the logits, 12 of the gradients' 35).
 bool few_words(const ekaid_linear_loss_t* a) {
-    return a->dtype == EKAID_F32 && a->V <= 256 && a->V <= a->D && a->D % 4 == 0 && (double)a->B * a->T * a->V * a->D < 2147483648.0;
+    return a->dtype == EKAID_F32 && a->V <= 256 && ((a->V + 15) & ~15) <= a->D && a->D % 4 == 0 && (double)a->B * a->T * a->V * a->D < 2147483648.0;
 }
 size_t kept_offset(const ekaid_linear_loss_t* a) { return (256 + (size_t)a->B * a->T * 20 + 255) & ~size_t(255); }
 struct LossPlan {

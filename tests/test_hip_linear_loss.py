@@ -106,11 +106,11 @@ def test_loss_and_gradients(shape, dtype):
 
 
 @gpu
-@pytest.mark.parametrize('shape', [(1, 1, 4, 1), (3, 7, 4, 4), (2, 33, 60, 60), (2, 40, 68, 65), (7, 97, 132, 129), (3, 50, 256, 256), (64, 90, 512, 148), (5, 61, 1028, 200)],
+@pytest.mark.parametrize('shape', [(1, 1, 4, 1), (3, 7, 4, 4), (2, 33, 60, 60), (2, 40, 68, 65), (7, 97, 132, 129), (2, 33, 60, 40), (7, 97, 132, 113), (2, 20, 16, 16), (9, 40, 20, 3), (3, 50, 256, 256), (64, 90, 512, 148), (5, 61, 1028, 200)],
                          ids=lambda s: 'x'.join(map(str, s)))
 def test_few_words(shape):
-    """No more words than the width (f32: whole rows of logits in one workgroup): whatever stands in rows that do not count, weighted rows, whole
-    workgroups of them without a counting row; each gradient alone is the one of the full call; x that is no whole vector takes the other route."""
+    """No more words, in whole sixteens, than the width (f32: whole rows of logits in one workgroup), and sizes just beside that: whatever stands
+    in rows that do not count, weighted rows; each gradient alone is the one of the full call; a weight gradient into an unaligned slot."""
     from ekaid_amd import ops
     B, T, D, V = shape
     t = make(F32, *shape)
@@ -130,7 +130,11 @@ def test_few_words(shape):
     for k, name in enumerate(('x', 'weight', 'bias')):
         leaf = {n: t[n].detach().requires_grad_(n == name) for n in ('x', 'weight', 'bias')}
         loss = ops.linear_lm_loss(leaf['x'], leaf['weight'], leaf['bias'], t['target'], t['mask'])
-        assert torch.equal(torch.autograd.grad(loss, leaf[name], torch.tensor(0.5, device=DEV))[0], got[1 + k]), name
+        alone = torch.autograd.grad(loss, leaf[name], torch.tensor(0.5, device=DEV))[0]
+        if (V + 15) // 16 * 16 <= D:
+            assert torch.equal(alone, got[1 + k]), name
+        else:                                                 # the other route: a bias gradient alone is summed in another order, within its bound
+            assert bool(((alone.double() - want[0][1 + k]).abs() <= want[1][1 + k] + 1e-30).all()), name
     flat = torch.zeros(V * D + 1, device=DEV)                 # the weight's gradient into a slot of a flat buffer that is no whole vector
     ops._grad_slots[t['weight'].data_ptr()] = (t['weight'], flat, 1, V * D, (V, D))
     try:
@@ -418,3 +422,31 @@ def test_c_entry_refuses_bad_descriptors():
     assert L.ekaid_linear_loss_bwd(ctypes.byref(desc()), 1 << 20, 16, None) < 0
     assert L.ekaid_linear_loss_bwd(ctypes.byref(desc(B=0)), 1 << 20, 1 << 40, None) < 0
     assert L.ekaid_linear_loss_fwd(None, None, 0, None) < 0 and L.ekaid_linear_loss_bwd(None, None, 0, None) < 0
+
+
+def test_few_words_state_and_alignment():
+    """The logits kept for the backward are a matter of sizes, not of addresses; what the kernels write whole vectors to must be aligned."""
+    from ekaid_amd import hip
+    L = hip.load()
+
+    def desc(**kw):
+        d = hip.LinearLoss()
+        for n in ('x', 'weight', 'target', 'mask', 'loss', 'state', 'dloss', 'dx', 'dweight'):
+            setattr(d, n, 1 << 20)
+        d.dtype, d.B, d.T, d.D, d.V, d.ldx, d.ld_target, d.ld_mask = 0, 2, 3, 64, 50, 64, 3, 3
+        for n, x in kw.items():
+            setattr(d, n, x)
+        return d
+
+    def state(**kw):
+        return L.ekaid_linear_loss_state_bytes(ctypes.byref(desc(**kw)))
+    wide = state(V=65)
+    assert state() == state(x=(1 << 20) + 4, weight=0) == wide + 6 * 64 * 4
+    assert state(V=64) == state() and state(V=16) == wide + 6 * 16 * 4 and state(V=256, D=256, ldx=256) == wide + 6 * 256 * 4
+    for kw in (dict(V=257, D=512, ldx=512), dict(D=62, V=20, ldx=62), dict(dtype=1), dict(B=1 << 14, T=1 << 7, D=1024, ldx=1024, V=1)):
+        n = max(kw.get('B', 2) * kw.get('T', 3), 6)
+        assert state(**kw) <= 512 + 20 * n, kw
+    assert L.ekaid_linear_loss_workspace_bytes(ctypes.byref(desc()), 0) == 0
+    for kw in (dict(state=(1 << 20) + 8), dict(dx=(1 << 20) + 4)):
+        assert L.ekaid_linear_loss_bwd(ctypes.byref(desc(**kw)), 1 << 20, 1 << 40, None) < 0 and 'aligned' in hip.last_error(), kw
+    assert L.ekaid_linear_loss_fwd(ctypes.byref(desc(state=(1 << 20) + 8)), 1 << 20, 1 << 40, None) < 0
