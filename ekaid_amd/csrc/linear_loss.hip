@@ -6,7 +6,10 @@
 //   backward  per piece of the vocabulary: z again -> dz = (softmax - onehot) mask, rounded to the type, and the bias partials;
 //             dW = dz^T x;  dx partials += dz W.   Three products where the formula has three, one more than if logits were kept: at width D
 //             forming z again costs 2 D flops a logit, reading a kept f32 one and writing it 8 bytes.
-// f32: the same pieces around ekaid_gemm_f32 (its arithmetic: the two-term f16 or the exact three-term bf16 split).
+// Bound by the matrix instructions and the barrier of each 64-deep tile: 11008 counting rows x 2048 x 65536 bf16: statistics 2.64 ms (1120 TF),
+// dz 3.14 (940, it writes 1.4 GB of logit gradients), dW 2.71 (1090), dx 3.49 (850, f32 partials of 16 shares joined by a pass).
+// f32: the same kernels on 16-bit terms of the operands; few words: ll_narrow_*; other arithmetics and small products: passes around
+// ekaid_gemm_f32.
 #include "common.h"
 #include "../../include/ekaid_hip.h"
 #include <algorithm>
@@ -1200,7 +1203,7 @@ constexpr size_t PIECE_BYTES = size_t(512) << 20;              // dz (or f32 log
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Few words (f32): one launch forms the logits, their statistics and the losses, one both gradients, and the logits, no larger than x
-// itself, stay in the state.  A rule of sizes alone, since it says what the state holds.  5760 rows (half of them counting) of width 512, 148
+// itself, stay in the state.  A rule of sizes alone, since it says what the state holds.  5760 rows (3740 counting) of width 512, 148
 // words, against the route through ekaid_gemm_f32 with its 13 launches: kernels 125 -> 71 us (16 rows a workgroup, bound by the latency of
 // the second-level cache and of three dependent stages, not by the f32 matrix rate: 5 of the 22 us of the logits, 12 of the gradients' 35).
 bool few_words(const ekaid_linear_loss_t* a) {
