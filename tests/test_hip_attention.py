@@ -346,6 +346,24 @@ def test_relative_attention(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('shape', [(1, 3, 64, 2, 1300), (2, 2, 128, 70, 1200), (1, 2, 256, 80, 1090), (2, 6, 64, 1150, 70)], ids=lambda s: 'x'.join(map(str, s)))
+def test_largest_reach(shape, dtype):
+    """The last bucket begins at the largest distance that is taken: the tables and sums in LDS at their full size."""
+    from ekaid_amd import ops
+    KV, H, dh, Lq, Lk = shape
+    md = max(m for m in range(900, 2000) if ops.relative_borders(64, m)[-1] <= 1024)
+    assert ops.relative_borders(64, md)[-1] == 1024
+    for two in (False, True):
+        t = make(dtype, 1, H, KV, dh, Lq, Lk, seed=3, nb=128 if two else 64, md=md)
+        kw = dict(bidirectional=two, causal=not two)
+        if Lq < Lk:
+            kw['q_pos'] = torch.tensor([Lk - Lq])
+        vals, bnds = reference(t, H, KV, dh, md=md, **kw)
+        compare(run(t, H, KV, md=md, **{n: dev(x) if torch.is_tensor(x) else x for n, x in kw.items()}), vals, bnds, str(two))
+
+
+@gpu
 @pytest.mark.parametrize('bidirectional', [True, False])
 @pytest.mark.parametrize('causal', [True, False])
 def test_positions_masks_and_directions(bidirectional, causal):
