@@ -1206,8 +1206,10 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // itself, stay in the state.  A rule of sizes alone, since it says what the state holds.  5760 rows (3740 counting) of width 512, 148
 // words, against the route through ekaid_gemm_f32 with its 13 launches: kernels 125 -> 71 us (16 rows a workgroup, bound by the latency of
 // the second-level cache and of three dependent stages, not by the f32 matrix rate: 5 of the 22 us of the logits, 12 of the gradients' 35).
+// Up to 2^30 products of a matrix, where the f32 matrix rate begins to weigh.  Whole calls, this against 257 words on the other route: 5760 x
+// 512 x 256 146 / 172 us, 3500 x 1024 x 256 142 / 170, 8000 x 512 x 256 162 / 166, 2000 x 2048 x 256 180 / 173, beyond it 16000 x 512 x 256 287 / 249.
 bool few_words(const ekaid_linear_loss_t* a) {
-    return a->dtype == EKAID_F32 && a->V <= 256 && ((a->V + 15) & ~15) <= a->D && a->D % 4 == 0 && (double)a->B * a->T * a->V * a->D < 2147483648.0;
+    return a->dtype == EKAID_F32 && a->V <= 256 && ((a->V + 15) & ~15) <= a->D && a->D % 4 == 0 && (double)a->B * a->T * a->V * a->D <= 1073741824.0;
 }
 size_t kept_offset(const ekaid_linear_loss_t* a) { return (256 + (size_t)a->B * a->T * 20 + 255) & ~size_t(255); }
 struct LossPlan {

@@ -737,7 +737,7 @@ int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_byte
  * nothing whatever x and target hold there (16-bit types leave them out of the products as well); a target outside [0, V) in a row that
  * counts makes the loss NaN.  All-zero mask: loss 0/0, gradients 0.
  * state (ekaid_linear_loss_state_bytes, 16-byte aligned) is written by fwd and read by bwd, which is given the same inputs.  dloss: device
- * scalar.  dx [B T][D], dweight [V][D], dbias [V] contiguous, any may be NULL.  f32: V <= 256, V (in whole sixteens) <= D, D % 4 == 0, N V D < 2^31 and 16-byte
+ * scalar.  dx [B T][D], dweight [V][D], dbias [V] contiguous, any may be NULL.  f32: V <= 256, V (in whole sixteens) <= D, D % 4 == 0, N V D <= 2^30 and 16-byte
  * aligned x, weight (dx then too) run on f32 matrix instructions and keep the logits in the state; otherwise the arithmetic `arith`: two
  * f16 terms with row scales for z and dx and the exact three bf16 terms for dweight (EKAID_GEMM_F16X2, N V D >= 2^31, D % 8 == 0 and
  * 16-byte aligned x, weight), else as ekaid_gemm_f32.  16-bit

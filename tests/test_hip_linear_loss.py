@@ -443,7 +443,8 @@ def test_few_words_state_and_alignment():
     wide = state(V=65)
     assert state() == state(x=(1 << 20) + 4, weight=0) == wide + 6 * 64 * 4
     assert state(V=64) == state() and state(V=16) == wide + 6 * 16 * 4 and state(V=256, D=256, ldx=256) == wide + 6 * 256 * 4
-    for kw in (dict(V=257, D=512, ldx=512), dict(D=62, V=20, ldx=62), dict(dtype=1), dict(B=1 << 14, T=1 << 7, D=1024, ldx=1024, V=1)):
+    for kw in (dict(V=257, D=512, ldx=512), dict(D=62, V=20, ldx=62), dict(dtype=1), dict(B=1 << 14, T=1 << 7, D=1024, ldx=1024, V=1),
+               dict(B=1 << 13, T=1 << 7, D=1028, ldx=1028, V=1)):
         n = max(kw.get('B', 2) * kw.get('T', 3), 6)
         assert state(**kw) <= 512 + 20 * n, kw
     assert L.ekaid_linear_loss_workspace_bytes(ctypes.byref(desc()), 0) == 0
