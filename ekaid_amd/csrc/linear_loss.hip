@@ -204,7 +204,8 @@ template <int PAIRS> __device__ __forceinline__ int pair_b(int i) { return PAIRS
 
 // acc[mi][ni] += sum over k in [64 kt0, 64 kt1) of A(m, k) B(n, k), for every pair of planes; BM x BN per workgroup, WM x WN per wave.  Two LDS buffers: the copies
 // of tile t + 1 are under way while tile t is multiplied; ONE barrier a tile, behind a wait for this wave's copies and LDS reads.
-template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int PAIRS> struct TileProduct {
+// TURN: the pairs in the order of the product with A and B exchanged, so that both give the same sums.
+template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int PAIRS, bool TURN = false> struct TileProduct {
     static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, NT = 64 * NW, MI = WM / 32, NI = WN / 32, STAGES = BM == 128 ? 4 : 2;
     typedef Operand<BM, ACOL, NW> A;
     typedef Operand<BN, BCOL, NW> B;
@@ -246,8 +247,8 @@ template <typename T, int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int 
         if (kt0 < kt1) {
             int kt = kt0, pair = 0;                         // of the tile copied next
             auto copy = [&](char* la, char* lb) __attribute__((always_inline)) {
-                oa.issue(la, kt, pair_a<PAIRS>(pair), K, wave);
-                ob.issue(lb, kt, pair_b<PAIRS>(pair), K, wave);
+                oa.issue(la, kt, TURN ? pair_b<PAIRS>(pair) : pair_a<PAIRS>(pair), K, wave);
+                ob.issue(lb, kt, TURN ? pair_a<PAIRS>(pair) : pair_b<PAIRS>(pair), K, wave);
                 if (++kt == kt1) { kt = kt0; ++pair; }
             };
             const int total = PAIRS * (kt1 - kt0);
@@ -402,7 +403,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_stats_kernel(co
                 if (F32) s4 = *reinterpret_cast<const f32x4*>(scale + ml) * sx;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = acc[i][j][4 * q + e] * s4[e] + b4[e];
+                    const float z = fmaf(acc[i][j][4 * q + e], s4[e], b4[e]);
                     acc[i][j][4 * q + e] = z;
                     mx = fmaxf(mx, z);
                     tz = ml + e == tl ? z : tz;
@@ -537,7 +538,7 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NI], Bits bit
 // backward of the logits of one piece: lanes = words, registers = rows
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const LossArgs a) {
-    typedef TileProduct<typename Term<T>::type, BM, BN, WM, WN, false, false, Term<T>::pairs> P;
+    typedef TileProduct<typename Term<T>::type, BM, BN, WM, WN, false, false, Term<T>::pairs, true> P;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int NP = Term<T>::planes;
     LL_LDS(BM, BN);
@@ -589,7 +590,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
             for (int j = 0; j < P::NI; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] * (F32 ? s4[e] * wscale[j] : LOG2E) + (bias[j] - l4[e]));
+                    // (f32: the logit rounded as in the forward, so that p is what its denominator holds of it)
+                    const float x = acc[i][j][4 * q + e];
+                    const float p = __builtin_amdgcn_exp2f(F32 ? fmaf(x, s4[e] * wscale[j], bias[j]) - l4[e] : x * LOG2E + (bias[j] - l4[e]));
                     const float dz = w4[e] == 0.f ? 0.f : (p - (t4[e] == word[j] ? 1.f : 0.f)) * w4[e];
                     acc[i][j][4 * q + e] = dz;
                     sum[j] += dz;
@@ -613,15 +616,18 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
         store_tile<BM, BN, WM, WN, P::MI, P::NI, P::NT>(acc, [&](float v) { return to_bits<T>(v * DzScale<T>::up); }, a.dz + (long long)m0 * a.ldz + wt * BN, a.ldz, BM,
                                                         cols, la0, la1, lb0, lb1, tid, wave, lane);
     } else {
-        // Two f16 terms of dz times the weight's scale for dx.  |dz| <= (1 - p_target) |mask| in a row: brought to 2^13 against the largest
-        // weight scale, so that a row decided by one word keeps its small values.  Then three bf16 terms of dz for dW.  The values are
-        // scaled and unscaled by powers of two in place, and hidden from the optimizer between the passes: it would keep every
-        // conversion of one pass for the next and spill.
+        // Two f16 terms of dz times the weight's scale for dx.  |dz| <= (1 - p_target) |mask| in a row, as far as the rounding of lse (half a
+        // unit of |lse| in every p of the row) and of its logarithm lets p sum to one; and |dz| <= |mask|, as no logit is above lse.  That bound
+        // is brought to [2^12, 2^13) against the largest weight scale, so that a row decided by one word keeps its small values.  It holds
+        // because the logits are the forward's bit for bit; should a matrix unit add in another order for exchanged operands, a value past it
+        // is rounding error alone, and is held at the largest f16 (NaN stays NaN).  Then three bf16 terms of dz for dW.  The values are scaled
+        // and unscaled by powers of two in place, and hidden from the optimizer between the passes: it would keep every conversion of one
+        // pass for the next and spill.
         const float wtop = a.st.sums[2];
         for (int i = tid; i < BM; i += P::NT) {
             float u = 0.f;
             if (m0 + i < count) {
-                const float miss = fmaxf(1.f - __builtin_amdgcn_exp2f(a.st.tz[m0 + i] - slse[i]), 0x1p-24f);
+                const float miss = fmaxf(1.f - __builtin_amdgcn_exp2f(a.st.tz[m0 + i] - slse[i]), 0.f) + fmaf(fabsf(slse[i]), 0x1p-24f, 0x1p-21f);
                 int e;
                 (void)frexpf(fminf(miss, 1.f) * wtop * fabsf(sw[i]), &e);
                 u = ldexpf(1.f, max(min(13 - e, 120), -120));
@@ -655,7 +661,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
         unsigned short* b16 = a.dzb + (long long)m0 * 3 * a.ldz + wt * BN;
         const auto bf = [](float v) { return to_bits<__bf16>(v); };
         const auto rest = [](float v, float, float) { return v - (float)(__bf16)v; };
-        each([](float v, float u, float w) { return v * (u * w); });
+        each([](float v, float u, float w) {
+            const float x = v * (u * w);
+            return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
+        });
         put([](float v) { return to_bits<_Float16>(v); }, f16, 2ll * a.ldz);
         each([](float v, float, float) { return v; });
         put([](float v) { return to_bits<_Float16>(v - (float)(_Float16)v); }, f16 + a.ldz, 2ll * a.ldz);

@@ -451,3 +451,37 @@ def test_few_words_state_and_alignment():
     for kw in (dict(state=(1 << 20) + 8), dict(dx=(1 << 20) + 4)):
         assert L.ekaid_linear_loss_bwd(ctypes.byref(desc(**kw)), 1 << 20, 1 << 40, None) < 0 and 'aligned' in hip.last_error(), kw
     assert L.ekaid_linear_loss_fwd(ctypes.byref(desc(state=(1 << 20) + 8)), 1 << 20, 1 << 40, None) < 0
+
+
+@gpu
+@pytest.mark.parametrize('offset', [0.0, 40.0, -3000.0])
+@pytest.mark.parametrize('V', [6001, 10007], ids=['128-tiles', '256-tiles'])
+def test_f32_rows_decided_by_their_own_target(V, offset):
+    """Well predicted words, target logits of 20 to 90 above a common offset: what is left of 1 - p is the rounding of the logits, and
+    every gradient keeps its bound.  (N V D above 2^31: the route of two f16 terms.)"""
+    B, T, D = 8, 128, 512
+    t = make(F32, B, T, D, V)
+    height = torch.linspace(20, 90, B * T, device=DEV).view(B, T, 1)
+    t['mask'][:] = 1
+    t['mask'][3, 50:] = 0.25
+    w = t['weight'][t['target']]
+    t['x'] = w * (height / (w * w).sum(2, keepdim=True))
+    t['bias'] = t['bias'] * 0.1 + offset
+    assert B * T * V * D >= 1 << 31
+    want = reference(t)
+    compare(run(t), want)
+    t['x'][0, 5:9] *= -1                                          # some of them predicted as badly
+    compare(run(t), reference(t), 'mixed')
+
+
+@gpu
+def test_f32_rows_decided_against_large_cancelling_bias():
+    """Logits that are the small difference of a large bias and a large product: their error is that of the large parts, no gradient overflows."""
+    B, T, D, V = 8, 128, 512, 6001
+    t = make(F32, B, T, D, V)
+    t['mask'][:] = 1
+    w = t['weight'][t['target']]
+    t['x'] = w * (60.0 / (w * w).sum(2, keepdim=True))
+    t['x'][..., 0], t['weight'][:, 0] = 64.0, -64.0                # -4096 in every logit
+    t['bias'] = t['bias'] * 0.1 + 4096.0
+    compare(run(t), reference(t))
