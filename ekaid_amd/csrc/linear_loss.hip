@@ -824,6 +824,7 @@ template <typename T> __global__ __launch_bounds__(1024) void ll_db_kernel(const
 
 // ---- f32 operands as 16-bit terms.  One wave a row: the compact rows of x (zeros behind them to a multiple of 256), then the rows of the
 // weight.  f16: the row times a power of two that brings its largest magnitude to [2^13, 2^14), in two terms; its inverse in sx / sw.
+// (rows below 2^-107 are brought less far; the largest finite row takes 2^-114)
 __global__ __launch_bounds__(256) void ll_terms_kernel(const LossArgs a, unsigned short* xp, unsigned short* xb, unsigned short* wp, float* sx, float* sw, int nx) {
     const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), D = a.d.D, count = a.st.count[0], rows = (count + 255) & ~255;
     const bool of_x = r < nx;
@@ -840,7 +841,7 @@ __global__ __launch_bounds__(256) void ll_terms_kernel(const LossArgs a, unsigne
     mx = wave_max(mx);
     int e = 0;
     if (mx > 0.f && mx < __builtin_inff()) (void)frexpf(mx, &e);
-    e = max(min(14 - e, 120), -100);
+    e = min(14 - e, 120);
     const float s = ldexpf(1.f, e);
     if (lane == 0) (of_x ? sx[r] : sw[v]) = ldexpf(1.f, -e);
     unsigned short* out = of_x ? xp + (long long)r * 2 * D : wp + (long long)v * 2 * D;

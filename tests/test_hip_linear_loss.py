@@ -485,3 +485,13 @@ def test_f32_rows_decided_against_large_cancelling_bias():
     t['x'][..., 0], t['weight'][:, 0] = 64.0, -64.0                # -4096 in every logit
     t['bias'] = t['bias'] * 0.1 + 4096.0
     compare(run(t), reference(t))
+
+
+@gpu
+def test_f32_terms_of_the_largest_magnitudes():
+    """A row of x near the end of f32's range: its logits are finite, and so is everything else (N V D above 2^31)."""
+    t = make(F32, 4, 256, 256, 8200)
+    t['mask'][:] = 1
+    t['mask'][1, :100] = 0
+    t['x'][2, 7] *= 2.0 ** 120
+    compare(run(t), reference(t))
