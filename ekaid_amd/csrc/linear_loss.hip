@@ -662,13 +662,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ll_dz_kernel(const
         const auto bf = [](float v) { return to_bits<__bf16>(v); };
         const auto rest = [](float v, float, float) { return v - (float)(__bf16)v; };
         each([](float v, float u, float w) {
-            const float x = v * (u * w);
+            const float x = v * fmaxf(u * w, 0x1p-60f);       // (so far below f16 it is nothing there, but dW takes v back)
             return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
         });
         put([](float v) { return to_bits<_Float16>(v); }, f16, 2ll * a.ldz);
         each([](float v, float, float) { return v; });
         put([](float v) { return to_bits<_Float16>(v - (float)(_Float16)v); }, f16 + a.ldz, 2ll * a.ldz);
-        each([](float v, float u, float w) { return u == 0.f ? 0.f : v * (1.f / (u * w)); });
+        each([](float v, float u, float w) { return v * (1.f / fmaxf(u * w, 0x1p-60f)); });
         put(bf, b16, 3ll * a.ldz);
         each(rest);
         put(bf, b16 + a.ldz, 3ll * a.ldz);

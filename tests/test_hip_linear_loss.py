@@ -495,3 +495,22 @@ def test_f32_terms_of_the_largest_magnitudes():
     t['mask'][1, :100] = 0
     t['x'][2, 7] *= 2.0 ** 120
     compare(run(t), reference(t))
+
+
+@gpu
+def test_f32_words_of_a_hundred_powers_of_ten():
+    """Words of 2^90 and 2^-100 of the usual size beside the others: their gradients come out as every other word's (N V D above 2^31)."""
+    t = make(F32, 4, 256, 256, 8200)
+    t['mask'][:] = 1
+    t['weight'][5] *= 2.0 ** 90
+    t['weight'][9] *= 2.0 ** -100
+    t['target'][t['target'] == 5] = 6
+    got, want = run(t), reference(t)
+    compare(got, want)
+    # the largest word's bound hides the others': for the tiny word, where the largest takes no part (its logit far below), by hand
+    x, w, u = t['x'].double().view(-1, 256), t['weight'].double(), 2.0 ** -24
+    z = x @ w.t() + t['bias'].double()
+    p = torch.softmax(z, 1)[:, 9:10]
+    S = float((x.abs() @ torch.cat((w[:5], w[6:])).abs().t()).max())
+    rel = 2 * ((256 + 8) * u + 2.0 ** -21) * S + (300 + 8200 / 64) * u + 8 * u * (1 + S) + (1024 + 8) * u + 2.0 ** -21
+    assert bool(((got[2][9].double() - want[0][2][9]).abs() <= rel * (p * x.abs()).sum(0) / 1024 + 2.0 ** -23 * want[0][2][9].abs()).all())
