@@ -63,7 +63,11 @@ DeviceState& device_state() {
     }
     return s;
 }
+static thread_local int t_gemm_mode = -1;         // of the products this thread issues inside a GemmModeScope
+GemmModeScope::GemmModeScope(int mode) : outer(t_gemm_mode) { t_gemm_mode = mode; }
+GemmModeScope::~GemmModeScope() { t_gemm_mode = outer; }
 int gemm_mode() {
+    if (t_gemm_mode >= 0) return t_gemm_mode;
     DeviceState& s = device_state();
     int m = s.gemm_mode.load();
     if (m < 0) { m = default_gemm_mode(); s.gemm_mode.store(m); }

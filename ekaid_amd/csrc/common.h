@@ -19,7 +19,14 @@ int check_launch(const char* what);
 // per-device state (api.hip): created by ekaid_init(device) or on first use of a device; no other mutable globals
 struct DeviceState;
 DeviceState& device_state();                       // of the calling thread's current HIP device
-int gemm_mode();                                   // 0 = f32 MFMA, 1 = exact bf16 split (per device)
+int gemm_mode();                                   // 0 = f32 MFMA, 1 = exact bf16 split, 2 = two-term f16 split (per device)
+struct GemmModeScope {                             // the calling thread's products run in `mode` while this lives, whatever the device's mode
+    explicit GemmModeScope(int mode);
+    ~GemmModeScope();
+    GemmModeScope(const GemmModeScope&) = delete;
+    GemmModeScope& operator=(const GemmModeScope&) = delete;
+    int outer;
+};
 int set_gemm_mode(int mode);
 int seq_mode();                                    // 0 = step-wise sequence chains, 1 = persistent sequence kernels where supported (per device)
 #ifndef EKAID_GEMM_MODE_DEFAULT

@@ -1202,6 +1202,7 @@ int ll_check(const ekaid_linear_loss_t* a, const char* who) {
         set_error("%s: bad sizes B=%d T=%d D=%d V=%d", who, a->B, a->T, a->D, a->V);
         return EKAID_ERR_ARG;
     }
+    if (a->dtype == EKAID_F32 && (a->arith < EKAID_GEMM_F32_MFMA || a->arith > EKAID_GEMM_F16X2)) { set_error("%s: arithmetic %d", who, a->arith); return EKAID_ERR_ARG; }
     const int al = a->dtype == EKAID_F32 ? 4 : 16;
     if ((uintptr_t)a->state & 15) { set_error("%s: the state must be 16-byte aligned", who); return EKAID_ERR_ARG; }
     if (a->dtype != EKAID_F32 && (a->D % 8 || a->ldx % 8)) { set_error("%s: width %d / row stride %lld must be multiples of 8", who, a->D, a->ldx); return EKAID_ERR_UNSUPPORTED; }
@@ -1238,7 +1239,7 @@ struct LossPlan {
     int bounds;
 };
 bool f32_bounds(const ekaid_linear_loss_t* a, long long n, int vp) {
-    return gemm_mode() == EKAID_GEMM_F16X2 && (double)n * vp * a->D >= 6e9 && a->D % 4 == 0 && a->ldx % 4 == 0 && std::min({(long long)a->D, n, (long long)vp}) >= 32 &&
+    return a->arith == EKAID_GEMM_F16X2 && (double)n * vp * a->D >= 6e9 && a->D % 4 == 0 && a->ldx % 4 == 0 && std::min({(long long)a->D, n, (long long)vp}) >= 32 &&
            !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
 }
 ekaid_gemm_t product(const float* A, const float* B, float* C, int M, int N, int K, int lda, int ldb, int ldc, int tA, int tB) {
@@ -1495,12 +1496,14 @@ extern "C" size_t ekaid_linear_loss_state_bytes(const ekaid_linear_loss_t* a) {
 }
 extern "C" size_t ekaid_linear_loss_workspace_bytes(const ekaid_linear_loss_t* a, int backward) {
     if (ekaid::ll_check(a, "linear_loss_workspace_bytes")) return 0;
+    const ekaid::GemmModeScope mode(a->arith);             // (what ekaid_gemm_f32 needs depends on it)
     return ekaid::loss_plan(a, backward).total;
 }
 extern "C" int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace ekaid;
     if (int rc = ll_check(a, "linear_loss_fwd")) return rc;
     if (!a->loss || !a->state || !a->weight || (a->B * (long long)a->T && (!a->x || !a->target || !a->mask))) { set_error("linear_loss_fwd: null operand"); return EKAID_ERR_ARG; }
+    const GemmModeScope mode(a->arith);
     const LossPlan p = loss_plan(a, 0);
     if (workspace_bytes < p.total || (p.total && !workspace)) { set_error("linear_loss_fwd: workspace of %zu bytes needed", p.total); return EKAID_ERR_ARG; }
     hipStream_t s = (hipStream_t)stream;
@@ -1524,6 +1527,7 @@ extern "C" int ekaid_linear_loss_fwd(const ekaid_linear_loss_t* a, void* workspa
 extern "C" int ekaid_linear_loss_bwd(const ekaid_linear_loss_t* a, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace ekaid;
     if (int rc = ll_check(a, "linear_loss_bwd")) return rc;
+    const GemmModeScope mode(a->arith);                    // (the forward's, whatever the device's mode has become)
     const LossPlan p = loss_plan(a, 1);
     if (p.n == 0) { set_error("linear_loss_bwd: no rows (the caller zeroes the gradients)"); return EKAID_ERR_ARG; }
     if (!a->dloss || !a->state || !a->x || !a->weight || !a->target || !a->mask) { set_error("linear_loss_bwd: null operand"); return EKAID_ERR_ARG; }

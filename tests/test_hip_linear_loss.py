@@ -514,3 +514,38 @@ def test_f32_words_of_a_hundred_powers_of_ten():
     S = float((x.abs() @ torch.cat((w[:5], w[6:])).abs().t()).max())
     rel = 2 * ((256 + 8) * u + 2.0 ** -21) * S + (300 + 8200 / 64) * u + 8 * u * (1 + S) + (1024 + 8) * u + 2.0 ** -21
     assert bool(((got[2][9].double() - want[0][2][9]).abs() <= rel * (p * x.abs()).sum(0) / 1024 + 2.0 ** -23 * want[0][2][9].abs()).all())
+
+
+@gpu
+@pytest.mark.parametrize('shape', [(2, 21, 37, 203), (3, 50, 64, 300), (8, 256, 516, 6001)], ids=str)
+@pytest.mark.parametrize('first,then', [(0, 1), (1, 0), (2, 0), (1, 2)])
+def test_f32_arithmetic_is_the_forwards(first, then, shape):
+    """The mode is changed between the forward and its backward: the backward stays with the arithmetic its denominators came from."""
+    from ekaid_amd import ops
+    t = make(F32, *shape)
+    leaves = [t[n].detach().requires_grad_(True) for n in ('x', 'weight', 'bias')]
+    old, res = ops.get_gemm_mode(), []
+    try:
+        for later in (first, then):
+            ops.set_gemm_mode(first)
+            loss = ops.linear_lm_loss(*leaves, t['target'], t['mask'])
+            ops.set_gemm_mode(later)
+            res.append([loss.detach()] + list(torch.autograd.grad(loss, leaves)))
+            assert ops.get_gemm_mode() == later
+    finally:
+        ops.set_gemm_mode(old)
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_c_entry_refuses_unknown_arithmetics():
+    from ekaid_amd import hip
+    L = hip.load()
+    d = hip.LinearLoss()
+    for n in ('x', 'weight', 'target', 'mask', 'loss', 'state', 'dloss', 'dx', 'dweight'):
+        setattr(d, n, 1 << 20)
+    d.dtype, d.B, d.T, d.D, d.V, d.ldx, d.ld_target, d.ld_mask = 0, 2, 3, 64, 500, 64, 3, 3
+    for arith in (-1, 3, 7):
+        d.arith = arith
+        for entry in (L.ekaid_linear_loss_fwd, L.ekaid_linear_loss_bwd):
+            assert entry(ctypes.byref(d), 1 << 20, 1 << 40, None) < 0 and 'arithmetic' in hip.last_error()
+        assert L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 1) == 0
