@@ -1893,7 +1893,8 @@ class LinearLossFn(Function):
     def forward(ctx, x, weight, bias, target, mask, denom):
         shape = x.shape
         x2, ld = _rows2d(x)
-        if x2.numel() and (ld * x2.element_size() % 16 or x2.data_ptr() % 16):          # whole 16-byte vectors, else a copy
+        if x2.numel() and shape[2] * x2.element_size() % 16 == 0 and (ld * x2.element_size() % 16 or x2.data_ptr() % 16):
+            # rows of whole 16-byte vectors that do not lie at such (another width lies at none in a copy either)
             x2, ld = x2.clone(memory_format=torch.contiguous_format), shape[2]
         weight, bias = _c(weight), (None if bias is None else _c(bias))
         if weight.data_ptr() % 16:

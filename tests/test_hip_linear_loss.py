@@ -549,3 +549,16 @@ def test_c_entry_refuses_unknown_arithmetics():
         for entry in (L.ekaid_linear_loss_fwd, L.ekaid_linear_loss_bwd):
             assert entry(ctypes.byref(d), 1 << 20, 1 << 40, None) < 0 and 'arithmetic' in hip.last_error()
         assert L.ekaid_linear_loss_workspace_bytes(ctypes.byref(d), 1) == 0
+
+
+@gpu
+def test_operands_are_copied_only_where_it_helps():
+    """A width of no whole vectors has no aligned rows to copy to: x is kept as it is.  Rows that a copy aligns are copied."""
+    from ekaid_amd import ops
+    t = make(F32, 2, 9, 37, 300)
+    for x, kept in ((t['x'], True), (make(F32, 2, 9, 40, 300)['x'], True), (torch.randn(2 * 9 * 37 + 1, device=DEV)[1:].view(2, 9, 37), True), (torch.randn(2, 9, 41, device=DEV)[..., :40], False),
+                    (torch.randn(2 * 9 * 40 + 1, device=DEV)[1:].view(2, 9, 40), False)):
+        w = torch.randn(300, x.shape[2], device=DEV, requires_grad=True)
+        loss = ops.linear_lm_loss(x, w, None, t['target'], t['mask'])
+        assert (loss.grad_fn.saved_tensors[0].data_ptr() == x.data_ptr()) == kept
+        assert torch.equal(loss.detach(), ops.linear_lm_loss(x.clone(memory_format=torch.contiguous_format), w, None, t['target'], t['mask']).detach())
