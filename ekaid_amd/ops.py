@@ -12,7 +12,7 @@ import math
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import hip
@@ -2432,7 +2432,8 @@ def _attention(what, q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, ca
     p = float(p) if training else 0.0
     cfg = (heads, kv_heads, None if k_len is None else _c(k_len), key_mask, None if q_pos is None else _c(q_pos), bool(causal), bool(bidirectional),
            int(max_distance), scale, p, next_seed() if p > 0.0 else 0)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad))
+            or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, table))):        # (tangents: the node refuses them)
         out = AttentionFn.apply(q, k, v, table, cfg)
     else:
         out = AttentionFn.launch(q, k, v, table, cfg, False)[0]

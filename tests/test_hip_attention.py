@@ -521,3 +521,21 @@ def test_c_entry_refuses_bad_descriptors():
         assert L.ekaid_attn_bwd(ctypes.byref(d), 1 << 20, 1 << 40, None) < 0
     assert L.ekaid_attn_fwd(None, None, 0, None) < 0
     assert ctypes.sizeof(hip.Attn) > 0
+
+
+@gpu
+def test_forward_mode_derivatives_are_errors():
+    """An operand that carries a tangent: refused, as every operator without a forward derivative does, not a result that has lost it."""
+    import torch.autograd.forward_ad as fw
+    from ekaid_amd import ops
+    q, k, v, tab = (torch.randn(*s, device=DEV) for s in ((1, 4, 16), (1, 6, 16), (1, 6, 16), (4, 1)))
+    want = ops.relative_attention(q, k, v, tab, 1, max_distance=9)
+    with fw.dual_level():
+        for i in range(4):
+            a = [fw.make_dual(x, torch.ones_like(x)) if i == n else x for n, x in enumerate((q, k, v, tab))]
+            with pytest.raises(NotImplementedError):
+                ops.relative_attention(*a, 1, max_distance=9)
+            if i < 3:
+                with pytest.raises(NotImplementedError):
+                    ops.cross_attention(*a[:3], 1)
+        assert torch.equal(ops.relative_attention(q, k, v, tab, 1, max_distance=9), want)
