@@ -9,6 +9,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import numbers
 import os
 
 import torch
@@ -2425,7 +2426,7 @@ def _attention(what, q, k, v, table, heads, kv_heads, k_len, key_mask, q_pos, ca
         side = table.shape[0] // 2 if bidirectional else table.shape[0]
         if not 2 <= side <= 128:
             refuse('2 to 128 buckets a direction (got %d)', side)
-        if int(max_distance) != max_distance or max_distance <= side // 2:
+        if not isinstance(max_distance, numbers.Real) or not math.isfinite(max_distance) or int(max_distance) != max_distance or max_distance <= side // 2:
             refuse('max_distance %r must exceed the %d exact buckets', max_distance, side // 2)
         if relative_borders(side, int(max_distance))[-1] > _ATTN_MAX_REACH:
             refuse('the last bucket must begin within %d positions', _ATTN_MAX_REACH)

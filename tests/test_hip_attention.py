@@ -539,3 +539,16 @@ def test_forward_mode_derivatives_are_errors():
                 with pytest.raises(NotImplementedError):
                     ops.cross_attention(*a[:3], 1)
         assert torch.equal(ops.relative_attention(q, k, v, tab, 1, max_distance=9), want)
+
+
+@gpu
+def test_max_distance_that_is_no_whole_number_is_refused():
+    from ekaid_amd import ops
+    from ekaid_amd.hip import EkaidError
+    q, k, tab = torch.zeros(2, 3, 64, device=DEV), torch.zeros(2, 5, 64, device=DEV), torch.zeros(8, 2, device=DEV)
+    for md in (math.inf, -math.inf, math.nan, 9.5, None, '9'):
+        with pytest.raises(EkaidError):
+            ops.relative_attention(q, k, k, tab, 2, max_distance=md)
+    import numpy as np
+    assert torch.equal(ops.relative_attention(q, k, k, tab, 2, max_distance=np.int64(9)), ops.relative_attention(q, k, k, tab, 2, max_distance=9))
+    assert torch.equal(ops.relative_attention(q, k, k, tab, 2, max_distance=9.0), ops.relative_attention(q, k, k, tab, 2, max_distance=9))
