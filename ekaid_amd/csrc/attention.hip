@@ -285,15 +285,15 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     for (int mt = 0; mt < MT; ++mt) o[mt] = zero_acc<G>();
     float m = NEG_INF, l = 0.f;
     if (t0 < t1) {
-        ck.issue(k0, t0 * KT, len, d.dh, ring.tile(t0), wave);
-        cv.issue(v0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+        ck.issue(k0, t0 * KT, kend, d.dh, ring.tile(t0), wave);
+        cv.issue(v0, t0 * KT, kend, d.dh, ring.tile(t0), wave);
     }
     auto tile = [&](int t, const T* ks, const T* vs, T* kn, T* vn) __attribute__((always_inline)) {
         settle();
         ring.step(t);
         if (t + 1 < t1) {
-            ck.issue(kn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
-            cv.issue(vn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+            ck.issue(kn, (t + 1) * KT, kend, d.dh, ring.tile(t + 1), wave);
+            cv.issue(vn, (t + 1) * KT, kend, d.dh, ring.tile(t + 1), wave);
         }
         if (!live || (d.causal && t * KT > pmax)) return;
         if constexpr (DH * sizeof(T) > 128) tf.refresh();

@@ -79,8 +79,8 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
         for (int e = 0; e < Elem<T>::epl; ++e) n2 += elem<T>(gf[c], e) * elem<T>(gf[c], e);
     }
     if (t0 < t1) {
-        ck.issue(k0, t0 * KT, len, d.dh, ring.tile(t0), wave);
-        cv.issue(v0, t0 * KT, len, d.dh, ring.tile(t0), wave);
+        ck.issue(k0, t0 * KT, kend, d.dh, ring.tile(t0), wave);
+        cv.issue(v0, t0 * KT, kend, d.dh, ring.tile(t0), wave);
     }
     delta = across_groups_sum<G>(delta);
     n2 = across_groups_sum<G>(n2);
@@ -146,8 +146,8 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
         settle();
         ring.step(t);
         if (t + 1 < t1) {
-            ck.issue(kn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
-            cv.issue(vn, (t + 1) * KT, len, d.dh, ring.tile(t + 1), wave);
+            ck.issue(kn, (t + 1) * KT, kend, d.dh, ring.tile(t + 1), wave);
+            cv.issue(vn, (t + 1) * KT, kend, d.dh, ring.tile(t + 1), wave);
         }
         const unsigned char* km = ring.tile(t);
 #pragma unroll
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
     const int b = bk % d.B, kvh = bk / d.B, group = d.H / d.KV;
     const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tl * NW * G, jw = j0 + wave * G, j = jw + lane % G;
     const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
-    const bool ok = j < len && (!mask || mask[j]), live = jw < len;
+    const bool ok = j < len && (!d.causal || j - d.Lq < p0) && (!mask || mask[j]), live = jw < len;      // (causal: some row may attend it)
     const int qtiles = (d.Lq + QT - 1) / QT, first = d.causal ? min(qtiles, max(0, j0 - p0) / QT) : 0, run = qtiles - first;
     const int items = j0 < len ? group * run : 0, per = (items + a.splits - 1) / a.splits, t0 = split * per, t1 = min(items, t0 + per);
 

@@ -130,7 +130,8 @@ template <typename T, int G> __device__ __forceinline__ u32x4 row_frag_global(co
 // in groups of lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31: with blocks of 16 rows, where lanes 16 on read the next slot, rows whose
 // swz() differ by 1 must lie in one group (dk / dv of 128-wide 16-bit heads: 2 extra cycles of every 8 otherwise).  The permutation is
 // applied to the global
-// address.  Rows that do not exist or are masked, and columns beyond dh, are read from a zero vector: NaN or Inf there never arrives.
+// address.  Rows that do not exist, are masked or (causal) lie behind the last position of the workgroup, and columns beyond dh, are read
+// from a zero vector: NaN or Inf there never arrives.
 __device__ __attribute__((aligned(16))) const uint32_t attn_zero16[4] = {0u, 0u, 0u, 0u};
 typedef __attribute__((address_space(3))) void* lds_void;
 typedef const __attribute__((address_space(1))) void* global_void;

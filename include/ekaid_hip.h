@@ -676,7 +676,8 @@ long long ekaid_launch_count(int which);
  * Attention of query rows to the states of another length, with shared keys, ragged lengths and a learned relative position bias.
  *   s[i][j] = scale <q_i, k_j> (+ table[bucket(j - (q_pos + i))][head]),   o_i = sum_j softmax_j(s[i][:]) v_j
  * over the keys j < k_len[b] with key_mask[b][j] != 0 (causal: also j <= q_pos + i).  A row without any such key gives o = 0 and
- * gradients 0.  Masked key and value rows are never read into a product (NaN there stays there).  Scores are never stored.
+ * gradients 0.  Masked key and value rows, and (causal) those behind the last row's position, are never read into a product (NaN there
+ * stays there; a key that some row attends meets the rows before it with the weight 0, so NaN in it reaches them).  Scores are never stored.
  * q [B][Lq][H dh], k and v [B][Lk][KV dh]: strides between samples and rows in elements, heads dh apart, all 16-byte aligned;
  * out, dout, dq [B][Lq][H dh] and dk, dv [B][Lk][KV dh] contiguous.  H % KV == 0, dh % 8 == 0, dh <= 256.  dtype: EKAID_F32 / BF16 / F16
  * of every tensor but lse, table; products accumulate and softmax statistics are held in f32; probabilities and score gradients are

@@ -552,3 +552,22 @@ def test_max_distance_that_is_no_whole_number_is_refused():
     import numpy as np
     assert torch.equal(ops.relative_attention(q, k, k, tab, 2, max_distance=np.int64(9)), ops.relative_attention(q, k, k, tab, 2, max_distance=9))
     assert torch.equal(ops.relative_attention(q, k, k, tab, 2, max_distance=9.0), ops.relative_attention(q, k, k, tab, 2, max_distance=9))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('Lq', [1, 16, 17, 70, 130])
+def test_causal_rows_read_nothing_behind_the_last_position(Lq, dtype):
+    """A chunk of rows over a cache without lengths: what stands behind the last row's position (NaN, Inf) reaches no result."""
+    B, H, KV, dh, Lk = 2, 4, 2, 64, 300
+    t = make(dtype, B, H, KV, dh, Lq, Lk, nb=16)
+    q_pos = torch.tensor([3, 141])
+    behind = torch.arange(Lk)[None] >= (q_pos + Lq)[:, None]
+    res = []
+    for kx, vx in ((0.0, 0.0), (float('nan'), float('nan')), (1.0, float('inf'))):
+        t['k'][behind], t['v'][behind] = kx, vx
+        res.append(run(t, H, KV, md=30, causal=True, q_pos=dev(q_pos)))
+    for other in res[1:]:
+        for n, a, b in zip(('out', 'dq', 'dk', 'dv', 'dtable'), res[0], other):
+            assert torch.equal(a, b), n
+    assert (res[0][2][behind] == 0).all() and (res[0][3][behind] == 0).all()
