@@ -290,18 +290,24 @@ __device__ __forceinline__ float table_at(const ekaid_attn_t& d, int bucket, int
     if (d.table_dtype == EKAID_BF16) return (float)reinterpret_cast<const __bf16*>(d.table)[i];
     return (float)reinterpret_cast<const _Float16*>(d.table)[i];
 }
-// bias of `heads` heads by distance, in units of the power-of-two softmax: bias[h][rel + reach], rel in [-reach, reach]
+// in units of the power-of-two softmax.  An entry of -6e4 or less closes its distances like -inf: a row that meets nothing else would have
+// such a number as its maximum and denominator, where f32 has no room left for the scores and for the logarithm of the sum.
+__device__ __forceinline__ float bias_at(const ekaid_attn_t& d, int rel, int head) {
+    const float t = table_at(d, rel_bucket(d, rel), head);
+    return t <= EKAID_ATTN_CLOSED ? NEG_INF : t * LOG2E;
+}
+// bias of `heads` heads by distance: bias[h][rel + reach], rel in [-reach, reach]
 __device__ __forceinline__ void fill_bias(const ekaid_attn_t& d, float* bias, int head0, int heads, int tid, int nt) {
     const int w = 2 * d.reach + 1;
-    for (int i = tid; i < heads * w; i += nt) bias[i] = table_at(d, rel_bucket(d, i % w - d.reach), head0 + i / w) * LOG2E;
+    for (int i = tid; i < heads * w; i += nt) bias[i] = bias_at(d, i % w - d.reach, head0 + i / w);
 }
 
 // the same for one head, padded, and only the distances `lo` .. `hi` a workgroup meets (and the two of everything beyond the reach)
 __device__ __forceinline__ void fill_bias_range(const ekaid_attn_t& d, float* bias, int head, int lo, int hi, int tid, int nt) {
     lo = max(lo, -d.reach - BIAS_PAD);
     hi = min(hi, d.reach + BIAS_PAD);
-    for (int rel = lo + tid; rel <= hi; rel += nt) bias[rel + d.reach + BIAS_PAD] = table_at(d, rel_bucket(d, min(max(rel, -d.reach), d.reach)), head) * LOG2E;
-    if (tid < 2) bias[BIAS_PAD + tid * 2 * d.reach] = table_at(d, rel_bucket(d, tid ? d.reach : -d.reach), head) * LOG2E;
+    for (int rel = lo + tid; rel <= hi; rel += nt) bias[rel + d.reach + BIAS_PAD] = bias_at(d, min(max(rel, -d.reach), d.reach), head);
+    if (tid < 2) bias[BIAS_PAD + tid * 2 * d.reach] = bias_at(d, tid ? d.reach : -d.reach, head);
 }
 
 // which workgroup works on what: consecutive work items (tiles of one head, which share their keys) on ONE die -- workgroups are dealt

@@ -2458,7 +2458,8 @@ def relative_attention(q, k, v, table, heads, kv_heads=None, k_len=None, key_mas
     (``q_pos`` (B,) int32 / int64, default 0: a new token of a cache passes its position).  ``causal``: j <= pos_i only.  ``table``
     (buckets, heads), float32 or q's type; ``bidirectional`` (default: not causal) gives half the buckets to j > pos_i, otherwise those
     share bucket 0.  Per direction the nearest half of the buckets hold one distance each, the others share the distances up to
-    ``max_distance`` by logarithm (``relative_borders``), the last takes everything beyond.  The bias is never a (heads, Lq, Lk) tensor;
+    ``max_distance`` by logarithm (``relative_borders``), the last takes everything beyond.  An entry of -6e4 or less (-inf, the lowest value
+    of any type) closes its distances: their keys are not attended.  The bias is never a (heads, Lq, Lk) tensor;
     its gradient is summed in float32 in a fixed order."""
     if table is None:
         raise hip.EkaidError('relative_attention: table is required')

@@ -685,7 +685,8 @@ long long ekaid_launch_count(int which);
  * ((b H + h) Lq + i) Lk + j.
  * Relative bias (table != NULL): table [buckets][H]; bucket of a distance = number of `border` entries <= distance (n_border of them,
  * not descending); distances: |j - pos| with the upper half of the buckets for j > pos (bidirectional), else max(pos - j, 0).  reach >= 1 and
- * >= the last border, <= EKAID_ATTN_MAX_REACH.
+ * >= the last border, <= EKAID_ATTN_MAX_REACH.  A table entry <= EKAID_ATTN_CLOSED (the lowest value of every type is) closes its distances:
+ * their keys are not attended, as with -inf.
  * lse [B][H][Lq]: log2 of the softmax denominator (+inf for an empty row); written by fwd when not NULL, read by bwd.
  * bwd writes dq, dk, dv and (table != NULL) dtable [buckets][H] of type table_dtype.  No float atomics: bit-reproducible.
  * No counterpart in the reference: its SelfAttention (modules.py:17-77) is the equal-length, unmasked, unbiased case.
@@ -695,6 +696,7 @@ long long ekaid_launch_count(int which);
 #define EKAID_F16 2
 #define EKAID_ATTN_MAX_BUCKETS 128
 #define EKAID_ATTN_MAX_REACH 1024
+#define EKAID_ATTN_CLOSED (-6e4f)
 typedef struct ekaid_attn {
     const void* q;
     const void* k;

@@ -571,3 +571,22 @@ def test_causal_rows_read_nothing_behind_the_last_position(Lq, dtype):
         for n, a, b in zip(('out', 'dq', 'dk', 'dv', 'dtable'), res[0], other):
             assert torch.equal(a, b), n
     assert (res[0][2][behind] == 0).all() and (res[0][3][behind] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize('Lq', [1, 40, 90])
+@pytest.mark.parametrize('dtype,table_dtype,low', [(F32, F32, -1e9), (F32, F32, -6e4), (F32, F32, torch.finfo(F32).min), (BF16, BF16, -1e9), (BF16, BF16, torch.finfo(BF16).min),
+                                                   (F16, F16, torch.finfo(F16).min), (F16, F32, -1e5)], ids=str)
+def test_lowest_entries_of_the_table_close_their_distances(dtype, table_dtype, low, Lq):
+    """A table with a large negative entry in place of -inf: the same results, rows that see nothing but such distances among them."""
+    B, H, KV, dh, Lk = 3, 2, 1, 64, 80
+    t = make(dtype, B, H, KV, dh, Lq, Lk, nb=8, table_dtype=table_dtype)
+    q_pos = torch.tensor([0, 400, 30])                            # the second sample's keys all lie in the farthest bucket behind
+    res = []
+    for x in (-math.inf, low):
+        t['table'][3] = x
+        res.append(run(t, H, KV, md=16, q_pos=dev(q_pos)))
+    for n, a, b in zip(('out', 'dq', 'dk', 'dv', 'dtable'), *res):
+        assert torch.isfinite(a).all() and torch.equal(a, b), n
+    for x in res[1][:4]:
+        assert (x[1] == 0).all() and not (x[2] == 0).all()
