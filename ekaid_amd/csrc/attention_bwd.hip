@@ -6,15 +6,53 @@
 
 namespace ekaid {
 
-// f16 only: powers of two that keep the score gradients P (dP - delta) inside the f16 range whatever the scale of the incoming gradient
-// (a loss divided by thousands of tokens): |dP_ij| <= |dout_i| |v_j|, so |dout_i| is brought to ~2^4.  Exact, taken out in f32.
-template <typename T> __device__ __forceinline__ float ds_scale(float norm2) {
+// f16 only: powers of two that keep the score gradients P (keep dP - delta) inside the f16 range whatever the scale of the incoming gradient
+// (a loss divided by thousands of tokens) and of the values: |dP_ij| <= |dout_i| |v_j| and |delta_i| <= inv_keep |dout_i| max |v|, so their
+// difference is at most 2 inv_keep |dout_i| max |v|, which is brought to [2^13, 2^15).  Exact, taken out in f32.
+template <typename T> __device__ __forceinline__ float ds_scale(const AttnArgs& a, float dout2, float v2) {
     if constexpr (__is_same(T, _Float16)) {
-        if (!(norm2 > 0.f) || norm2 == POS_INF) return 1.f;
-        const int e = (int)((__builtin_bit_cast(uint32_t, norm2) >> 23) & 255) - 127;      // norm^2 in [2^e, 2^(e+1))
-        const int k = 4 - (e >> 1);
-        return ldexpf(1.f, k < -60 ? -60 : k > 60 ? 60 : k);
+        const float n = dout2 * v2;                           // (f16 rows: within 2^-96 .. 2^81)
+        if (!(n > 0.f) || n == POS_INF) return 1.f;
+        const int e = (int)((__builtin_bit_cast(uint32_t, n) >> 23) & 255) - 127;          // n in [2^e, 2^(e+1))
+        return ldexpf(1.f, 13 - (e >> 1) - a.keep_exp);
     } else return 1.f;
+}
+// largest squared norm of the value rows a sample's rows may attend, by parts of the keys; one workgroup a part.  Reads the values once more:
+// 8 samples x 4 heads of 64, up to 2048 keys 5.1 us; 4 x 16 heads of 128, 2048 keys (34 MB) 9.1 us, of 346 and 680 us of whole passes
+__global__ __launch_bounds__(256) void attn_vnorm_kernel(const AttnArgs a) {
+    const ekaid_attn_t& d = a.d;
+    const int part = blockIdx.x % a.v_parts, bk = blockIdx.x / a.v_parts, b = bk % d.B, kvh = bk / d.B, tid = threadIdx.x;
+    const int len = key_len(d, b), p0 = query_pos(d, b), per = (d.Lk + a.v_parts - 1) / a.v_parts;
+    int lanes = 1;                                            // that share a row, 16 bytes each
+    while (8 * lanes < d.dh) lanes <<= 1;
+    const int col = tid % lanes * 8, step = 256 / lanes, end = min(len, (part + 1) * per);
+    const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
+    const _Float16* v = reinterpret_cast<const _Float16*>(d.v) + b * d.v_batch + (long long)kvh * d.dh + col;
+    float mx = 0.f;
+    for (int j0 = part * per; j0 < end; j0 += step) {         // (whole waves stay together for the exchange)
+        const int j = j0 + tid / lanes;
+        float s = 0.f;
+        if (j < end && col < d.dh && (!d.causal || j - d.Lq < p0) && (!mask || mask[j])) {
+            const f16x8 x = *reinterpret_cast<const f16x8*>(v + j * d.v_row);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += (float)x[e] * (float)x[e];
+        }
+        for (int o = 1; o < lanes; o <<= 1) s += __shfl_xor(s, o, 64);
+        mx = fmaxf(mx, s);
+    }
+    __shared__ float part_max[4];
+    mx = wave_max(mx);
+    if ((tid & 63) == 0) part_max[tid >> 6] = mx;
+    __syncthreads();
+    if (tid == 0) a.vn[(long long)(b * d.KV + kvh) * a.v_parts + part] = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+}
+// the largest of them for one key head, in every lane
+template <typename T> __device__ __forceinline__ float value_norm2(const AttnArgs& a, int b, int kvh, int lane) {
+    if constexpr (!__is_same(T, _Float16)) return 0.f;
+    float mx = 0.f;
+    const float* n = a.vn + (long long)(b * a.d.KV + kvh) * a.v_parts;
+    for (int x = lane; x < a.v_parts; x += 64) mx = fmaxf(mx, n[x]);
+    return wave_max(mx);
 }
 
 // dq: lane = query row.  Units of 32 keys of a tile: scores and dP of a unit, then its share of dq.  Three products a pair; bound as the
@@ -87,7 +125,7 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     const long long srow = ((long long)w.b * d.H + h) * d.Lq + i;
     const float lse = ok ? d.lse[srow] : POS_INF;
     if (ok && g == 0 && w.split == 0 && (!REL || a.splits > 1)) a.delta[srow] = delta;
-    const float rs = ds_scale<T>(n2);
+    const float rs = ds_scale<T>(a, n2, value_norm2<T>(a, w.b, w.kvh, lane));
     if constexpr (__is_same(T, _Float16)) {
         const float mx = wave_max(n2);
         if (lane == 0) red[wave] = mx;
@@ -229,7 +267,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
         float mx = 0.f;
         const float* n = a.nrm + (long long)(b * d.H + kvh * group) * a.dq_parts;
         for (int x = lane; x < group * a.dq_parts; x += 64) mx = fmaxf(mx, n[x]);
-        rs = ds_scale<T>(wave_max(mx));
+        rs = ds_scale<T>(a, wave_max(mx), value_norm2<T>(a, b, kvh, lane));
     }
     typename Blk<G>::acc dk[MT], dv[MT];
 #pragma unroll
@@ -504,7 +542,8 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const AttnArgs a, int nb
 struct BwdPlan {
     int gq, nwq, tq, sq;        // dq: block edge, waves, row tiles, splits
     int gk, nwk, tk, sk;        // dk / dv
-    size_t delta, nrm, eps, tab, po, pk, total;      // float offsets
+    size_t delta, nrm, vn, eps, tab, po, pk, total;      // float offsets
+    int v_parts;
 };
 static size_t align4(size_t n) { return (n + 3) & ~(size_t)3; }
 
@@ -533,6 +572,9 @@ static BwdPlan bwd_plan(const ekaid_attn_t* a) {
     size_t o = 0;
     p.delta = o; o += align4(rows);
     p.nrm = o; o += align4(bh * p.tq * p.sq);
+    // (value norms: some 2048 workgroups, 64 rows or more each)
+    p.v_parts = a->dtype == EKAID_F16 ? std::min(cdiv(a->Lk, 64), std::max(1, std::min(64, 2048 / std::max(1, a->B * a->KV)))) : 0;
+    p.vn = o; o += align4((size_t)a->B * a->KV * p.v_parts);
     p.eps = o; o += a->table && p.sq > 1 ? align4(rows * p.sq) : 0;
     p.tab = o; o += align4(bh * p.tk * p.sk * nb);
     p.po = o; o += p.sq > 1 ? p.sq * rows * a->dh : 0;
@@ -582,6 +624,10 @@ template <typename T> static int run_bwd(AttnArgs a, const BwdPlan& p, hipStream
     a.tiles = p.tq;
     a.splits = p.sq;
     a.dq_parts = p.tq * p.sq;
+    if (p.v_parts) {
+        hipLaunchKernelGGL(attn_vnorm_kernel, dim3(d.B * d.KV * p.v_parts), dim3(256), 0, st, a);
+        if ((rc = check_launch("attn_vnorm"))) return rc;
+    }
     if (d.table)
         rc = d.dh <= 64 ? pick_dq<T, 64, true>(a, p, st) : d.dh <= 128 ? pick_dq<T, 128, true>(a, p, st) : pick_dq<T, 256, true>(a, p, st);
     else
@@ -636,6 +682,10 @@ extern "C" int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t wor
     float* w = (float*)workspace;
     k.delta = w + p.delta;
     k.nrm = w + p.nrm;
+    k.vn = w + p.vn;
+    k.v_parts = p.v_parts;
+    (void)frexpf(k.inv_keep, &k.keep_exp);
+    if (k.inv_keep == ldexpf(1.f, k.keep_exp - 1)) --k.keep_exp;
     k.eps = w + p.eps;
     k.ptab = w + p.tab;
     k.po = w + p.po;

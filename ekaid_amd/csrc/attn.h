@@ -40,6 +40,9 @@ struct AttnArgs {
     float* pml;                       // their (max, sum) pairs
     float* delta;                     // [B][H][Lq]
     float* nrm;                       // [B * H][dq_parts]
+    float* vn;                        // [B * KV][v_parts]: largest squared norms of value rows (f16)
+    int v_parts;
+    int keep_exp;                     // smallest power of two >= inv_keep
     float* eps;                       // [splits][B][H][Lq] shares of delta's correction (split dq with a bias table)
     float* ptab;                      // [B * H][key tiles * splits][nb]
     float* pk;                        // partial dk, dv

@@ -590,3 +590,42 @@ def test_lowest_entries_of_the_table_close_their_distances(dtype, table_dtype, l
         assert torch.isfinite(a).all() and torch.equal(a, b), n
     for x in res[1][:4]:
         assert (x[1] == 0).all() and not (x[2] == 0).all()
+
+
+def f16_score_gradient_floor(t, H, KV, dh, inv_keep=1.0):
+    """What f16 score gradients lose below the normal range, in dq and dk: they are stored with 2 |dout| max |v| inv_keep brought to at least
+    2^13, so half a step is 2^-25 of a 2^13th of that."""
+    split = lambda x, n: x.double().view(x.shape[0], x.shape[1], n, dh)                 # noqa: E731
+    do, v = split(t['dout'], H).norm(dim=3).amax((1, 2)), split(t['v'], KV).norm(dim=3).amax((1, 2))
+    lost = (2.0 ** -25 * 2 * inv_keep / 2 ** 13 * do * v * dh ** -0.5)[:, None, None]
+    kq = split(t['k'], KV).abs().sum(1).repeat_interleave(H // KV, 1).flatten(1)[:, None]
+    qk = split(t['q'], H).abs().sum(1).view(-1, KV, H // KV, dh).sum(2).flatten(1)[:, None]
+    return lost * kq, lost * qk
+
+
+@gpu
+@pytest.mark.parametrize('shape', [(1, 2, 1, 256, 40, 150), (2, 2, 2, 128, 70, 90), (1, 4, 2, 64, 200, 200), (2, 2, 2, 64, 5, 33)], ids=str)
+def test_f16_values_of_thousands(shape):
+    """Values up to half of f16's range, sharp rows: the score gradients of such rows pass f16's range many times over, no gradient does."""
+    B, H, KV, dh, Lq, Lk = shape
+    t = make(F16, B, H, KV, dh, Lq, Lk, scale_out=2e-3)
+    t['q'], t['v'] = t['q'] * 4, (t['v'].float() * 7000).half()
+    vals, bnds = reference(t, H, KV, dh)
+    eq, ek = f16_score_gradient_floor(t, H, KV, dh)
+    compare(run(t, H, KV), vals, [bnds[0], bnds[1] + eq, bnds[2] + ek, bnds[3]])
+
+
+@gpu
+@pytest.mark.parametrize('p', [0.5, 0.98])
+def test_f16_dropout(p):
+    """Kept probabilities of up to fifty times their size beside values of some thirty: score gradients stay in range."""
+    from ekaid_amd import ops
+    B, H, KV, dh, Lq, Lk = 2, 4, 2, 64, 40, 90
+    t = make(F16, B, H, KV, dh, Lq, Lk, scale_out=0.05)
+    t['q'], t['v'] = t['q'] * 3, (t['v'].float() * 30).half()
+    ops.manual_seed(5)
+    keep = ops.dropout(torch.ones(B * H * Lq * Lk, device=DEV), p, True)
+    vals, bnds = reference(t, H, KV, dh, keep=keep)
+    eq, ek = f16_score_gradient_floor(t, H, KV, dh, 1 / (1 - p))
+    ops.manual_seed(5)
+    compare(run(t, H, KV, p=p, training=True), vals, [bnds[0], bnds[1] + eq, bnds[2] + ek, bnds[3]])
