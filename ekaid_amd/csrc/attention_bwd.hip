@@ -249,7 +249,8 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
     const int b = bk % d.B, kvh = bk / d.B, group = d.H / d.KV;
     const int len = key_len(d, b), p0 = query_pos(d, b), j0 = tl * NW * G, jw = j0 + wave * G, j = jw + lane % G;
     const unsigned char* mask = d.key_mask ? d.key_mask + b * d.mask_batch : nullptr;
-    const bool ok = j < len && (!d.causal || j - d.Lq < p0) && (!mask || mask[j]), live = jw < len;      // (causal: some row may attend it)
+    const int kend = d.causal ? max(0, min(len, p0 + d.Lq)) : len;                                        // keys that some row may attend
+    const bool ok = j < kend && (!mask || mask[j]), live = jw < len;
     const int qtiles = (d.Lq + QT - 1) / QT, first = d.causal ? min(qtiles, max(0, j0 - p0) / QT) : 0, run = qtiles - first;
     const int items = j0 < len ? group * run : 0, per = (items + a.splits - 1) / a.splits, t0 = split * per, t1 = min(items, t0 + per);
 
