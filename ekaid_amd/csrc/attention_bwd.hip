@@ -263,6 +263,9 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
         kf[c] = row_frag_global<T, G>(krow, c, d.dh, ok, lane);
         vf[c] = row_frag_global<T, G>(vrow, c, d.dh, ok, lane);
     }
+    // f16: probabilities enter dv's product times 2^(15 - keep_exp) (kept ones at most 2^15): one in 2^14 keys or more would be below f16's
+    // normal range.  Exact, taken out in f32.
+    const float ps = __is_same(T, _Float16) ? ldexpf(1.f, 15 - a.keep_exp) : 1.f;
     float rs = 1.f;
     if constexpr (__is_same(T, _Float16)) {                   // the largest |dout| row of the heads that share these keys
         float mx = 0.f;
@@ -402,7 +405,10 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
 #pragma unroll
             for (int x = 0; x < NB; ++x)
 #pragma unroll
-                for (int r = 0; r < 4 * nq; ++r) dp[x][r] *= rs;
+                for (int r = 0; r < 4 * nq; ++r) {
+                    dp[x][r] *= rs;
+                    s[x][r] *= ps;
+                }
         }
         u32x4 pf[PC], df[PC];
 #pragma unroll
@@ -486,7 +492,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
                 for (int c = tid; c < nbuckets; c += NT) part_of(h)[c] = 0.f;
     }
     if (j >= d.Lk) return;
-    const float f = d.scale / rs;
+    const float f = d.scale / rs, fv = 1.f / ps;
     const long long row = ((long long)b * d.Lk + j) * d.KV * d.dh + (long long)kvh * d.dh;
     const long long n = (long long)d.B * d.Lk * d.KV * d.dh;
 #pragma unroll
@@ -497,7 +503,7 @@ __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             x[e] = ok ? dk[q / nq][r + e] * f : 0.f;
-            y[e] = ok ? dv[q / nq][r + e] : 0.f;
+            y[e] = ok ? dv[q / nq][r + e] * fv : 0.f;
         }
         if (a.splits > 1) {
             store4<float>(a.pk + split * n + row + col, x[0], x[1], x[2], x[3]);

@@ -629,3 +629,19 @@ def test_f16_dropout(p):
     eq, ek = f16_score_gradient_floor(t, H, KV, dh, 1 / (1 - p))
     ops.manual_seed(5)
     compare(run(t, H, KV, p=p, training=True), vals, [bnds[0], bnds[1] + eq, bnds[2] + ek, bnds[3]])
+
+
+@gpu
+def test_f16_value_gradients_of_many_keys():
+    """818400 equal keys: a probability of 1.2e-6 lies between two of f16's smallest numbers.  Every score is exactly 0, every power 1 and
+    the sum exact, so a value's gradient is sum_i dout_i / 818400: rounding of the probability (h), of the result (h), 24 f32 additions and a
+    logarithm of 20 in f32 (2^-24 * 20, twice)."""
+    from ekaid_amd import ops
+    Lk, Lq, dh = 818400, 24, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q = torch.zeros(1, Lq, dh, device=DEV, dtype=F16, requires_grad=True)
+    k, v = (torch.rand(1, Lk, dh, generator=g, device=DEV).half().requires_grad_(True) for _ in range(2))
+    dout = (torch.rand(1, Lq, dh, generator=g, device=DEV) * 200 + 100).half()
+    (dv,) = torch.autograd.grad(ops.cross_attention(q, k, v, 1), [v], dout)
+    want = dout.double().sum(1, keepdim=True) / Lk
+    assert float(((dv.double() - want).abs() / want).max()) <= 2 * 2.0 ** -11 + (24 + 2 * 20 + 10) * 2.0 ** -24
