@@ -11,7 +11,7 @@ __device__ __forceinline__ void drop_scores(const AttnArgs& a, typename Blk<G>::
 #pragma unroll
     for (int q = 0; q < NB * nq; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[q / nq][4 * (q % nq) + e] *= drop_keep(a, seed, b, h, i, j0 + 4 * ng * q + 4 * (lane / G) + e);
+        for (int e = 0; e < 4; ++e) s[q / nq][4 * (q % nq) + e] *= drop_kept(a, seed, b, h, i, j0 + 4 * ng * q + 4 * (lane / G) + e);
 }
 
 template <typename T, int DH, int G>
@@ -37,7 +37,7 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const RowWork& w, 
         }
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : a.inv_keep / l;
     T* p = reinterpret_cast<T*>(a.d.out) + ((long long)w.b * a.d.Lq + i) * a.d.H * a.d.dh + (long long)h * a.d.dh;
 #pragma unroll
     for (int q = 0; q < DH / G * nq; ++q) {
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_f
             for (int e = 0; e < 4; ++e) {
                 s[b][e] = __builtin_amdgcn_exp2f(s[b][e] - base);
                 l += s[b][e];
-                if (d.drop_p > 0.f) s[b][e] *= drop_keep(a, seed, w.b, h, i, t * KB + 16 * b + 4 * g + e);
+                if (d.drop_p > 0.f) s[b][e] *= drop_kept(a, seed, w.b, h, i, t * KB + 16 * b + 4 * g + e);
             }
         if (__any(alpha != 1.f)) {
 #pragma unroll
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * DH >= 512 ? 1 : 2) void attn_f
     const float base = M == NEG_INF ? 0.f : M;
 #pragma unroll
     for (int k = 0; k < NW; ++k) sum += sml[k][1][n] * __builtin_amdgcn_exp2f(sml[k][0][n] - base);
-    const float f = __builtin_amdgcn_exp2f(m - base) * (a.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum);
+    const float f = __builtin_amdgcn_exp2f(m - base) * (a.splits > 1 ? 1.f : sum == 0.f ? 0.f : a.inv_keep / sum);
     const long long row = ((long long)w.b * d.H + h) * d.Lq + i, total = (long long)d.B * d.H * d.Lq;
     if (ok) {
         float* p = join + (wave * rows + n) * DH;
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     float l = 0.f;
     for (int s = lane; s < a.splits; s += 64) l += a.pml[2 * (s * rows + row) + 1] * __builtin_amdgcn_exp2f(a.pml[2 * (s * rows + row)] - base);
     l = wave_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : a.inv_keep / l;
     const long long i = row % d.Lq, bh = row / d.Lq;
     T* out = reinterpret_cast<T*>(d.out) + ((bh / d.H) * d.Lq + i) * d.H * d.dh + (bh % d.H) * d.dh;
     for (int c = 4 * lane; c < d.dh; c += 256) {

@@ -344,6 +344,11 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+// the forward's: 1 or 0 -- the factor of what is kept joins the division by the sum, so that f16 holds the probabilities whatever it is
+__device__ __forceinline__ float drop_kept(const AttnArgs& a, uint64_t seed, int b, int h, int i, int j) {
+    const uint64_t idx = (((uint64_t)b * a.d.H + h) * a.d.Lq + i) * (uint64_t)a.d.Lk + j;
+    return dropout_scale(seed, idx, a.d.drop_p, 1.f);
+}
 __device__ __forceinline__ float drop_keep(const AttnArgs& a, uint64_t seed, int b, int h, int i, int j) {
     const uint64_t idx = (((uint64_t)b * a.d.H + h) * a.d.Lq + i) * (uint64_t)a.d.Lk + j;
     return dropout_scale(seed, idx, a.d.drop_p, a.inv_keep);

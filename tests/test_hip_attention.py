@@ -645,3 +645,25 @@ def test_f16_value_gradients_of_many_keys():
     (dv,) = torch.autograd.grad(ops.cross_attention(q, k, v, 1), [v], dout)
     want = dout.double().sum(1, keepdim=True) / Lk
     assert float(((dv.double() - want).abs() / want).max()) <= 2 * 2.0 ** -11 + (24 + 2 * 20 + 10) * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize('shape', [(1, 16, 16, 32, 64, 1024), (8, 16, 16, 32, 1, 8192)], ids=str)
+def test_f16_dropout_that_keeps_almost_nothing(shape):
+    """One probability in 2^17 is kept, 2^17 times its size, which f16 does not hold; output and gradients it holds."""
+    from ekaid_amd import ops
+    B, H, KV, dh, Lq, Lk = shape
+    p = 1 - 2.0 ** -17
+    t = make(F16, B, H, KV, dh, Lq, Lk, scale_out=0.05)
+    t['q'], t['v'] = t['q'] * 0.25, (t['v'].float() * 0.1).half()
+    seed = 0
+    while True:
+        ops.manual_seed(seed)
+        keep = ops.dropout(torch.ones(B * H * Lq * Lk, device=DEV), p, True)
+        if int((keep != 0).sum()) >= 4:
+            break
+        seed += 1
+    vals, bnds = reference(t, H, KV, dh, keep=keep)
+    eq, ek = f16_score_gradient_floor(t, H, KV, dh, 2.0 ** 17)
+    ops.manual_seed(seed)
+    compare(run(t, H, KV, p=p, training=True), vals, [bnds[0], bnds[1] + eq, bnds[2] + ek, bnds[3]])
