@@ -405,7 +405,9 @@ int attn_check(const ekaid_attn_t* a, const char* who) {
         for (int i = 0; i < a->n_border; ++i)
             if (a->border[i] < (i ? a->border[i - 1] : 1)) { set_error("%s: borders must not descend, from 1 on", who); return EKAID_ERR_ARG; }
     }
-    if ((long long)a->B * a->H * ((long long)a->Lq + a->Lk + 64) > (1ll << 33) || (long long)a->B * a->H > (1 << 24)) {
+    // a launch counts its threads in 32 bits: 256 a head of up to 16 rows, four a row or key, 64 a table entry
+    const long long bh = (long long)a->B * a->H;
+    if (bh >= (1 << 24) || bh * ((long long)std::max(a->Lq, a->Lk) + 128) >= (1ll << 30) || (a->table && a->H >= (1 << 18))) {
         set_error("%s: too many rows for one launch", who);
         return EKAID_ERR_UNSUPPORTED;
     }

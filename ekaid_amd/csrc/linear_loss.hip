@@ -1195,6 +1195,12 @@ __global__ __launch_bounds__(256) void ll_narrow_sum_kernel(const ekaid_linear_l
 }
 
 // ---- host side
+// f32 as 16-bit terms through the tile kernels (below 2^31 products of a matrix the few tiles are bound by latency, and ekaid_gemm_f32 with
+// its splits is level or ahead)
+bool as_terms(const ekaid_linear_loss_t* a) {
+    return a->dtype == EKAID_F32 && a->arith == EKAID_GEMM_F16X2 && (double)a->B * a->T * a->V * a->D >= 2147483648.0 && a->D % 8 == 0 && a->ldx % 4 == 0 &&
+           !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
+}
 int ll_check(const ekaid_linear_loss_t* a, const char* who) {
     if (!a) { set_error("%s: null descriptor", who); return EKAID_ERR_ARG; }
     if (a->dtype < EKAID_F32 || a->dtype > EKAID_F16) { set_error("%s: dtype %d", who, a->dtype); return EKAID_ERR_ARG; }
@@ -1203,6 +1209,13 @@ int ll_check(const ekaid_linear_loss_t* a, const char* who) {
         return EKAID_ERR_ARG;
     }
     if (a->dtype == EKAID_F32 && (a->arith < EKAID_GEMM_F32_MFMA || a->arith > EKAID_GEMM_F16X2)) { set_error("%s: arithmetic %d", who, a->arith); return EKAID_ERR_ARG; }
+    // a launch counts its threads in 32 bits: 64 a row (f32; as terms also a word) or 16, 512 a tile of 256 x 256
+    const long long n = (long long)a->B * a->T;
+    const bool f32 = a->dtype == EKAID_F32, terms = as_terms(a);
+    if ((f32 ? n + (terms ? a->V : 0) : n / 4) > (1 << 26) - 512 || ((!f32 || terms) && (n + 255) / 256 * ((a->V + 255ll) / 256) >= (1 << 23))) {
+        set_error("%s: %lld rows and %d words are too many for one launch", who, n, a->V);
+        return EKAID_ERR_UNSUPPORTED;
+    }
     const int al = a->dtype == EKAID_F32 ? 4 : 16;
     if ((uintptr_t)a->state & 15) { set_error("%s: the state must be 16-byte aligned", who); return EKAID_ERR_ARG; }
     if (a->dtype != EKAID_F32 && (a->D % 8 || a->ldx % 8)) { set_error("%s: width %d / row stride %lld must be multiples of 8", who, a->D, a->ldx); return EKAID_ERR_UNSUPPORTED; }
@@ -1267,8 +1280,7 @@ LossPlan loss_plan(const ekaid_linear_loss_t* a, int backward) {
         p.total = o;
         return p;
     }
-    // (below 2^31 products of a matrix the few tiles are bound by latency, and ekaid_gemm_f32 with its splits is level or ahead)
-    p.terms = a->dtype == EKAID_F32 && a->arith == EKAID_GEMM_F16X2 && (double)p.n * a->V * a->D >= 2147483648.0 && a->D % 8 == 0 && a->ldx % 4 == 0 && !(((uintptr_t)a->x | (uintptr_t)a->weight) & 15);
+    p.terms = as_terms(a);
     if (a->dtype == EKAID_F32 && !p.terms) {
         long long vp = (long long)(PIECE_BYTES / 4) / std::max(1ll, p.n);
         vp = std::max(256ll, vp & ~255ll);

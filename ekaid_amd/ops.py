@@ -1951,7 +1951,8 @@ def linear_lm_loss(x, weight, bias, target, mask, denom=None):
     (V,) or None, of one type (float32, bfloat16, float16; 16-bit: D a multiple of 8); target (B, >= T) int64 and mask (B, >= T) float32
     as ``lm_loss`` takes them, mask values weigh their rows.  The vocabulary is taken in pieces and the logits are formed again in the
     backward (float32 with at most 256 words: kept, where they are no larger than x).  Rows with mask 0 add nothing and get zero gradients whatever x and target hold there; a target outside the vocabulary in
-    a row that counts makes the loss NaN; an all-zero mask gives 0 / 0 (as ``lm_loss``) with zero gradients."""
+    a row that counts makes the loss NaN; an all-zero mask gives 0 / 0 (as ``lm_loss``) with zero gradients.  Some 2^28 rows (float32 2^26) and
+    2^39 logits are the most a call takes."""
     require_cuda(x, weight, bias, target, mask, denom)
 
     def refuse(msg, *args):

@@ -679,8 +679,8 @@ long long ekaid_launch_count(int which);
  * gradients 0.  Masked key and value rows, and (causal) those behind the last row's position, are never read into a product (NaN there
  * stays there; a key that some row attends meets the rows before it with the weight 0, so NaN in it reaches them).  Scores are never stored.
  * q [B][Lq][H dh], k and v [B][Lk][KV dh]: strides between samples and rows in elements, heads dh apart, all 16-byte aligned;
- * out, dout, dq [B][Lq][H dh] and dk, dv [B][Lk][KV dh] contiguous.  H % KV == 0, dh % 8 == 0, dh <= 256.  dtype: EKAID_F32 / BF16 / F16
- * of every tensor but lse, table; products accumulate and softmax statistics are held in f32; probabilities and score gradients are
+ * out, dout, dq [B][Lq][H dh] and dk, dv [B][Lk][KV dh] contiguous.  H % KV == 0, dh % 8 == 0, dh <= 256;
+ * B H < 2^24, B H (max(Lq, Lk) + 128) < 2^30, with a table H < 2^18 (a launch's threads).  dtype: EKAID_F32 / BF16 / F16 of every tensor but lse, table; products accumulate and softmax statistics are held in f32; probabilities and score gradients are
  * rounded to the tensors' type where they enter a matrix product.  Dropout multiplies the probabilities, mask index
  * ((b H + h) Lq + i) Lk + j.
  * Relative bias (table != NULL): table [buckets][H]; bucket of a distance = number of `border` entries <= distance (n_border of them,
@@ -745,6 +745,7 @@ int ekaid_attn_bwd(const ekaid_attn_t* a, void* workspace, size_t workspace_byte
  * f16 terms with row scales for z and dx and the exact three bf16 terms for dweight (EKAID_GEMM_F16X2, N V D >= 2^31, D % 8 == 0 and
  * 16-byte aligned x, weight), else as ekaid_gemm_f32.  16-bit
  * products accumulate in f32, logit gradients are rounded to the type (scaled by an exact power of two) where they enter a product.  No float atomics.
+ * Rows and words: up to 2^28, f32 2^26 rows (terms: rows and words together); 16 bits and terms: 2^23 tiles of 256 x 256 (a launch's threads).
  * ref: DynamicSpeaker.logit + log_softmax (dynamic_speaker_change_pos.py:163,238) + LanguageModelCriterion (utils/utils.py:204-216).
  * ------------------------------------------------------------------------------------------ */
 typedef struct ekaid_linear_loss {

@@ -667,3 +667,20 @@ def test_f16_dropout_that_keeps_almost_nothing(shape):
     eq, ek = f16_score_gradient_floor(t, H, KV, dh, 2.0 ** 17)
     ops.manual_seed(seed)
     compare(run(t, H, KV, p=p, training=True), vals, [bnds[0], bnds[1] + eq, bnds[2] + ek, bnds[3]])
+
+
+def test_c_entry_refuses_more_threads_than_a_launch_counts():
+    from ekaid_amd import hip
+    L = hip.load()
+    for kw in (dict(B=1 << 12, H=1 << 12), dict(B=1 << 10, H=64, Lq=1 << 14), dict(B=1 << 10, H=64, Lk=1 << 14), dict(B=1, H=1 << 18, table=1 << 20, reach=9)):
+        d = hip.Attn()
+        d.q = d.k = d.v = d.out = d.dout = d.lse = d.dq = d.dk = d.dv = d.dtable = 1 << 20
+        d.B, d.H, d.KV, d.dh, d.Lq, d.Lk, d.scale = 2, 1, 1, 8, 1, 1, 1.0
+        for n, x in kw.items():
+            setattr(d, n, x)
+        d.KV = d.H
+        for entry in (L.ekaid_attn_fwd, L.ekaid_attn_bwd):
+            assert entry(ctypes.byref(d), 1 << 20, 1 << 50, None) < 0 and 'too many' in hip.last_error(), kw
+        assert L.ekaid_attn_workspace_bytes(ctypes.byref(d), 0) == 0
+        d.B, d.H, d.KV, d.Lq, d.Lk = 1, max(1, d.H >> 2), max(1, d.H >> 2), max(1, d.Lq >> 2), max(1, d.Lk >> 2)
+        assert L.ekaid_attn_workspace_bytes(ctypes.byref(d), 1) > 0, kw

@@ -562,3 +562,22 @@ def test_operands_are_copied_only_where_it_helps():
         loss = ops.linear_lm_loss(x, w, None, t['target'], t['mask'])
         assert (loss.grad_fn.saved_tensors[0].data_ptr() == x.data_ptr()) == kept
         assert torch.equal(loss.detach(), ops.linear_lm_loss(x.clone(memory_format=torch.contiguous_format), w, None, t['target'], t['mask']).detach())
+
+
+def test_c_entry_refuses_more_threads_than_a_launch_counts():
+    from ekaid_amd import hip
+    L = hip.load()
+
+    def desc(dtype, n, V, D=64, arith=2):
+        d = hip.LinearLoss()
+        for name in ('x', 'weight', 'target', 'mask', 'loss', 'state', 'dloss', 'dx', 'dweight'):
+            setattr(d, name, 1 << 20)
+        d.dtype, d.B, d.T, d.D, d.V, d.ldx, d.ld_target, d.ld_mask, d.arith = dtype, 1, n, D, V, D, n, n, arith
+        return d
+    for case in ((0, 1 << 26, 1), (0, 1 << 25, 1 << 25), (0, 1 << 20, 1 << 19), (1, 1 << 20, 1 << 19), (2, 1 << 28, 1)):
+        d = desc(*case)
+        for entry in (L.ekaid_linear_loss_fwd, L.ekaid_linear_loss_bwd):
+            assert entry(ctypes.byref(d), 1 << 20, 1 << 60, None) < 0 and 'too many' in hip.last_error(), case
+        assert L.ekaid_linear_loss_state_bytes(ctypes.byref(d)) == 0
+    for case in ((0, 1 << 25, 1), (0, 1 << 20, 1 << 19, 64, 0), (0, 1 << 19, 1 << 19), (1, 1 << 19, 1 << 19), (2, 1 << 27, 1)):
+        assert L.ekaid_linear_loss_state_bytes(ctypes.byref(desc(*case))) > 0, case
