@@ -228,9 +228,11 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
 }
 
 // dk, dv: lane = key; the rows of every head that shares it go by in tiles, in units of 32.  What a lane without a valid key computes stays in
-// that lane and is replaced by zero at the end.  Four products a pair.  The same shapes as at dq: 159 us, 600 TF, and 332 us, 410 TF -- with
-// 128-wide heads a block of 32 keys would leave one wave a SIMD its registers, so blocks of 16 read LDS twice as often, and a unit waits
-// for the fences around its diagonal sums.
+// that lane and is replaced by zero at the end.  Four products a pair.  The same shapes as at dq: 159 us, 600 TF, and 335 us, 410 TF.
+// 64 wide no unit is full (vector 38 %, matrix 35 %, LDS 26 % of a busy compute unit's cycles): one round of 512 workgroups, two a compute
+// unit and two waves a SIMD, near a third of them on keys behind their sample's length.  128 wide a block of 32 keys would leave one wave a
+// SIMD its registers, so blocks of 16 read LDS twice as often; 41 % of the wave time is waiting (vector 31 %, matrix 20 %, LDS 26 %).  The
+// table's sums, met by the 15 % of the pairs within the reach, cost it their LDS, registers and fences: 275 us without a table.
 template <typename T, int DH, int G, int NW, int QT, bool REL>
 __global__ __launch_bounds__(64 * NW, DH * (int)sizeof(T) * G > 4096 ? 1 : G == 16 && sizeof(T) == 2 && !(REL && DH > 64) ? 3 : 2) void attn_dkv_kernel(const AttnArgs a) {
     constexpr int NT = 64 * NW, U = QT < 32 ? QT : 32, NB = U / G, NC = DH / (Elem<T>::epl * Blk<G>::ng), PC = U / (Elem<T>::epl * Blk<G>::ng), MT = DH / G;

@@ -410,9 +410,10 @@ __device__ __forceinline__ Affine scores_by_row(const AttnArgs& a, typename Blk<
 
 // one workgroup's share of the forward / dq work list.  Order: tile, split, heads that share keys, `near` key heads, sample, the other key
 // heads -- what shares keys is together on a die, and every die sees many samples (dealt sample by sample, the die of the longest one
-// finishes last: 8 ragged samples in training 103 -> 89 us).  near = 4 for few query rows over short states, where latency is the bound
-// and neighbouring heads share pages (64 x 4 heads over 104 f32 states: 16 us, 27 with near = 1), else 1 (32 x 16 heads over a cache of
-// 4096: 83 us, 94 with near = 4).
+// finishes last: 8 ragged samples in training 103 -> 89 us).  near = 4 for few query rows over up to 512 states, where neighbouring heads share
+// pages (64 x 4 heads over 104 f32 states held in the caches: 16 us, 27 with near = 1), else 1 (32 x 16 heads over a cache of 4096: 83 us,
+// 94 with near = 4).  Both sides of the border, near = 4 / 1, us, states out of the caches: 64 x 4 heads of 256 f32 over 256 states 33.8 / 36.4,
+// 512 58.5 / 60.1, 1024 105.2 / 104.4, 2048 192 / 183; 64 x 16 heads of 64 bf16 over 512 31.9 / 32.9, 1024 59.6 / 57.4, 2048 113 / 100.
 struct RowWork {
     int b, head0, kvh, tile, split;
     __device__ __forceinline__ RowWork(const AttnArgs& a) {

@@ -1,13 +1,17 @@
 // Vocabulary loss of a linear layer without its logits, and its gradient (include/ekaid_hip.h: ekaid_linear_loss_t).
 //
-// 16-bit types: the rows that count (mask != 0) are listed once; products run on tiles of 256 x 256 x 64 (128 x 128 x 64 when the grid
-// would not fill the chip), operands copied to LDS without passing registers, one tile ahead of the matrix instructions.
+// 16-bit types: the rows that count (mask != 0) are listed once; products run on tiles of 256 x 256 x 64 (128 x 128 x 64 where
+// there are fewer than 128 of them), operands copied to LDS without passing registers, one tile ahead of the matrix instructions.
 //   forward   z^T = W x^T per tile -> per-row maximum and sum of the tile's words; a second small kernel joins the tiles
 //   backward  per piece of the vocabulary: z again -> dz = (softmax - onehot) mask, rounded to the type, and the bias partials;
 //             dW = dz^T x;  dx partials += dz W.   Three products where the formula has three, one more than if logits were kept: at width D
-//             forming z again costs 2 D flops a logit, reading a kept f32 one and writing it 8 bytes.
+//             forming z again costs 2 D flops a logit, keeping it in f32 8 bytes of traffic -- at 1120 TF and 4.74 TB/s as long from a width
+//             of some 950 on, beyond it forming it again is the price of holding no logits (at 2048 2.6 ms of 11.9 below, against 1.2).
 // Bound by the matrix instructions and the barrier of each 64-deep tile: 11008 counting rows x 2048 x 65536 bf16: statistics 2.64 ms (1120 TF),
-// dz 3.14 (940, it writes 1.4 GB of logit gradients), dW 2.71 (1090), dx 3.49 (850, f32 partials of 16 shares joined by a pass).
+// dz 3.14 (940, it writes 1.4 GB of logit gradients), dW 2.71 (1090), dx 3.49 (850: 688 workgroups, 344 tiles x 2 shares, are 2.7 rounds of 256,
+// and f32 partials are read and written once a piece).
+// Memory beside the operands: 16-bit dz of a piece of the vocabulary, up to 512 MB (f32: 10 bytes a logit, as five 16-bit planes), up to 16
+// f32 partials of dx within 512 MB, and of dW where its tiles are few.
 // f32: the same kernels on 16-bit terms of the operands; few words: ll_narrow_*; other arithmetics and small products: passes around
 // ekaid_gemm_f32.
 #include "common.h"
@@ -1312,6 +1316,9 @@ LossPlan loss_plan(const ekaid_linear_loss_t* a, int backward) {
         p.total = o;
         return p;
     }
+    // Tiles of 256 x 256 from half a round of the chip on, counted with all rows (how many count is known on the device alone).  128 / 256 wide,
+    // us, forward and gradients, every row counting: f32 1024 x 1024 x 4096 (64 tiles) 325 / 398, x 7936 (124) 585 / 493, 2048 x 1024 x 8192
+    // (256) 1093 / 695; bf16 1024 x 1024 x 4096 117 / 166 or more (host-bound), x 8192 (128) 182 / 182, 2048 x 1024 x 8192 316 / 220.
     p.big = (p.nr / 256) * (long long)cdiv(a->V, 256) >= 128;
     const int bt = p.big ? 256 : 128;
     if (p.terms) {

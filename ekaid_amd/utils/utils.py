@@ -132,8 +132,9 @@ class LanguageModelCriterion(nn.Module):
 
 
 class LinearLanguageModelCriterion(nn.Module):
-    """``LanguageModelCriterion`` of ``log_softmax(layer(hidden))`` for a large vocabulary: the logits are never kept
-    (``ops.linear_lm_loss``).  ``layer``: a Linear (``DynamicSpeaker.logit``); ``hidden``: its (B, T, D) input."""
+    """``LanguageModelCriterion`` of ``log_softmax(layer(hidden))`` for a large vocabulary (``ops.linear_lm_loss``): for a decoder of the
+    caller's own that hands over its (B, T, D) states ``hidden`` and its vocabulary layer ``layer`` (a Linear: ``weight`` (V, D), ``bias``);
+    ``DynamicSpeaker`` takes the logarithms itself and stays with ``LanguageModelCriterion``."""
 
     def forward(self, hidden, layer, target, mask, denom=None):
         if mask.dtype != torch.float32:
