@@ -124,6 +124,8 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
     n2 = across_groups_sum<G>(n2);
     const long long srow = ((long long)w.b * d.H + h) * d.Lq + i;
     const float lse = ok ? d.lse[srow] : POS_INF;
+    const bool empty = lse == POS_INF;                        // a row without any key: zeros, whatever dout holds there
+    if (empty) delta = 0.f;
     if (ok && g == 0 && w.split == 0 && (!REL || a.splits > 1)) a.delta[srow] = delta;
     const float rs = ds_scale<T>(a, n2, value_norm2<T>(a, w.b, w.kvh, lane));
     if constexpr (__is_same(T, _Float16)) {
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
         if (t + 1 < t1) tile(t + 1, k1, v1, k0, v0);
     }
     if constexpr (REL) {
-        rowsum = across_groups_sum<G>(rowsum);
+        rowsum = empty ? 0.f : across_groups_sum<G>(rowsum);
         if (ok && g == 0) {
             if (a.splits > 1) a.eps[(long long)w.split * d.B * d.H * d.Lq + srow] = rowsum;
             else a.delta[srow] = delta + rowsum;
@@ -220,10 +222,12 @@ __global__ __launch_bounds__(64 * NW, G == 32 && DH * (int)sizeof(T) > 256 ? 1 :
 #pragma unroll
     for (int q = 0; q < MT * nq; ++q) {
         const int col = 4 * ng * q + 4 * g, r = 4 * (q % nq);
-        const auto& x = o[q / nq];
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = empty ? 0.f : o[q / nq][r + e] * f;
         if (col >= d.dh) continue;
-        if (a.splits > 1) store4<float>(part + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
-        else store4<T>(out + col, x[r] * f, x[r + 1] * f, x[r + 2] * f, x[r + 3] * f);
+        if (a.splits > 1) store4<float>(part + col, x[0], x[1], x[2], x[3]);
+        else store4<T>(out + col, x[0], x[1], x[2], x[3]);
     }
 }
 

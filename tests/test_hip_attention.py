@@ -684,3 +684,24 @@ def test_c_entry_refuses_more_threads_than_a_launch_counts():
         assert L.ekaid_attn_workspace_bytes(ctypes.byref(d), 0) == 0
         d.B, d.H, d.KV, d.Lq, d.Lk = 1, max(1, d.H >> 2), max(1, d.H >> 2), max(1, d.Lq >> 2), max(1, d.Lk >> 2)
         assert L.ekaid_attn_workspace_bytes(ctypes.byref(d), 1) > 0, kw
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('Lq', [1, 20, 70, 130])
+def test_gradients_of_samples_without_states_are_zero_whatever_comes_in(Lq, dtype):
+    """Two samples attend nothing, by their length and by their mask, and NaN and Inf come in for them: zeros there, nothing changes elsewhere."""
+    B, H, KV, dh, Lk = 4, 4, 2, 64, 150
+    t = make(dtype, B, H, KV, dh, Lq, Lk, nb=16)
+    k_len, mask = torch.tensor([150, 0, 100, 150]), torch.ones(B, Lk, dtype=torch.bool)
+    mask[2] = False
+    res = []
+    for bad in (0.0, float('nan'), float('inf')):
+        t['dout'][1:3] = bad
+        res.append([run(t, H, KV, md=30, k_len=dev(k_len), key_mask=dev(mask)), run({n: x for n, x in t.items() if n != 'table'}, H, KV, k_len=dev(k_len), key_mask=dev(mask))])
+    for other in res[1:]:
+        for a, b in zip(res[0], other):
+            for n, x, y in zip(('out', 'dq', 'dk', 'dv', 'dtable'), a, b):
+                assert torch.equal(x, y), n
+            for x in b[:4]:
+                assert (x[1:3] == 0).all()
